@@ -22,8 +22,9 @@ _orc = None
 
 def reference_root():
     """The reference source tree: $KRAFLA_REF, else the `reference_path` of the
-    repository's BASELINE.json; None when neither names a directory here (as
-    on a machine without the reference, where the prebuilt oracle/_ref is used)."""
+    repository's BASELINE.json; None when neither names the tree here (as on
+    a machine without the reference, or with an empty folder in its place, where
+    the prebuilt oracle/_ref is used)."""
     root = os.environ.get("KRAFLA_REF")
     if not root:
         try:
@@ -32,7 +33,7 @@ def reference_root():
                 root = json.load(f).get("reference_path")
         except (OSError, ValueError):
             root = None
-    return root if root and os.path.isdir(root) else None
+    return root if root and os.path.isfile(os.path.join(root, "Makefile")) else None
 
 
 def build(ref_root=None):
