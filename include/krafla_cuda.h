@@ -260,8 +260,9 @@ void kc_dev_free(void *p);
 int kc_memcpy_htod(void *dst, const void *src, size_t bytes);
 int kc_memcpy_dtoh(void *dst, const void *src, size_t bytes);
 /* Waits for the current device. KC_E_IO when a kernel-level matvec call
- * (kc_matvec_dev, kc_matvec_f32_noalloc) on it had a device wait give up
- * since the last kc_dev_sync (its error word is then cleared). */
+ * (kc_matvec_dev, kc_matvec_f32_noalloc) on it had a device wait give up, or a
+ * serving operator skipped something out of range, since the last kc_dev_sync
+ * (the error words are then cleared). */
 int kc_dev_sync(void);
 /* Diagnostics for tests of the error path: the polls of the kernel-level
  * matvec's first wait on each chunk of weights (0: it gives up at once;
@@ -275,6 +276,113 @@ int kc_debug_wait_limit(int polls);
  * with blocks split between CTAs. Returns the previous mode. No reference
  * counterpart. */
 int kc_debug_ffn_split(int mode);
+
+/* ---- several sequences at once: a paged KV cache, and a batch's logits ----
+ *
+ * Operators for a caller that serves many sequences with its own loop, on
+ * device pointers of the current device and asynchronous on `stream` (NULL: the
+ * default stream); capturable into a CUDA graph after a first call outside one.
+ * No counterpart in the reference, whose cache is one sequence's.
+ *
+ * Sizes and pointers are checked on the host (KC_E_SHAPE with a message: NULL,
+ * host memory, another device's memory, alignment, strides). Page numbers,
+ * lengths, positions and offsets lie in device memory: the kernels skip what is
+ * out of range, and the next kc_dev_sync returns KC_E_IO and says what it was. */
+
+/* A pool of pages and the table that says which page holds which positions:
+ * position p of sequence s is slot p % page_size of page
+ * table[s * ld_table + p / page_size]. Row (page, kv head, slot) of k and v
+ * holds head_dim values of kv_type (KC_F32, KC_F16, KC_Q8_0: int8 with the
+ * scales kd and vd, one for each row). Entries of the table beyond a
+ * sequence's length are not read, slots beyond it may hold anything. */
+typedef struct {
+    void *k, *v;                 /* [n_pages][n_kv_heads][page_size][head_dim], 16-byte aligned */
+    float *kd, *vd;              /* KC_Q8_0: [n_pages][n_kv_heads][page_size]; else NULL */
+    const int *table;            /* [n_seqs][ld_table] */
+    int n_seqs, ld_table;
+    int n_pages, page_size, n_kv_heads;
+    int head_dim;                /* a multiple of 16, 16..256 */
+    int kv_type;
+} kc_paged_kv;
+
+/* The rotation tables of a model on the host, [n_pos][head_dim / 2] each, as
+ * kc_state_init makes them for its max_seq positions (with the header's RoPE
+ * scaling; local: the tables of the layers with rope_local_theta). */
+int kc_rope_tables(const kc_config *cfg, int n_pos, int local, float *cos_out, float *sin_out);
+
+/* Rows of new tokens: the norm of every query and key head (q_norm and k_norm,
+ * [head_dim] each; both NULL: none), x / sqrt(mean(x^2) + eps) * w, the rotation
+ * of adjacent pairs at the row's position (cos and sin [n_pos][head_dim / 2],
+ * the tables of kc_rope_tables), queries to q_out, keys and values into the
+ * cache in its type (8-bit rows by the rule of the model's cache). Row i goes
+ * to position pos[i] of sequence seqs[i] (seqs NULL: of sequence i); a negative
+ * sequence is padding: nothing is written for it. q, k, v: rows of n_heads,
+ * n_kv_heads, n_kv_heads heads, ld* floats apart (multiples of 4; views of one
+ * q|k|v matrix will do), 16-byte aligned. q_out may be q. Two rows of one
+ * call that name the same position leave either's values there, value by
+ * value. */
+typedef struct {
+    const float *q, *k, *v;
+    float *q_out;
+    long long ldq, ldk, ldv, ldo;
+    const float *cos, *sin;
+    const float *q_norm, *k_norm;
+    const int *seqs, *pos;       /* [rows] */
+    int rows, n_heads, n_pos;
+    float eps;
+} kc_append_args;
+int kc_paged_append_dev(const kc_paged_kv *kv, const kc_append_args *args, void *stream);
+
+/* The attention of one new token for each of the first n_seqs sequences: query
+ * row i (n_heads heads, heads h * n_kv_heads / n_heads sharing a KV head)
+ * against positions max(0, lens[i] - window) .. lens[i] - 1 (window 0: from 0)
+ * of sequence i. scores q . k * scale, through softcap * tanh(score / softcap)
+ * when softcap > 0; an 8-bit cache takes the query quantized per head, as the
+ * model's does. A sequence of length 0 gets zeros. The sums of a row do not
+ * depend on what else is running, but how a row is cut into pieces depends on
+ * the other rows' lengths: results of different batches differ by float
+ * rounding. ws: at least kc_paged_attend_ws bytes of scratch, 16-byte aligned,
+ * not initialised; calls (or replayed graphs) that may overlap in time need one
+ * each. */
+typedef struct {
+    const float *q;
+    float *out;
+    long long ldq, ldo;          /* floats between rows, multiples of 4 */
+    const int *lens;             /* [n_seqs] */
+    int n_seqs, n_heads, window;
+    float scale, softcap;
+    void *ws;
+    size_t ws_bytes;
+} kc_attend_args;
+int kc_paged_attend_dev(const kc_paged_kv *kv, const kc_attend_args *args, void *stream);
+int kc_paged_attend_ws(const kc_paged_kv *kv, int n_heads, size_t *bytes);
+
+/* Logits before a token is chosen, rows [vocab] of in to out (out may be in):
+ * with c the times that token v is in the row's history,
+ *   c > 0: z = z > 0 ? z / repeat : z * repeat (the sampler's penalty,
+ *          model/sampler.c:30-42), then z -= frequency * c, z -= presence;
+ *   z += the bias that the row's list gives v (its last entry for v counts);
+ *   z = -inf where the row's mask does not allow v.
+ * history [rows][ld_history], the first history_len[i] (NULL: history_cap) of
+ * row i; tokens outside 0..vocab-1 are ignored, there and in bias_ids. repeat,
+ * presence, frequency: one value per row (each may be NULL: off). Biases: row
+ * i's entries are bias_off[i] .. bias_off[i + 1] - 1 of bias_ids and bias_vals
+ * (n_bias entries). mask [rows][ld_mask] words, bit v % 32 of word v / 32 set:
+ * allowed. A row that allows nothing is all -inf. */
+typedef struct {
+    const float *in;
+    float *out;
+    long long ld_in, ld_out;
+    const int *history, *history_len;
+    long long ld_history;
+    const float *repeat, *presence, *frequency;
+    const int *bias_off, *bias_ids;
+    const float *bias_vals;
+    const uint32_t *mask;
+    long long ld_mask;
+    int rows, vocab, history_cap, n_bias;
+} kc_logits_args;
+int kc_logits_process_dev(const kc_logits_args *args, void *stream);
 
 #ifdef __cplusplus
 }

@@ -50,6 +50,10 @@ struct DevLayer {
     int window = 0, local_rope = 0;
 };
 
+/* The serving kernels' error word on a device (NULL before their first use there) and what its bits say (kc_serve.cu). */
+unsigned *serve_err_word(int dev);
+std::string serve_err_text(unsigned w);
+
 struct PfModel;     /* packed weights of the batched prefill (kc_prefill.cu) */
 struct PfScratch;   /* its per-state buffers */
 

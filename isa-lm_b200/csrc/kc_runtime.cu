@@ -673,6 +673,33 @@ static double rope_inv_freq(const kc_config &c, int i) {
     return (1.0 - smooth) * inv / f + smooth * inv;
 }
 
+/* The angles of positions 0..T-1 in double, stored as float (model/transformer.c:146-162);
+ * local: the sliding-window layers' own theta, without scaling. */
+static void fill_rope(const kc_config &c, size_t T, bool local, float *cs, float *sn) {
+    const size_t h2 = (size_t)c.head_dim / 2;
+    const double af = !local && c.rope_type == KC_ROPE_YARN ? c.rope_attn_factor : 1.0;
+    for (size_t i = 0; i < h2; i++) {
+        const double freq =
+            local ? std::pow((double)c.rope_local_theta, -2.0 * (double)i / c.head_dim) : rope_inv_freq(c, (int)i);
+        for (size_t p = 0; p < T; p++) {
+            const double ang = (double)p * freq;
+            cs[p * h2 + i] = (float)(std::cos(ang) * af);
+            sn[p * h2 + i] = (float)(std::sin(ang) * af);
+        }
+    }
+}
+
+extern "C" int kc_rope_tables(const kc_config *cfg, int n_pos, int local, float *cos_out, float *sin_out) {
+    clear_error();
+    const float theta = cfg ? (local ? cfg->rope_local_theta : cfg->rope_theta) : 0.0f;
+    if (!cfg || !cos_out || !sin_out || n_pos < 0 || cfg->head_dim < 2 || cfg->head_dim % 2 || !(theta > 0.0f)) {
+        set_error("rope tables: an even head_dim, a positive theta and two arrays are needed");
+        return KC_E_SHAPE;
+    }
+    fill_rope(*cfg, (size_t)n_pos, local != 0, cos_out, sin_out);
+    return KC_OK;
+}
+
 /* Bytes per cache element of a KV type. */
 static size_t kv_elem_bytes(int kv_type) { return kv_type == KC_F32 ? 4 : (kv_type == KC_F16 ? 2 : 1); }
 
@@ -1101,21 +1128,9 @@ extern "C" int kc_state_init(kc_state **out, kc_model *m, int nthreads, int kv_t
     /* RoPE tables: double, stored as float (model/transformer.c:146-162) */
     {
         std::vector<float> cs(T * h2), sn(T * h2), lc, ls_;
-        const double af = c.rope_type == KC_ROPE_YARN ? c.rope_attn_factor : 1.0;
         if (s->lcos) { lc.resize(T * h2); ls_.resize(T * h2); }
-        for (size_t i = 0; i < h2; i++) {
-            const double freq = rope_inv_freq(c, (int)i);
-            const double lfreq = s->lcos ? std::pow((double)c.rope_local_theta, -2.0 * (double)i / c.head_dim) : 0.0;
-            for (size_t p = 0; p < T; p++) {
-                const double ang = (double)p * freq;
-                cs[p * h2 + i] = (float)(std::cos(ang) * af);
-                sn[p * h2 + i] = (float)(std::sin(ang) * af);
-                if (s->lcos) {
-                    lc[p * h2 + i] = (float)std::cos((double)p * lfreq);
-                    ls_[p * h2 + i] = (float)std::sin((double)p * lfreq);
-                }
-            }
-        }
+        fill_rope(c, T, false, cs.data(), sn.data());
+        if (s->lcos) fill_rope(c, T, true, lc.data(), ls_.data());
         e = cudaMemcpy(s->rcos, cs.data(), sizeof(float) * T * h2, cudaMemcpyHostToDevice);
         if (e == cudaSuccess) e = cudaMemcpy(s->rsin, sn.data(), sizeof(float) * T * h2, cudaMemcpyHostToDevice);
         if (e == cudaSuccess && s->lcos) e = cudaMemcpy(s->lcos, lc.data(), sizeof(float) * T * h2, cudaMemcpyHostToDevice);
@@ -1589,24 +1604,26 @@ extern "C" void kc_dev_free(void *p) { if (p) cudaFree(p); }
 extern "C" int kc_memcpy_htod(void *dst, const void *src, size_t n) { CK(cudaMemcpy(dst, src, n, cudaMemcpyHostToDevice)); return KC_OK; }
 extern "C" int kc_memcpy_dtoh(void *dst, const void *src, size_t n) { CK(cudaMemcpy(dst, src, n, cudaMemcpyDeviceToHost)); return KC_OK; }
 /* Waits for the current device, then reads (and clears) the sticky error
- * words of the kernel-level matvec entry points on it. */
+ * words of the kernel-level matvec and serving entry points on it. */
 extern "C" int kc_dev_sync(void) {
     clear_error();
     CK(cudaDeviceSynchronize());
     int dev = 0;
     const int rc = current_device(dev);
     if (rc != KC_OK) return rc;
-    unsigned *words[2] = { g_kl_err_ptr[dev], g_noalloc_ptr[dev] ? (unsigned *)(g_noalloc_ptr[dev] + NOALLOC_ERR_OFF) : nullptr };
+    unsigned *words[3] = { g_kl_err_ptr[dev], g_noalloc_ptr[dev] ? (unsigned *)(g_noalloc_ptr[dev] + NOALLOC_ERR_OFF) : nullptr,
+                           serve_err_word(dev) };
     const char *names[2] = { "kc_matvec_dev", "kc_matvec_f32_noalloc" };
     std::string msg;
-    for (int i = 0; i < 2; i++) {
+    for (int i = 0; i < 3; i++) {
         if (!words[i]) continue;
         unsigned w = 0;
         CK(cudaMemcpy(&w, words[i], sizeof w, cudaMemcpyDeviceToHost));
         if (!w) continue;
         CK(cudaMemset(words[i], 0, sizeof w));
-        msg += std::string(msg.empty() ? "" : "; ") + names[i] + ": a device wait gave up (error word " +
-               std::to_string(w) + ")";
+        msg += msg.empty() ? "" : "; ";
+        if (i < 2) msg += std::string(names[i]) + ": a device wait gave up (error word " + std::to_string(w) + ")";
+        else msg += "serving operators skipped " + serve_err_text(w);
     }
     if (msg.empty()) return KC_OK;
     set_error(msg);

@@ -1,0 +1,387 @@
+/* Serving several sequences: the C entries of the paged KV cache (rows of new
+ * tokens, attention of one new token per sequence) and of the processing of a
+ * batch's logits. Every argument that the host can see is checked before a
+ * launch; what lies in device memory is checked by the kernels, which skip what
+ * is out of range and flag it for the next kc_dev_sync. */
+#include <cuda_runtime.h>
+
+#include <algorithm>
+#include <cmath>
+#include <string>
+
+#include "kc_internal.h"
+#include "kc_logits.cuh"
+#include "kc_paged.cuh"
+
+namespace kc {
+
+static int sv_cuda(cudaError_t e, const char *what) {
+    if (e == cudaSuccess) return KC_OK;
+    set_error(std::string(what) + ": " + cudaGetErrorString(e));
+    (void)cudaGetLastError();
+    if (e == cudaErrorMemoryAllocation) return KC_E_NOMEM;
+    if (e == cudaErrorNoDevice || e == cudaErrorInsufficientDriver || e == cudaErrorNoKernelImageForDevice)
+        return KC_E_ISA;
+    return KC_E_IO;
+}
+#define SK(call, what)                                    \
+    do {                                                  \
+        const cudaError_t e_ = (call);                    \
+        if (e_ != cudaSuccess) return sv_cuda(e_, what);  \
+    } while (0)
+
+static int refuse(const std::string &msg) {
+    set_error(msg);
+    return KC_E_SHAPE;
+}
+
+constexpr int SV_MAX_DEVICES = 64;
+
+/* The serving kernels' error word, one per device, sticky until kc_dev_sync. */
+static __device__ unsigned g_sv_err;
+static unsigned *g_sv_err_ptr[SV_MAX_DEVICES];
+
+struct ServeDev {
+    int dev = 0, sms = 0;
+    unsigned *err = nullptr;
+};
+
+/* The current device: its SMs and error word (looked up once per device). */
+static int serve_device(ServeDev &d) {
+    static int sms[SV_MAX_DEVICES];
+    SK(cudaGetDevice(&d.dev), "current device");
+    if (d.dev < 0 || d.dev >= SV_MAX_DEVICES) return refuse("device index " + std::to_string(d.dev) + " beyond this library's table");
+    if (!g_sv_err_ptr[d.dev]) {
+        int major = 0, minor = 0, n = 0;
+        SK(cudaDeviceGetAttribute(&major, cudaDevAttrComputeCapabilityMajor, d.dev), "device");
+        SK(cudaDeviceGetAttribute(&minor, cudaDevAttrComputeCapabilityMinor, d.dev), "device");
+        if (major != 10 || minor != 0) {
+            set_error("not an sm_100 device");
+            return KC_E_ISA;
+        }
+        SK(cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, d.dev), "device");
+        void *p = nullptr;
+        SK(cudaGetSymbolAddress(&p, g_sv_err), "error word");
+        sms[d.dev] = n;
+        g_sv_err_ptr[d.dev] = (unsigned *)p;
+    }
+    d.sms = sms[d.dev];
+    d.err = g_sv_err_ptr[d.dev];
+    return KC_OK;
+}
+
+unsigned *serve_err_word(int dev) { return dev >= 0 && dev < SV_MAX_DEVICES ? g_sv_err_ptr[dev] : nullptr; }
+
+std::string serve_err_text(unsigned w) {
+    std::string s;
+    auto add = [&](unsigned bit, const char *t) {
+        if (w & bit) s += std::string(s.empty() ? "" : ", ") + t;
+    };
+    add(SE_HIST, "a history length beyond its rows");
+    add(SE_BIAS, "bias offsets out of order or beyond the list");
+    add(SE_LEN, "a sequence length below 0 or beyond its table row");
+    add(SE_PAGE, "a page number outside the pool");
+    add(SE_ROW, "a new row's sequence, position or page out of range");
+    return s;
+}
+
+/* Device memory of the current device, aligned to `align` bytes. */
+static int check_ptr(const void *p, int dev, size_t align, const char *name) {
+    if (!p) return refuse(std::string(name) + " is NULL");
+    if ((uintptr_t)p % align) return refuse(std::string(name) + " is not aligned to " + std::to_string(align) + " bytes");
+    cudaPointerAttributes at;
+    const cudaError_t e = cudaPointerGetAttributes(&at, p);
+    if (e != cudaSuccess) return sv_cuda(e, name);
+    if (at.type != cudaMemoryTypeDevice && at.type != cudaMemoryTypeManaged)
+        return refuse(std::string(name) + " is not device memory");
+    if (at.type == cudaMemoryTypeDevice && at.device != dev)
+        return refuse(std::string(name) + " lies on device " + std::to_string(at.device) + ", not on the current device " +
+                      std::to_string(dev));
+    return KC_OK;
+}
+#define PTR(p, align)                                                   \
+    do {                                                                \
+        const int rc_ = check_ptr((const void *)(p), d.dev, align, #p); \
+        if (rc_ != KC_OK) return rc_;                                   \
+    } while (0)
+
+/* The sizes of a cache, without its pointers. */
+static int check_cache(const kc_paged_kv *kv) {
+    if (!kv) return refuse("kv is NULL");
+    if (kv->kv_type != KC_F32 && kv->kv_type != KC_F16 && kv->kv_type != KC_Q8_0)
+        return refuse("kv_type must be KC_F32, KC_F16 or KC_Q8_0");
+    if (kv->head_dim < 16 || kv->head_dim > 256 || kv->head_dim % 16)
+        return refuse("head_dim must be a multiple of 16 from 16 to 256");
+    if (kv->n_pages < 1 || kv->page_size < 1 || kv->n_kv_heads < 1 || kv->n_seqs < 1 || kv->ld_table < 1)
+        return refuse("n_pages, page_size, n_kv_heads, n_seqs and ld_table must be at least 1");
+    if ((double)kv->n_pages * kv->page_size * kv->n_kv_heads >= 4294967296.0)
+        return refuse("the pool's rows (n_pages * page_size * n_kv_heads) must be fewer than 2^32");
+    if ((double)kv->ld_table * kv->page_size > 2147483647.0)
+        return refuse("a table row (ld_table * page_size) must hold fewer than 2^31 positions");
+    return KC_OK;
+}
+
+static int take_cache(const kc_paged_kv *kv, const ServeDev &d, PagedKV &o) {
+    PTR(kv->k, 16);
+    PTR(kv->v, 16);
+    PTR(kv->table, 4);
+    if (kv->kv_type == KC_Q8_0) {
+        PTR(kv->kd, 4);
+        PTR(kv->vd, 4);
+    }
+    o = PagedKV{ (uint8_t *)kv->k, (uint8_t *)kv->v, kv->kd, kv->vd, kv->table, kv->n_seqs, kv->ld_table, kv->n_pages,
+                 kv->page_size, kv->n_kv_heads, kv->head_dim };
+    return KC_OK;
+}
+
+/* ------------------------------------------------------------ append */
+
+template <int KV>
+static void launch_append(const AppendArgs &a, cudaStream_t st) {
+    const int hd = a.kv.hd, lph = hd <= 32 ? 8 : (hd <= 64 ? 16 : 32);
+    const long long items = (long long)a.rows * (a.n_heads + 2 * a.kv.n_kv), per = AP_THREADS / lph;
+    const unsigned grid = (unsigned)((items + per - 1) / per);
+    if (lph == 8) append_kernel<KV, 8, 1><<<grid, AP_THREADS, 0, st>>>(a);
+    else if (lph == 16) append_kernel<KV, 16, 1><<<grid, AP_THREADS, 0, st>>>(a);
+    else if (hd <= 128) append_kernel<KV, 32, 1><<<grid, AP_THREADS, 0, st>>>(a);
+    else append_kernel<KV, 32, 2><<<grid, AP_THREADS, 0, st>>>(a);
+}
+
+/* ------------------------------------------------------------ attention */
+
+/* One instance: its kernels, shared memory, and on each device the CTAs that fit. */
+struct AttendVariant {
+    void (*attend)(const AttendArgs);
+    void (*join)(const AttendArgs);
+    int smem, part, quantum;
+    int ctas[SV_MAX_DEVICES];
+};
+
+template <int KV, int HD, int MT, int S>
+static AttendVariant make_variant() {
+    AttendVariant v{};
+    v.attend = paged_attend_kernel<KV, HD, MT, S>;
+    v.join = paged_join_kernel<HD, MT>;
+    v.smem = attend_smem<KV, HD, MT, S>();
+    v.part = part_floats<HD, MT>();
+    v.quantum = AT_WARPS * AttType<KV>::TP;
+    return v;
+}
+
+template <int KV>
+static AttendVariant *variants_of(int hd, int group, int &mt) {
+    static AttendVariant v64 = make_variant<KV, 64, 1, 6>(), v128 = make_variant<KV, 128, 1, 3>(),
+                         v256 = make_variant<KV, 256, 1, 3>();
+    if constexpr (KV != KC_F32) {
+        /* more than 8 heads share a KV head: 16 at a time, so that the cache is read once */
+        static AttendVariant w64 = make_variant<KV, 64, 2, 6>(), w128 = make_variant<KV, 128, 2, 3>();
+        if (group > 8 && hd <= 128) {
+            mt = 2;
+            return hd <= 64 ? &w64 : &w128;
+        }
+    }
+    mt = 1;
+    return hd <= 64 ? &v64 : (hd <= 128 ? &v128 : &v256);
+}
+
+static int attend_variant(const kc_paged_kv *kv, int n_heads, const ServeDev &d, AttendVariant *&v, int &chunks) {
+    const int group = n_heads / kv->n_kv_heads;
+    int mt = 1;
+    v = kv->kv_type == KC_F32 ? variants_of<KC_F32>(kv->head_dim, group, mt)
+                              : (kv->kv_type == KC_F16 ? variants_of<KC_F16>(kv->head_dim, group, mt)
+                                                       : variants_of<KC_Q8_0>(kv->head_dim, group, mt));
+    chunks = (group + 8 * mt - 1) / (8 * mt);
+    if (!v->ctas[d.dev]) {
+        SK(cudaFuncSetAttribute((const void *)v->attend, cudaFuncAttributeMaxDynamicSharedMemorySize, v->smem), "attend");
+        int n = 0;
+        SK(cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, (const void *)v->attend, AT_THREADS, (size_t)v->smem), "attend");
+        if (n < 1) {
+            set_error("attend: no CTA fits an SM");
+            return KC_E_IO;
+        }
+        v->ctas[d.dev] = n * d.sms;
+    }
+    return KC_OK;
+}
+
+static size_t ws_bytes(const AttendVariant *v, int ctas) {
+    return (size_t)ctas * (sizeof(int4) + 2 * sizeof(float) * (size_t)v->part);
+}
+
+}  // namespace kc
+
+using namespace kc;
+
+extern "C" int kc_paged_append_dev(const kc_paged_kv *kv, const kc_append_args *x, void *stream) {
+    clear_error();
+    int rc = check_cache(kv);
+    if (rc != KC_OK) return rc;
+    if (!x) return refuse("args is NULL");
+    if (x->rows < 0 || x->n_heads < 1 || x->n_pos < 1) return refuse("rows must not be negative, n_heads and n_pos at least 1");
+    const long long qd = (long long)x->n_heads * kv->head_dim, kd = (long long)kv->n_kv_heads * kv->head_dim;
+    if (x->ldq % 4 || x->ldk % 4 || x->ldv % 4 || x->ldo % 4) return refuse("row strides must be multiples of 4 floats");
+    if (x->rows > 1 && (x->ldq < qd || x->ldo < qd || x->ldk < kd || x->ldv < kd))
+        return refuse("a row stride is shorter than its row");
+    if (!x->q_norm != !x->k_norm) return refuse("q_norm and k_norm come together");
+    if (!(x->eps >= 0.0f) || std::isinf(x->eps)) return refuse("eps must be finite and not negative");
+    if ((double)x->rows * (x->n_heads + 2 * kv->n_kv_heads) > 2147483647.0) return refuse("too many rows in one call");
+    if (!x->seqs && x->rows > kv->n_seqs) return refuse("more rows than sequences, and no seqs");
+    ServeDev d;
+    rc = serve_device(d);
+    if (rc != KC_OK) return rc;
+    if (x->rows == 0) return KC_OK;
+    AppendArgs a{};
+    rc = take_cache(kv, d, a.kv);
+    if (rc != KC_OK) return rc;
+    PTR(x->q, 16);
+    PTR(x->k, 16);
+    PTR(x->v, 16);
+    PTR(x->q_out, 16);
+    PTR(x->cos, 8);
+    PTR(x->sin, 8);
+    PTR(x->pos, 4);
+    if (x->seqs) PTR(x->seqs, 4);
+    if (x->q_norm) {
+        PTR(x->q_norm, 4);
+        PTR(x->k_norm, 4);
+    }
+    a.q = x->q; a.k = x->k; a.v = x->v; a.q_out = x->q_out;
+    a.ldq = x->ldq; a.ldk = x->ldk; a.ldv = x->ldv; a.ldo = x->ldo;
+    a.cos = x->cos; a.sin = x->sin; a.q_norm = x->q_norm; a.k_norm = x->k_norm; a.eps = x->eps;
+    a.seqs = x->seqs; a.pos = x->pos; a.rows = x->rows; a.n_heads = x->n_heads; a.n_pos = x->n_pos;
+    a.err = d.err;
+    const cudaStream_t st = (cudaStream_t)stream;
+    if (kv->kv_type == KC_F32) launch_append<KC_F32>(a, st);
+    else if (kv->kv_type == KC_F16) launch_append<KC_F16>(a, st);
+    else launch_append<KC_Q8_0>(a, st);
+    return sv_cuda(cudaGetLastError(), "append");
+}
+
+static int check_heads(const kc_paged_kv *kv, int n_heads) {
+    if (n_heads < 1 || n_heads % kv->n_kv_heads) return refuse("n_heads must be a multiple of n_kv_heads");
+    return KC_OK;
+}
+
+extern "C" int kc_paged_attend_ws(const kc_paged_kv *kv, int n_heads, size_t *bytes) {
+    clear_error();
+    int rc = check_cache(kv);
+    if (rc == KC_OK) rc = check_heads(kv, n_heads);
+    if (rc != KC_OK) return rc;
+    ServeDev d;
+    AttendVariant *v = nullptr;
+    int chunks = 0;
+    rc = serve_device(d);
+    if (rc == KC_OK) rc = attend_variant(kv, n_heads, d, v, chunks);
+    if (rc != KC_OK) return rc;
+    *bytes = ws_bytes(v, v->ctas[d.dev]);
+    return KC_OK;
+}
+
+extern "C" int kc_paged_attend_dev(const kc_paged_kv *kv, const kc_attend_args *x, void *stream) {
+    clear_error();
+    int rc = check_cache(kv);
+    if (rc != KC_OK) return rc;
+    if (!x) return refuse("args is NULL");
+    rc = check_heads(kv, x->n_heads);
+    if (rc != KC_OK) return rc;
+    if (x->n_seqs < 0 || x->n_seqs > kv->n_seqs) return refuse("n_seqs must be 0 to the cache's");
+    const long long qd = (long long)x->n_heads * kv->head_dim;
+    if (x->ldq % 4 || x->ldo % 4) return refuse("row strides must be multiples of 4 floats");
+    if (x->n_seqs > 1 && (x->ldq < qd || x->ldo < qd)) return refuse("a row stride is shorter than its row");
+    if (x->window < 0) return refuse("window must not be negative");
+    if (!std::isfinite(x->scale) || !std::isfinite(x->softcap) || x->softcap < 0.0f)
+        return refuse("scale and softcap must be finite, softcap not negative");
+    ServeDev d;
+    rc = serve_device(d);
+    if (rc != KC_OK) return rc;
+    if (x->n_seqs == 0) return KC_OK;
+    AttendArgs a{};
+    AttendVariant *v = nullptr;
+    rc = attend_variant(kv, x->n_heads, d, v, a.chunks);
+    if (rc != KC_OK) return rc;
+    const int ctas = v->ctas[d.dev];
+    if (x->ws_bytes < ws_bytes(v, ctas))
+        return refuse("workspace of " + std::to_string(x->ws_bytes) + " bytes, " + std::to_string(ws_bytes(v, ctas)) +
+                      " needed (kc_paged_attend_ws)");
+    rc = take_cache(kv, d, a.kv);
+    if (rc != KC_OK) return rc;
+    PTR(x->q, 16);
+    PTR(x->out, 16);
+    PTR(x->lens, 4);
+    PTR(x->ws, 16);
+    a.q = x->q; a.out = x->out; a.ldq = x->ldq; a.ldo = x->ldo; a.lens = x->lens;
+    a.n_seqs = x->n_seqs; a.n_heads = x->n_heads; a.group = x->n_heads / kv->n_kv_heads;
+    a.window = x->window; a.scale = x->scale; a.softcap = x->softcap;
+    a.min_quanta = 1;
+    a.desc = (int4 *)x->ws;
+    a.part = (float *)((char *)x->ws + sizeof(int4) * (size_t)ctas);
+    a.err = d.err;
+    const cudaStream_t st = (cudaStream_t)stream;
+    v->attend<<<ctas, AT_THREADS, v->smem, st>>>(a);
+    SK(cudaGetLastError(), "attend");
+    /* a sequence of one quantum is never shared out: nothing to join */
+    if ((long long)kv->ld_table * kv->page_size <= v->quantum) return KC_OK;
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3((unsigned)ctas);
+    cfg.blockDim = dim3(JN_THREADS);
+    cfg.stream = st;
+    cudaLaunchAttribute at{};
+    at.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    at.val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = &at;
+    cfg.numAttrs = 1;
+    SK(cudaLaunchKernelEx(&cfg, v->join, a), "attend join");
+    return KC_OK;
+}
+
+/* ------------------------------------------------------------ logits */
+
+extern "C" int kc_logits_process_dev(const kc_logits_args *x, void *stream) {
+    clear_error();
+    if (!x) return refuse("args is NULL");
+    if (x->rows < 0 || x->vocab < 1 || x->vocab > (1 << 27)) return refuse("rows must not be negative, vocab 1 to 2^27");
+    if (x->rows > 1 && (x->ld_in < x->vocab || x->ld_out < x->vocab)) return refuse("a row stride is shorter than its row");
+    const bool pen = x->repeat || x->presence || x->frequency;
+    if (x->history_cap < 0 || (x->history && x->rows > 1 && x->ld_history < x->history_cap))
+        return refuse("history_cap must not be negative nor beyond ld_history");
+    if (!x->history && x->history_cap > 0) return refuse("history is NULL");
+    const bool bias = x->bias_off != nullptr;
+    if (x->n_bias < 0 || (bias && x->n_bias > 0 && (!x->bias_ids || !x->bias_vals)))
+        return refuse("biases need offsets, ids and values");
+    if (!bias && (x->bias_ids || x->bias_vals)) return refuse("biases need offsets, ids and values");
+    if (x->mask && x->rows > 1 && x->ld_mask < (x->vocab + 31) / 32) return refuse("a mask row is shorter than the vocabulary");
+    ServeDev d;
+    int rc = serve_device(d);
+    if (rc != KC_OK) return rc;
+    if (x->rows == 0) return KC_OK;
+    PTR(x->in, 4);
+    PTR(x->out, 4);
+    if (x->history) PTR(x->history, 4);
+    if (x->history_len) PTR(x->history_len, 4);
+    if (x->repeat) PTR(x->repeat, 4);
+    if (x->presence) PTR(x->presence, 4);
+    if (x->frequency) PTR(x->frequency, 4);
+    if (bias) {
+        PTR(x->bias_off, 4);
+        if (x->n_bias > 0) {
+            PTR(x->bias_ids, 4);
+            PTR(x->bias_vals, 4);
+        }
+    }
+    if (x->mask) PTR(x->mask, 4);
+    LogitsArgs a{};
+    a.in = x->in; a.out = x->out; a.ld_in = x->ld_in; a.ld_out = x->ld_out; a.vocab = x->vocab;
+    a.hist = x->history; a.hist_len = x->history_len; a.ld_hist = x->ld_history; a.hist_cap = x->history_cap;
+    a.repeat = x->repeat; a.presence = x->presence; a.frequency = x->frequency; a.repeat1 = 1.0f;
+    a.bias_off = x->bias_off; a.bias_ids = x->bias_ids; a.bias_vals = x->bias_vals; a.n_bias = x->n_bias;
+    a.mask = x->mask; a.ld_mask = x->ld_mask;
+    a.err = d.err;
+    const dim3 grid((unsigned)x->rows, (unsigned)((x->vocab + 3 + LG_CHUNK - 1) / LG_CHUNK));
+    const cudaStream_t st = (cudaStream_t)stream;
+    const bool hist = pen && x->history_cap > 0;
+    if (hist && bias) logits_kernel<true, true><<<grid, LG_THREADS, 0, st>>>(a);
+    else if (hist) logits_kernel<true, false><<<grid, LG_THREADS, 0, st>>>(a);
+    else if (bias) logits_kernel<false, true><<<grid, LG_THREADS, 0, st>>>(a);
+    else logits_kernel<false, false><<<grid, LG_THREADS, 0, st>>>(a);
+    return sv_cuda(cudaGetLastError(), "logits");
+}

@@ -103,6 +103,9 @@ def lib():
             "kc_dev_alloc": (P, [S]), "kc_dev_free": (None, [P]), "kc_memcpy_htod": (I, [P, P, S]),
             "kc_memcpy_dtoh": (I, [P, P, S]), "kc_dev_sync": (I, []), "kc_debug_wait_limit": (I, [I]),
             "kc_debug_ffn_split": (I, [I]),
+            "kc_rope_tables": (I, [P, I, I, P, P]), "kc_paged_append_dev": (I, [P, P, P]),
+            "kc_paged_attend_dev": (I, [P, P, P]), "kc_paged_attend_ws": (I, [P, I, C.POINTER(S)]),
+            "kc_logits_process_dev": (I, [P, P]),
         }
         for name, (res, args) in sig.items():
             f = getattr(L, name)
@@ -408,6 +411,239 @@ def block_sums(wtype, wq, rows, cols, xq):
     _check(lib().kc_block_sums_dev(bs.ptr, wtype, bw.ptr, rows, cols, bx.ptr, None), "block sums")
     _check(lib().kc_dev_sync(), "sync")
     return bs.get(np.int32, rows * (cols // 32)).reshape(rows, cols // 32)
+
+
+# ---------------------------------------------------------------- several sequences
+
+class DevArray(DevBuf):
+    """A DevBuf that knows its shape and type: what the operators below take
+    beside torch's CUDA tensors (anything with data_ptr, shape, stride, dtype)."""
+
+    def __init__(self, shape, dtype):
+        self.shape, self.dtype = tuple(int(n) for n in shape), np.dtype(dtype)
+        super().__init__(int(np.prod(self.shape, dtype=np.int64)) * self.dtype.itemsize)
+
+    @classmethod
+    def of(cls, arr):
+        a = np.ascontiguousarray(arr)
+        b = cls(a.shape, a.dtype)
+        if a.nbytes:
+            _check(lib().kc_memcpy_htod(b.ptr, a.ctypes.data_as(C.c_void_p), a.nbytes), "htod")
+        return b
+
+    def data_ptr(self):
+        return self.ptr
+
+    def stride(self):
+        return tuple(int(np.prod(self.shape[i + 1:], dtype=np.int64)) for i in range(len(self.shape)))
+
+    def numpy(self):
+        return self.get(self.dtype, int(np.prod(self.shape, dtype=np.int64))).reshape(self.shape)
+
+
+_TYPE_NAMES = {}      # dtype object (numpy's or torch's) -> "float32", "int32", ...
+
+
+def _shape_error(msg):
+    e = KraflaError(E_SHAPE, msg)
+    e.args = (f"{msg}: {STATUS[E_SHAPE]}",)
+    return e
+
+
+def _array(x, types, name):
+    """Checks an array's type; its shape."""
+    dt = x.dtype
+    t = _TYPE_NAMES.get(dt)
+    if t is None:
+        t = _TYPE_NAMES[dt] = str(dt).replace("torch.", "")
+    if t not in types:
+        raise _shape_error(f"{name} is {t}, not {' or '.join(types)}")
+    return x.shape
+
+
+_F, _I, _W = ("float32",), ("int32",), ("int32", "uint32")
+
+
+def _rows(x, types, n, width, name):
+    """Rows of `width` values, [n, width] or [n, ...] with contiguous rows: the row stride."""
+    shape, st = _array(x, types, name), x.stride()
+    size, at = 1, 1
+    for i in range(len(shape) - 1, 0, -1):
+        if st[i] != at and shape[i] != 1:
+            raise _shape_error(f"{name}: the values of a row are not contiguous")
+        size *= shape[i]
+        at = size
+    if len(shape) < 2 or shape[0] != n or size != width:
+        raise _shape_error(f"{name} is {list(shape)}, not [{n}, {width}]")
+    return st[0] if n > 1 else size
+
+
+def _flat(x, types, shape, name):
+    """A contiguous array of this shape: its address (None passes)."""
+    if x is None:
+        return None
+    s = _array(x, types, name)
+    if tuple(s) != shape:
+        raise _shape_error(f"{name} is {list(s)}, not {list(shape)}")
+    st, at = x.stride(), 1
+    for i in range(len(s) - 1, -1, -1):
+        if st[i] != at and s[i] > 1:
+            raise _shape_error(f"{name} is not contiguous")
+        at *= s[i]
+    return x.data_ptr()
+
+
+class _PagedKV(C.Structure):
+    _fields_ = [(n, C.c_void_p) for n in ("k", "v", "kd", "vd", "table")] + [
+        (n, C.c_int) for n in ("n_seqs", "ld_table", "n_pages", "page_size", "n_kv_heads", "head_dim", "kv_type")]
+
+
+class _AppendArgs(C.Structure):
+    _fields_ = [(n, C.c_void_p) for n in ("q", "k", "v", "q_out")] + [
+        (n, C.c_longlong) for n in ("ldq", "ldk", "ldv", "ldo")] + [
+        (n, C.c_void_p) for n in ("cos", "sin", "q_norm", "k_norm", "seqs", "pos")] + [
+        (n, C.c_int) for n in ("rows", "n_heads", "n_pos")] + [("eps", C.c_float)]
+
+
+class _AttendArgs(C.Structure):
+    _fields_ = [("q", C.c_void_p), ("out", C.c_void_p), ("ldq", C.c_longlong), ("ldo", C.c_longlong),
+                ("lens", C.c_void_p), ("n_seqs", C.c_int), ("n_heads", C.c_int), ("window", C.c_int),
+                ("scale", C.c_float), ("softcap", C.c_float), ("ws", C.c_void_p), ("ws_bytes", C.c_size_t)]
+
+
+class _LogitsArgs(C.Structure):
+    _fields_ = [("inp", C.c_void_p), ("out", C.c_void_p), ("ld_in", C.c_longlong), ("ld_out", C.c_longlong),
+                ("history", C.c_void_p), ("history_len", C.c_void_p), ("ld_history", C.c_longlong)] + [
+        (n, C.c_void_p) for n in ("repeat", "presence", "frequency", "bias_off", "bias_ids", "bias_vals", "mask")] + [
+        ("ld_mask", C.c_longlong)] + [(n, C.c_int) for n in ("rows", "vocab", "history_cap", "n_bias")]
+
+
+def rope_tables(config, n_pos, local=False):
+    """kc_rope_tables: (cos, sin), numpy [n_pos, head_dim / 2] float32, of a model's
+    configuration (Model.config, or a dict with head_dim, rope_theta and the scaling fields)."""
+    c = _Config()
+    for n, _ in c._fields_:
+        setattr(c, n, config.get(n, 0))
+    h2 = max(0, c.head_dim // 2)
+    cs, sn = np.empty((n_pos, h2), np.float32), np.empty((n_pos, h2), np.float32)
+    _check(lib().kc_rope_tables(C.byref(c), int(n_pos), int(bool(local)), cs.ctypes.data_as(C.c_void_p),
+                                sn.ctypes.data_as(C.c_void_p)), "rope tables")
+    return cs, sn
+
+
+class PagedKV:
+    """A paged KV cache of several sequences (kc_paged_kv) over the caller's arrays:
+
+        k, v    [n_pages, n_kv_heads, page_size, head_dim], float32, float16 or int8
+        kd, vd  an int8 cache's row scales [n_pages, n_kv_heads, page_size], float32
+        table   [n_seqs, pages per sequence] int32: the page of every page_size positions
+
+    Arrays are torch CUDA tensors or DevArrays on the current device; the caller
+    fills the table. The handle keeps them alive and holds the attention's
+    workspace for n_heads query heads: calls of `attend` that may overlap in time
+    (streams, threads, graphs) take one of their own from workspace(). `stream`
+    is a CUDA stream's handle (None: the default stream); nothing is waited for."""
+
+    def __init__(self, k, v, table, kv_type, kd=None, vd=None, n_heads=None):
+        types = {F32: _F, F16: ("float16",), Q8_0: ("int8",)}.get(kv_type)
+        if types is None:
+            raise _shape_error("kv_type must be F32, F16 or Q8_0")
+        shape = tuple(_array(k, types, "k"))
+        if len(shape) != 4:
+            raise _shape_error(f"k is {list(shape)}, not [n_pages, n_kv_heads, page_size, head_dim]")
+        self.n_heads = int(n_heads or shape[1])
+        if (kv_type == Q8_0) != (kd is not None and vd is not None) or (kd is None) != (vd is None):
+            raise _shape_error("an int8 cache has the scales kd and vd, another has none")
+        ts = tuple(_array(table, _I, "table"))
+        if len(ts) != 2:
+            raise _shape_error(f"table is {list(ts)}, not [n_seqs, pages]")
+        self.kv_type, self.n_seqs, self.head_dim = kv_type, ts[0], shape[3]
+        self.n_kv_heads, self.page_size = shape[1], shape[2]
+        self._keep = (k, v, kd, vd, table)
+        self._c = _PagedKV(_flat(k, types, shape, "k"), _flat(v, types, shape, "v"), _flat(kd, _F, shape[:3], "kd"),
+                           _flat(vd, _F, shape[:3], "vd"), _flat(table, _I, ts, "table"), ts[0], ts[1], shape[0],
+                           shape[2], shape[1], shape[3], kv_type)
+        self._ref = C.byref(self._c)
+        self._q = self.n_heads * self.head_dim
+        self._ws = self.workspace()
+
+    def workspace(self):
+        """Scratch for the attention calls of one stream."""
+        n = C.c_size_t()
+        _check(lib().kc_paged_attend_ws(self._ref, self.n_heads, C.byref(n)), "attend workspace")
+        return DevBuf(n.value)
+
+    def append(self, qkv, pos, cos, sin, q_out, seqs=None, q_norm=None, k_norm=None, eps=1e-5, stream=None):
+        """kc_paged_append_dev: rows of q|k|v ([rows, (n_heads + 2 n_kv_heads) head_dim], or the
+        three as a tuple) normed, rotated, queries to q_out, keys and values into the cache."""
+        n, hd, kw = q_out.shape[0], self.head_dim, self.n_kv_heads * self.head_dim
+        if isinstance(qkv, tuple):
+            q, k, v = qkv
+            ldq, ldk, ldv = _rows(q, _F, n, self._q, "q"), _rows(k, _F, n, kw, "k"), _rows(v, _F, n, kw, "v")
+            pq, pk, pv = q.data_ptr(), k.data_ptr(), v.data_ptr()
+        else:
+            ldq = ldk = ldv = _rows(qkv, _F, n, self._q + 2 * kw, "qkv")
+            pq = qkv.data_ptr()
+            pk, pv = pq + 4 * self._q, pq + 4 * (self._q + kw)
+        n_pos = cos.shape[0]
+        a = _AppendArgs(pq, pk, pv, q_out.data_ptr(), ldq, ldk, ldv, _rows(q_out, _F, n, self._q, "q_out"),
+                        _flat(cos, _F, (n_pos, hd // 2), "cos"), _flat(sin, _F, (n_pos, hd // 2), "sin"),
+                        _flat(q_norm, _F, (hd,), "q_norm"), _flat(k_norm, _F, (hd,), "k_norm"),
+                        _flat(seqs, _I, (n,), "seqs"), _flat(pos, _I, (n,), "pos"), n, self.n_heads, n_pos, eps)
+        st = lib().kc_paged_append_dev(self._ref, C.byref(a), stream)
+        if st:
+            raise KraflaError(st, "append")
+        return q_out
+
+    def attend(self, q, lens, out, scale=None, window=0, softcap=0.0, stream=None, ws=None):
+        """kc_paged_attend_dev: query rows [n, n_heads, head_dim] of the first n sequences
+        against their cached positions (the last `window` of lens[i]; 0: all) into out."""
+        n = q.shape[0]
+        ldq = _rows(q, _F, n, self._q, "q")
+        w = ws or self._ws
+        a = _AttendArgs(q.data_ptr(), out.data_ptr(), ldq, _rows(out, _F, n, self._q, "out"),
+                        _flat(lens, _I, (n,), "lens"), n, self.n_heads, window,
+                        self.head_dim ** -0.5 if scale is None else scale, softcap, w.ptr, w.nbytes)
+        st = lib().kc_paged_attend_dev(self._ref, C.byref(a), stream)
+        if st:
+            raise KraflaError(st, "attend")
+        return out
+
+
+def process_logits(out, logits, history=None, history_len=None, repeat=None, presence=None, frequency=None,
+                   bias_off=None, bias_ids=None, bias_vals=None, mask=None, stream=None):
+    """kc_logits_process_dev: penalties, biases and a mask of allowed tokens on rows of
+    logits [rows, vocab] into out (which may be logits). history [rows, cap] int32 with
+    history_len [rows]; repeat, presence, frequency [rows]; bias_off [rows + 1] into bias_ids
+    and bias_vals; mask [rows, words] with bit v % 32 of word v / 32 set where v is allowed."""
+    shape = _array(logits, _F, "logits")
+    if len(shape) != 2:
+        raise _shape_error(f"logits is {list(shape)}, not [rows, vocab]")
+    n, v = shape
+    ld_h, cap, ld_m = 0, 0, 0
+    if history is None and not (repeat is presence is frequency is history_len is None):
+        raise _shape_error("penalties need the rows' history")
+    if history is not None:
+        cap = history.shape[-1]
+        ld_h = _rows(history, _I, n, cap, "history")
+    if mask is not None:
+        words = mask.shape[-1]
+        if words < (v + 31) // 32:
+            raise _shape_error(f"mask has {words} words a row for {v} tokens")
+        ld_m = _rows(mask, _W, n, words, "mask")
+    n_bias = 0
+    if bias_ids is not None:
+        n_bias = bias_ids.shape[0]
+    a = _LogitsArgs(logits.data_ptr(), out.data_ptr(), _rows(logits, _F, n, v, "logits"), _rows(out, _F, n, v, "out"),
+                    history.data_ptr() if cap else None, _flat(history_len, _I, (n,), "history_len"), ld_h,
+                    _flat(repeat, _F, (n,), "repeat"), _flat(presence, _F, (n,), "presence"),
+                    _flat(frequency, _F, (n,), "frequency"), _flat(bias_off, _I, (n + 1,), "bias_off"),
+                    _flat(bias_ids, _I, (n_bias,), "bias_ids"), _flat(bias_vals, _F, (n_bias,), "bias_vals"),
+                    mask.data_ptr() if mask is not None else None, ld_m, n, v, cap, n_bias)
+    st = lib().kc_logits_process_dev(C.byref(a), stream)
+    if st:
+        raise KraflaError(st, "process logits")
+    return out
 
 
 # ---------------------------------------------------------------- model writer
