@@ -342,8 +342,8 @@ int kc_paged_append_dev(const kc_paged_kv *kv, const kc_append_args *args, void 
  * depend on what else is running, but how a row is cut into pieces depends on
  * the other rows' lengths: results of different batches differ by float
  * rounding. ws: at least kc_paged_attend_ws bytes of scratch, 16-byte aligned,
- * not initialised; calls (or replayed graphs) that may overlap in time need one
- * each. */
+ * prepared once by kc_paged_attend_ws_init; calls (or replayed graphs) that may
+ * overlap in time need one each, one after the other any calls may share it. */
 typedef struct {
     const float *q;
     float *out;
@@ -356,6 +356,7 @@ typedef struct {
 } kc_attend_args;
 int kc_paged_attend_dev(const kc_paged_kv *kv, const kc_attend_args *args, void *stream);
 int kc_paged_attend_ws(const kc_paged_kv *kv, int n_heads, size_t *bytes);
+int kc_paged_attend_ws_init(void *ws, size_t bytes);
 
 /* Logits before a token is chosen, rows [vocab] of in to out (out may be in):
  * with c the times that token v is in the row's history,

@@ -20,6 +20,7 @@ namespace kc {
 
 constexpr int LG_THREADS = 256;
 constexpr int LG_VEC = 4;                              /* float4 per thread */
+constexpr int LG_HIST = 8;                             /* history tokens a thread requests at once */
 constexpr int LG_CHUNK = LG_THREADS * LG_VEC * 4;      /* logits per CTA */
 
 struct LogitsArgs {
@@ -31,7 +32,6 @@ struct LogitsArgs {
     long long ld_hist;
     int hist_cap;
     const float *repeat, *presence, *frequency;
-    float repeat1;                  /* the rows' repeat where `repeat` is NULL */
     const int *bias_off, *bias_ids;
     const float *bias_vals;
     int n_bias;
@@ -42,8 +42,8 @@ struct LogitsArgs {
 
 template <bool HIST, bool BIAS>
 __global__ void __launch_bounds__(LG_THREADS) logits_kernel(const LogitsArgs a) {
-    __shared__ int s_count[HIST ? LG_CHUNK : 1];
-    __shared__ int s_bias[BIAS ? LG_CHUNK : 1];        /* the last list entry of each token, -1 none */
+    __shared__ __align__(16) int s_count[HIST ? LG_CHUNK : 1];
+    __shared__ __align__(16) int s_bias[BIAS ? LG_CHUNK : 1];        /* the last list entry of each token, -1 none */
     const int tid = threadIdx.x, V = a.vocab;
     const long long row = blockIdx.x;
     const float *in = a.in + row * a.ld_in;
@@ -64,27 +64,50 @@ __global__ void __launch_bounds__(LG_THREADS) logits_kernel(const LogitsArgs a) 
             for (int i = 0; i < 4; i++) z[k][i] = e + i >= 0 && e + i < V ? in[e + i] : 0.0f;
         }
     }
+    /* the words that hold bits e .. e + 3 of each vector */
+    uint32_t ma[LG_VEC], mb[LG_VEC];
+#pragma unroll
+    for (int k = 0; k < LG_VEC; k++) {
+        ma[k] = mb[k] = 0xffffffffu;
+        const int e = e0 + 4 * (tid + k * LG_THREADS), w = e >> 5;
+        if (a.mask && e + 3 >= 0 && e < V) {
+            const uint32_t *mask = a.mask + row * a.ld_mask;
+            if (w >= 0) ma[k] = mb[k] = __ldg(mask + w);
+            if (((e + 3) >> 5) != w && ((e + 3) >> 5) <= (V - 1) >> 5) mb[k] = __ldg(mask + ((e + 3) >> 5));
+        }
+    }
     float rep = 1.0f, pres = 0.0f, freq = 0.0f;
     if constexpr (HIST || BIAS) {
-        for (int i = tid; i < LG_CHUNK; i += LG_THREADS) {
-            if constexpr (HIST) s_count[i] = 0;
-            if constexpr (BIAS) s_bias[i] = -1;
+        const int *h = a.hist + row * a.ld_hist;
+        int t0[HIST ? LG_HIST : 1], n = 0;
+        if constexpr (HIST) {
+#pragma unroll
+            for (int k = 0; k < LG_HIST; k++) {
+                const int i = tid + k * LG_THREADS;
+                t0[k] = i < a.hist_cap ? __ldg(h + i) : -1;
+            }
+            n = a.hist_len ? a.hist_len[row] : a.hist_cap;
+            rep = a.repeat ? a.repeat[row] : 1.0f;
+            if (a.presence) pres = a.presence[row];
+            if (a.frequency) freq = a.frequency[row];
+        }
+        for (int i = tid; i < LG_CHUNK / 4; i += LG_THREADS) {
+            if constexpr (HIST) ((int4 *)s_count)[i] = make_int4(0, 0, 0, 0);
+            if constexpr (BIAS) ((int4 *)s_bias)[i] = make_int4(-1, -1, -1, -1);
         }
         __syncthreads();
         if constexpr (HIST) {
-            int n = a.hist_len ? a.hist_len[row] : a.hist_cap;
             if (n > a.hist_cap) {
                 if (tid == 0 && blockIdx.y == 0) atomicOr(a.err, 1u);
                 n = a.hist_cap;
             }
-            const int *h = a.hist + row * a.ld_hist;
-            for (int i = tid; i < n; i += LG_THREADS) {
-                const int t = h[i];
+            auto seen = [&](int t) {
                 if (t >= 0 && t < V && t >= e0 && t - e0 < LG_CHUNK) atomicAdd(&s_count[t - e0], 1);
-            }
-            rep = a.repeat ? a.repeat[row] : a.repeat1;
-            if (a.presence) pres = a.presence[row];
-            if (a.frequency) freq = a.frequency[row];
+            };
+#pragma unroll
+            for (int k = 0; k < LG_HIST; k++)
+                if (tid + k * LG_THREADS < n) seen(t0[k]);
+            for (int i = tid + LG_HIST * LG_THREADS; i < n; i += LG_THREADS) seen(__ldg(h + i));
         }
         if constexpr (BIAS) {
             int b0 = a.bias_off[row], b1 = a.bias_off[row + 1];
@@ -99,30 +122,21 @@ __global__ void __launch_bounds__(LG_THREADS) logits_kernel(const LogitsArgs a) 
         }
         __syncthreads();
     }
-    const uint32_t *mask = a.mask ? a.mask + row * a.ld_mask : nullptr;
 #pragma unroll
     for (int k = 0; k < LG_VEC; k++) {
         const int o = 4 * (tid + k * LG_THREADS), e = e0 + o;
         if (e + 3 < 0 || e >= V) continue;
-        /* the vector's mask bits: one word or two */
-        unsigned bits = 0xfu;
-        if (mask) {
-            const int ea = max(e, 0), eb = min(e + 3, V - 1);
-            const uint32_t wa = __ldg(mask + (ea >> 5));
-            const uint32_t wb = (eb >> 5) != (ea >> 5) ? __ldg(mask + (eb >> 5)) : wa;
-            bits = 0u;
-#pragma unroll
-            for (int i = 0; i < 4; i++) {
-                const int v = min(max(e + i, ea), eb);
-                const uint32_t w = (v >> 5) == (ea >> 5) ? wa : wb;
-                bits |= ((w >> (v & 31)) & 1u) << i;
-            }
-        }
+        /* the vector's mask bits, from its two words (elements before the row have e < 0: any bit will do) */
+        const unsigned bits = __funnelshift_r(ma[k], mb[k], (unsigned)e & 31u);
+        int4 cn = make_int4(0, 0, 0, 0), bn = make_int4(-1, -1, -1, -1);
+        if constexpr (HIST) cn = *(const int4 *)(s_count + o);
+        if constexpr (BIAS) bn = *(const int4 *)(s_bias + o);
+        const int cc[4] = { cn.x, cn.y, cn.z, cn.w }, bb[4] = { bn.x, bn.y, bn.z, bn.w };
 #pragma unroll
         for (int i = 0; i < 4; i++) {
             float x = z[k][i];
             if constexpr (HIST) {
-                const int c = s_count[o + i];
+                const int c = cc[i];
                 if (c > 0) {
                     x = x > 0.0f ? __fdiv_rn(x, rep) : __fmul_rn(x, rep);
                     x = __fsub_rn(x, __fmul_rn(freq, (float)c));
@@ -130,7 +144,7 @@ __global__ void __launch_bounds__(LG_THREADS) logits_kernel(const LogitsArgs a) 
                 }
             }
             if constexpr (BIAS) {
-                const int b = s_bias[o + i];
+                const int b = bb[i];
                 if (b >= 0) x = __fadd_rn(x, a.bias_vals[b]);
             }
             z[k][i] = (bits >> i) & 1u ? x : -INFINITY;

@@ -42,6 +42,7 @@ struct AppendArgs {
 };
 
 constexpr int AP_THREADS = 256;
+constexpr int AP_HEADS = 4;                /* heads that a group of lanes takes at once */
 
 /* The sum over the LPH lanes that hold a head's row. */
 template <int LPH, class T>
@@ -51,155 +52,172 @@ __device__ __forceinline__ T head_sum(T v) {
     return v;
 }
 
-/* Norm (y = x / sqrt(mean(x^2) + eps) * w) and rotation of adjacent pairs of
- * the 4 * NV values that each lane of a head holds, in type T. */
+/* 1 / sqrt(mean(x^2) + eps) of each of a lane's AP_HEADS heads, in type T. The
+ * root and the division are taken once for all of them: lane k of a group does
+ * head k's and hands it round. */
 template <class T, int LPH, int NV>
-__device__ __forceinline__ void norm_rope(const float (&x)[NV][4], float (&y)[NV][4], const float *w, float eps, int hd,
-                                          const float *cs, const float *sn, int lane) {
-    T inv = (T)1;
-    if (w) {
+__device__ __forceinline__ void head_norms(const float (&x)[AP_HEADS][NV][4], T (&inv)[AP_HEADS], float eps, int hd) {
+    T mine = (T)0;
+#pragma unroll
+    for (int k = 0; k < AP_HEADS; k++) {
         T s = (T)0;
 #pragma unroll
         for (int j = 0; j < NV; j++)
 #pragma unroll
-            for (int i = 0; i < 4; i++) s += (T)x[j][i] * (T)x[j][i];
+            for (int i = 0; i < 4; i++) s += (T)x[k][j][i] * (T)x[k][j][i];
         s = head_sum<LPH>(s);
-        if constexpr (sizeof(T) == 8) inv = 1.0 / sqrt(s / (double)hd + (double)eps);
-        else inv = __fdiv_rn(1.0f, __fsqrt_rn(__fadd_rn(__fdiv_rn(s, (float)hd), eps)));
+        if (threadIdx.x % AP_HEADS == k) mine = s;
     }
+    if constexpr (sizeof(T) == 8) mine = 1.0 / sqrt(mine / (double)hd + (double)eps);
+    else mine = __fdiv_rn(1.0f, __fsqrt_rn(__fadd_rn(__fdiv_rn(mine, (float)hd), eps)));
+#pragma unroll
+    for (int k = 0; k < AP_HEADS; k++) inv[k] = __shfl_sync(0xffffffffu, mine, k, LPH);
+}
+
+/* y = x inv w, then the rotation of adjacent pairs, of 4 * NV values of a head, in type T. */
+template <class T, int NV>
+__device__ __forceinline__ void norm_rope(float (&x)[NV][4], bool norm, T inv, const float4 (&w)[NV], const float2 (&cs)[NV],
+                                          const float2 (&sn)[NV]) {
 #pragma unroll
     for (int j = 0; j < NV; j++) {
-        const int d = 4 * (lane + j * LPH);
-        if (d >= hd) continue;
-        const float2 c = __ldg((const float2 *)(cs + d / 2)), s = __ldg((const float2 *)(sn + d / 2));
-        float4 g = make_float4(1.0f, 1.0f, 1.0f, 1.0f);
-        if (w) g = make_float4(__ldg(w + d), __ldg(w + d + 1), __ldg(w + d + 2), __ldg(w + d + 3));
-        const T a = (T)x[j][0] * inv * (T)g.x, b = (T)x[j][1] * inv * (T)g.y;
-        const T e = (T)x[j][2] * inv * (T)g.z, f = (T)x[j][3] * inv * (T)g.w;
-        y[j][0] = (float)(a * (T)c.x - b * (T)s.x);
-        y[j][1] = (float)(a * (T)s.x + b * (T)c.x);
-        y[j][2] = (float)(e * (T)c.y - f * (T)s.y);
-        y[j][3] = (float)(e * (T)s.y + f * (T)c.y);
+        T a = (T)x[j][0], b = (T)x[j][1], e = (T)x[j][2], f = (T)x[j][3];
+        if (norm) {
+            a = a * inv * (T)w[j].x;
+            b = b * inv * (T)w[j].y;
+            e = e * inv * (T)w[j].z;
+            f = f * inv * (T)w[j].w;
+        }
+        x[j][0] = (float)(a * (T)cs[j].x - b * (T)sn[j].x);
+        x[j][1] = (float)(a * (T)sn[j].x + b * (T)cs[j].x);
+        x[j][2] = (float)(e * (T)cs[j].y - f * (T)sn[j].y);
+        x[j][3] = (float)(e * (T)sn[j].y + f * (T)cs[j].y);
     }
 }
 
-/* One head of one row per group of LPH lanes, 4 * NV values a lane. Bound by
- * memory: every value is read once and written once.
+/* A warp takes AP_HEADS heads of one kind (queries, keys or values) of a row
+ * for each of its groups of LPH lanes, 4 * NV values of a head a lane. Bound by
+ * memory: every value is read once and written once, so all of a warp's heads
+ * are requested before anything waits, and the row's place in the cache (three
+ * dependent loads), its angles and the norm's weights are fetched once for them.
  *
  * K rows of an 8-bit cache are normed and rotated in 64 bits and rounded once,
  * so that which side of a step's border a value falls on does not depend on
  * the order of the norm's sum; queries and wider caches use 32 bits. */
 template <int KV, int LPH, int NV>
 __global__ void __launch_bounds__(AP_THREADS) append_kernel(const AppendArgs a) {
-    const int lane = threadIdx.x % LPH;
-    const int heads = a.n_heads + 2 * a.kv.n_kv, hd = a.kv.hd;
-    const long long item = ((long long)blockIdx.x * AP_THREADS + threadIdx.x) / LPH, total = (long long)a.rows * heads;
-    const bool live = item < total;
-    const int row = live ? (int)(item / heads) : 0, h = live ? (int)(item % heads) : 0;
-    const bool isq = h < a.n_heads, isv = h >= a.n_heads + a.kv.n_kv;
-    const int hh = isq ? h : (isv ? h - a.n_heads - a.kv.n_kv : h - a.n_heads);
+    constexpr int HW = AP_HEADS * (32 / LPH);          /* heads per warp */
+    const int lane = threadIdx.x % LPH, sub = threadIdx.x % 32 / LPH, hd = a.kv.hd;
+    const int tq = (a.n_heads + HW - 1) / HW, tk = (a.kv.n_kv + HW - 1) / HW, tasks = tq + 2 * tk;
+    const long long item = ((long long)blockIdx.x * AP_THREADS + threadIdx.x) / 32;
+    if (item >= (long long)a.rows * tasks) return;     /* (whole warps) */
+    const int row = (int)(item / tasks), task = (int)(item % tasks);
+    const bool isq = task < tq, isv = task >= tq + tk;
+    const int h0 = HW * (isq ? task : (isv ? task - tq - tk : task - tq)) + sub, nh = isq ? a.n_heads : a.kv.n_kv;
     const float *src = isq ? a.q + row * a.ldq : (isv ? a.v + row * a.ldv : a.k + row * a.ldk);
-    src += (size_t)hh * hd;
-    float x[NV][4], y[NV][4];
+    const int seq = a.seqs ? a.seqs[row] : row, p = a.pos[row];
+    if (seq < 0) return;                               /* padding */
+    float x[AP_HEADS][NV][4];
 #pragma unroll
-    for (int j = 0; j < NV; j++) {
-        const int d = 4 * (lane + j * LPH);
-        float4 t = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-        if (live && d < hd) t = __ldcs((const float4 *)(src + d));
-        x[j][0] = t.x; x[j][1] = t.y; x[j][2] = t.z; x[j][3] = t.w;
-    }
-    /* where the row goes: the same for all lanes of the head */
-    const int seq = live ? (a.seqs ? a.seqs[row] : row) : -1, p = live ? a.pos[row] : 0;
-    bool ok = seq >= 0;
-    int page = 0, slot = 0;
+    for (int k = 0; k < AP_HEADS; k++)
+#pragma unroll
+        for (int j = 0; j < NV; j++) {
+            const int d = 4 * (lane + j * LPH), h = h0 + k * (32 / LPH);
+            float4 t = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+            if (h < nh && d < hd) t = __ldcs((const float4 *)(src + (size_t)h * hd + d));
+            x[k][j][0] = t.x; x[k][j][1] = t.y; x[k][j][2] = t.z; x[k][j][3] = t.w;
+        }
+    const int pi = p >= 0 ? p / a.kv.page : 0, slot = p - pi * a.kv.page;
+    bool ok = seq < a.kv.n_seqs && p >= 0 && p < a.n_pos && pi < a.kv.ld_table;
+    int page = 0;
     if (ok) {
-        const int pi = p >= 0 ? p / a.kv.page : 0;
-        slot = p - pi * a.kv.page;
-        if (seq >= a.kv.n_seqs || p < 0 || p >= a.n_pos || pi >= a.kv.ld_table) ok = false;
-        else {
-            page = a.kv.table[(size_t)seq * a.kv.ld_table + pi];
-            ok = page >= 0 && page < a.kv.n_pages;
-        }
-        if (!ok && lane == 0 && h == 0) atomicOr(a.err, (unsigned)SE_ROW);
+        page = a.kv.table[(size_t)seq * a.kv.ld_table + pi];
+        ok = page >= 0 && page < a.kv.n_pages;
     }
-    /* no early return: the lanes of a warp meet in the sums */
-    const float *cs = a.cos + (size_t)(ok ? p : 0) * (hd / 2), *sn = a.sin + (size_t)(ok ? p : 0) * (hd / 2);
-    if (isv) {
-#pragma unroll
-        for (int j = 0; j < NV; j++)
-#pragma unroll
-            for (int i = 0; i < 4; i++) y[j][i] = x[j][i];
+    if (!ok) {
+        if (threadIdx.x % 32 == 0) atomicOr(a.err, (unsigned)SE_ROW);
+        return;
     }
-    /* (the norm's shuffles are taken by all lanes of a warp: heads of different
-     * kinds may share it, so each kind's pass runs warp-wide where one needs it) */
-    float t[NV][4];
-    const bool any_q = __any_sync(0xffffffffu, isq), any_k = __any_sync(0xffffffffu, !isq && !isv);
-    if (KV != KC_Q8_0 || any_q) {
-        norm_rope<float, LPH, NV>(x, t, a.q_norm ? (isq ? a.q_norm : a.k_norm) : nullptr, a.eps, hd, cs, sn, lane);
-        if (isq || (KV != KC_Q8_0 && !isv)) {
-#pragma unroll
-            for (int j = 0; j < NV; j++)
-#pragma unroll
-                for (int i = 0; i < 4; i++) y[j][i] = t[j][i];
-        }
-    }
-    if (KV == KC_Q8_0 && any_k) {
-        norm_rope<double, LPH, NV>(x, t, a.k_norm, a.eps, hd, cs, sn, lane);
-        if (!isq && !isv) {
-#pragma unroll
-            for (int j = 0; j < NV; j++)
-#pragma unroll
-                for (int i = 0; i < 4; i++) y[j][i] = t[j][i];
-        }
-    }
-    float amax = 0.0f;
-    if constexpr (KV == KC_Q8_0) {
-#pragma unroll
-        for (int j = 0; j < NV; j++)
-            if (4 * (lane + j * LPH) < hd)
-                amax = fmaxf(amax, fmaxf(fmaxf(fabsf(y[j][0]), fabsf(y[j][1])), fmaxf(fabsf(y[j][2]), fabsf(y[j][3]))));
-#pragma unroll
-        for (int o = LPH / 2; o > 0; o >>= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, o));
-    }
-    if (!ok) return;
-    if (isq) {
-        float *dst = a.q_out + row * a.ldo + (size_t)hh * hd;
+    if (!isv) {
+        const float *wt = isq ? a.q_norm : a.k_norm;
+        float4 w[NV];
+        float2 cs[NV], sn[NV];
 #pragma unroll
         for (int j = 0; j < NV; j++) {
             const int d = 4 * (lane + j * LPH);
-            if (d < hd) *(float4 *)(dst + d) = make_float4(y[j][0], y[j][1], y[j][2], y[j][3]);
+            cs[j] = sn[j] = make_float2(0.0f, 0.0f);
+            w[j] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+            if (d < hd) {
+                cs[j] = __ldg((const float2 *)(a.cos + (size_t)p * (hd / 2) + d / 2));
+                sn[j] = __ldg((const float2 *)(a.sin + (size_t)p * (hd / 2) + d / 2));
+                if (wt) w[j] = __ldg((const float4 *)(wt + d));
+            }
         }
+        auto turn = [&](auto one) {
+            using T = decltype(one);
+            T inv[AP_HEADS];
+            if (wt) head_norms<T, LPH, NV>(x, inv, a.eps, hd);
+#pragma unroll
+            for (int k = 0; k < AP_HEADS; k++) norm_rope<T, NV>(x[k], wt != nullptr, wt ? inv[k] : one, w, cs, sn);
+        };
+        if (KV == KC_Q8_0 && !isq) turn(1.0);
+        else turn(1.0f);
+    }
+    if (isq) {
+        float *dst = a.q_out + row * a.ldo;
+#pragma unroll
+        for (int k = 0; k < AP_HEADS; k++)
+#pragma unroll
+            for (int j = 0; j < NV; j++) {
+                const int d = 4 * (lane + j * LPH), h = h0 + k * (32 / LPH);
+                if (h < nh && d < hd)
+                    *(float4 *)(dst + (size_t)h * hd + d) = make_float4(x[k][j][0], x[k][j][1], x[k][j][2], x[k][j][3]);
+            }
         return;
     }
-    const size_t r = ((size_t)page * a.kv.n_kv + hh) * a.kv.page + slot;
     uint8_t *pool = isv ? a.kv.v : a.kv.k;
-    /* the single-scale row rule of the model's 8-bit cache (ops/ops.c:81-96) */
-    const bool tiny = amax < 1e-30f;
-    const float id = KV == KC_Q8_0 && !tiny ? __fdiv_rn(127.0f, amax) : 0.0f;
+    const size_t r0 = (size_t)page * a.kv.n_kv * a.kv.page + slot;
 #pragma unroll
-    for (int j = 0; j < NV; j++) {
-        const int d = 4 * (lane + j * LPH);
-        if (d >= hd) continue;
-        if constexpr (KV == KC_F32) {
-            ((float4 *)pool)[(r * hd + d) / 4] = make_float4(y[j][0], y[j][1], y[j][2], y[j][3]);
-        } else if constexpr (KV == KC_F16) {
-            __half2 lo = __floats2half2_rn(y[j][0], y[j][1]), hi = __floats2half2_rn(y[j][2], y[j][3]);
-            ((uint2 *)pool)[(r * hd + d) / 4] = make_uint2(*(unsigned *)&lo, *(unsigned *)&hi);
-        } else {
-            unsigned w = 0;
+    for (int k = 0; k < AP_HEADS; k++) {
+        const int h = h0 + k * (32 / LPH);
+        const size_t r = r0 + (size_t)h * a.kv.page;
+        /* the single-scale row rule of the model's 8-bit cache (ops/ops.c:81-96) */
+        float amax = 0.0f, id = 0.0f;
+        bool tiny = false;
+        if constexpr (KV == KC_Q8_0) {
 #pragma unroll
-            for (int i = 0; i < 4; i++) {
-                int qi = 0;
-                if (!tiny) {
-                    const float u = truncf(__fadd_rn(__fmul_rn(y[j][i], id), copysignf(0.5f, y[j][i])));
-                    qi = (int)fminf(fmaxf(u, -127.0f), 127.0f);
-                }
-                w |= ((unsigned)qi & 0xffu) << (8 * i);
-            }
-            ((unsigned *)pool)[(r * hd + d) / 4] = w;
+            for (int j = 0; j < NV; j++)               /* (values beyond the head are zero) */
+                amax = fmaxf(amax, fmaxf(fmaxf(fabsf(x[k][j][0]), fabsf(x[k][j][1])), fmaxf(fabsf(x[k][j][2]), fabsf(x[k][j][3]))));
+#pragma unroll
+            for (int o = LPH / 2; o > 0; o >>= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, o));
+            tiny = amax < 1e-30f;
+            id = tiny ? 0.0f : __fdiv_rn(127.0f, amax);
         }
+#pragma unroll
+        for (int j = 0; j < NV; j++) {
+            const int d = 4 * (lane + j * LPH);
+            if (h >= nh || d >= hd) continue;
+            const float *y = x[k][j];
+            if constexpr (KV == KC_F32) {
+                ((float4 *)pool)[(r * hd + d) / 4] = make_float4(y[0], y[1], y[2], y[3]);
+            } else if constexpr (KV == KC_F16) {
+                __half2 lo = __floats2half2_rn(y[0], y[1]), hi = __floats2half2_rn(y[2], y[3]);
+                ((uint2 *)pool)[(r * hd + d) / 4] = make_uint2(*(unsigned *)&lo, *(unsigned *)&hi);
+            } else {
+                unsigned w = 0;
+#pragma unroll
+                for (int i = 0; i < 4; i++) {
+                    int qi = 0;
+                    if (!tiny) {
+                        const float u = truncf(__fadd_rn(__fmul_rn(y[i], id), copysignf(0.5f, y[i])));
+                        qi = (int)fminf(fmaxf(u, -127.0f), 127.0f);
+                    }
+                    w |= ((unsigned)qi & 0xffu) << (8 * i);
+                }
+                ((unsigned *)pool)[(r * hd + d) / 4] = w;
+            }
+        }
+        if (KV == KC_Q8_0 && lane == 0 && h < nh) (isv ? a.kv.vd : a.kv.kd)[r] = tiny ? 0.0f : __fdiv_rn(amax, 127.0f);
     }
-    if (KV == KC_Q8_0 && lane == 0) (isv ? a.kv.vd : a.kv.kd)[r] = tiny ? 0.0f : __fdiv_rn(amax, 127.0f);
 }
 
 /* ------------------------------------------------------------ attention */
@@ -208,12 +226,14 @@ __global__ void __launch_bounds__(AP_THREADS) append_kernel(const AppendArgs a) 
  * softcap * tanh of that over softcap) for t in [max(0, len - window), len).
  *
  * Work is cut into quanta of AT_WARPS tiles of TP positions of one unit (a
- * sequence's KV head, or a chunk of 8 * MT of its query heads). The quanta of
- * all units in a row are shared out evenly over the CTAs, so that ragged
- * lengths leave none idle; a CTA's share may begin and end inside a unit, whose
- * pieces paged_join_kernel puts together. Within a quantum each warp has a tile,
- * its own ring of shared-memory slots (cp.async) and its own running softmax;
- * the warps meet once per unit.
+ * sequence's KV head, or a chunk of 8 * MT of its query heads). All units in a
+ * row, each unit_cost quanta's time for itself and one for each quantum, are
+ * shared out evenly over the CTAs, so that ragged lengths leave none idle; a
+ * CTA's share may begin and end inside a unit: it then leaves its piece in the
+ * workspace, and the CTA that brings a unit's last missing piece joins them all,
+ * in the CTAs' order, so that the result does not depend on who came last.
+ * Within a quantum each warp has a tile, its own ring of shared-memory slots
+ * (cp.async) and its own running softmax; the warps meet once per unit.
  *
  * Both products run on the tensor cores with the query heads as the 16-row
  * side: rows 0-7 hold the high halves of eight heads' values, rows 8-15 what
@@ -226,13 +246,10 @@ constexpr int AT_THREADS = AT_WARPS * 32;
 constexpr int AT_COMB = 4;                /* heads that the warps of a CTA put together at a time */
 
 template <int KV>
-struct AttType;
-template <>
-struct AttType<KC_F32> { static constexpr int ES = 4, TP = 8; };
-template <>
-struct AttType<KC_F16> { static constexpr int ES = 2, TP = 16; };
-template <>
-struct AttType<KC_Q8_0> { static constexpr int ES = 1, TP = 32; };
+constexpr int att_es() { return KV == KC_F32 ? 4 : (KV == KC_F16 ? 2 : 1); }
+/* positions of a warp's tile: 32 * TM bytes of each dimension */
+template <int KV, int TM>
+constexpr int att_tp() { return 32 / att_es<KV>() * TM; }
 
 struct AttendArgs {
     PagedKV kv;
@@ -243,9 +260,10 @@ struct AttendArgs {
     int n_seqs, n_heads, group, chunks;   /* chunks: head chunks per KV head */
     int window;
     float scale, softcap;
-    int min_quanta;                       /* least quanta of a CTA's share */
-    float *part;                          /* [2 * CTAs] partial results */
-    int4 *desc;                           /* [CTAs] what to join */
+    int unit_cost;                        /* a unit's own time, in quanta */
+    int min_share;                        /* least such time of a CTA's share */
+    unsigned *count;                      /* [CTAs] pieces that have come, of the unit that ends there; 0 between calls */
+    float *part;                          /* [2 * CTAs] pieces */
     unsigned *err;
 };
 
@@ -321,11 +339,19 @@ __device__ __forceinline__ int seq_span(const AttendArgs &a, int b, int &first, 
 }
 
 /* Shared memory of a warp's ring slot: K rows, V rows, and (8-bit) their scales. */
-template <int KV, int HD>
-constexpr int slot_bytes() { return 2 * 32 * HD + (KV == KC_Q8_0 ? 2 * 32 * 4 : 0); }
-template <int KV, int HD, int MT, int S>
+template <int KV, int HD, int TM>
+constexpr int slot_bytes() {
+    return 2 * 32 * TM * HD + (KV == KC_Q8_0 ? 2 * att_tp<KV, TM>() * 4 : 0);
+}
+template <int KV, int HD, int TM, int MT, int S>
 constexpr int attend_smem() {
-    return AT_WARPS * (S * (slot_bytes<KV, HD>() + 16) + AT_COMB * HD * 4 + 2 * 8 * MT * 4);
+    return AT_WARPS * (S * (slot_bytes<KV, HD, TM>() + 16) + AT_COMB * HD * 4 + 2 * 8 * MT * 4);
+}
+
+/* The share of CTA i of n of `total`: [i total / n, (i + 1) total / n); the owner of x. */
+__device__ __forceinline__ long long share_lo(long long i, long long n, long long total) { return i * total / n; }
+__device__ __forceinline__ int share_owner(long long x, long long n, long long total) {
+    return (int)(((x + 1) * n - 1) / total);
 }
 
 /* sum / weights; nothing attended gives zeros */
@@ -334,15 +360,61 @@ __device__ __forceinline__ float4 over(float4 o, float l) {
     return make_float4(o.x * inv, o.y * inv, o.z * inv, o.w * inv);
 }
 
-/* The share of CTA i of n of `total` quanta: [i total / n, (i + 1) total / n). */
-__device__ __forceinline__ long long share_lo(long long i, long long n, long long total) { return i * total / n; }
+/* The pieces of CTAs c0..c1 of one unit, in that order, into the output. */
+template <int HD, int MT>
+__device__ __noinline__ void join_pieces(const AttendArgs &a, int b, int u, int c0, int c1) {
+    constexpr int HC = 8 * MT, PF = part_floats<HD, MT>(), UN = 8;
+    const int g = u / a.chunks, h0 = (u - g * a.chunks) * HC, nh = min(HC, a.group - h0);
+    auto piece = [&](int c) { return a.part + ((size_t)2 * c + (c == c0 ? 1 : 0)) * PF; };
+    for (int idx = threadIdx.x; idx < nh * (HD / 4); idx += AT_THREADS) {
+        const int h = idx / (HD / 4), e = 4 * (idx - h * (HD / 4));
+        float M = -INFINITY, L = 0.0f;
+        float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        for (int k0 = c0; k0 <= c1; k0 += UN) {
+            float m[UN], l[UN];
+            float4 t[UN];
+#pragma unroll
+            for (int i = 0; i < UN; i++) {
+                m[i] = -INFINITY;
+                l[i] = 0.0f;
+                t[i] = o;
+                if (k0 + i <= c1) {
+                    const float *p = piece(k0 + i);
+                    m[i] = __ldcg(p + HC * HD + h);
+                    l[i] = __ldcg(p + HC * HD + HC + h);
+                    t[i] = __ldcg((const float4 *)(p + h * HD + e));
+                }
+            }
+            float mn = M;
+#pragma unroll
+            for (int i = 0; i < UN; i++) mn = fmaxf(mn, m[i]);
+            const float base = mn == -INFINITY ? 0.0f : mn, f0 = exp2f(M - base);
+            M = mn;
+            L *= f0;
+            o = make_float4(o.x * f0, o.y * f0, o.z * f0, o.w * f0);
+#pragma unroll
+            for (int i = 0; i < UN; i++)
+                if (k0 + i <= c1) {
+                    const float f = exp2f(m[i] - base);
+                    L += f * l[i];
+                    o.x += f * t[i].x;
+                    o.y += f * t[i].y;
+                    o.z += f * t[i].z;
+                    o.w += f * t[i].w;
+                }
+        }
+        if (e < a.kv.hd) *(float4 *)(a.out + b * a.ldo + (size_t)(g * a.group + h0 + h) * a.kv.hd + e) = over(o, L);
+    }
+}
 
-template <int KV, int HD, int MT, int S>
-__global__ void __launch_bounds__(AT_THREADS, HD <= 128 ? 2 : 1) paged_attend_kernel(const __grid_constant__ AttendArgs a) {
-    constexpr int ES = AttType<KV>::ES, TP = AttType<KV>::TP, QP = AT_WARPS * TP;
+template <int KV, int HD, int TM, int MT, int S, int OCC>
+__global__ void __launch_bounds__(AT_THREADS, OCC) paged_attend_kernel(const __grid_constant__ AttendArgs a) {
+    constexpr int ES = att_es<KV>(), TP = att_tp<KV, TM>(), QP = AT_WARPS * TP;
     constexpr int PITCH = HD * ES, CPR = PITCH / 16;   /* bytes and 16-byte chunks of a row */
     constexpr int NT = TP / 8;                         /* 8-position column blocks of the scores */
-    constexpr int SLOT = slot_bytes<KV, HD>();
+    constexpr int LK = TP > 32 ? TP / 32 : 1;          /* tile rows whose page a lane looks up */
+    constexpr int RW = TP / LK;
+    constexpr int SLOT = slot_bytes<KV, HD, TM>(), VOFF = TP * PITCH, DOFF = 2 * TP * PITCH;
     constexpr int HC = 8 * MT;
     extern __shared__ __align__(128) unsigned char at_raw[];
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
@@ -353,25 +425,27 @@ __global__ void __launch_bounds__(AT_THREADS, HD <= 128 ? 2 : 1) paged_attend_ke
     float *cml = comb + AT_WARPS * AT_COMB * HD;                      /* and their maxima and weights' sums */
     const uint32_t ring_s = smem_u32(ring);
     const int U = a.kv.n_kv * a.chunks;                /* units per sequence */
-
-    cudaTriggerProgrammaticLaunchCompletion();
+    const int W = a.unit_cost;
 
     /* ---- this CTA's share ---- */
     __shared__ long long s_sum[AT_WARPS];
-    __shared__ long long s_lo, s_total;
-    __shared__ int s_b, s_cnt, s_ncta;
-    __shared__ long long s_base;                       /* quanta of the sequences before s_b */
+    __shared__ long long s_lo, s_hi, s_total;
+    __shared__ int s_b, s_ncta, s_last;
+    __shared__ long long s_base;                       /* the time of the sequences before s_b */
     {
         const int per = (a.n_seqs + AT_THREADS - 1) / AT_THREADS;
         const int b0 = min(tid * per, a.n_seqs), b1 = min(b0 + per, a.n_seqs);
+        auto unit_time = [&](int b, bool &bad) {
+            int f;
+            const int n = seq_span(a, b, f, bad);
+            return n > 0 ? (n - f + QP - 1) / QP + W : 0;
+        };
         long long sum = 0;
         bool any_bad = false;
         for (int b = b0; b < b1; b++) {
-            int f;
             bool bad;
-            const int n = seq_span(a, b, f, bad);
+            sum += unit_time(b, bad);
             any_bad |= bad;
-            sum += (n - f + QP - 1) / QP;
         }
         if (any_bad && blockIdx.x == 0) atomicOr(a.err, (unsigned)SE_LEN);
         long long pre = sum;
@@ -381,7 +455,6 @@ __global__ void __launch_bounds__(AT_THREADS, HD <= 128 ? 2 : 1) paged_attend_ke
             if (lane >= o) pre += t;
         }
         if (lane == 31) s_sum[warp] = pre;
-        if (tid == 0) s_b = a.n_seqs;
         __syncthreads();
         long long off = 0, all = 0;
 #pragma unroll
@@ -389,33 +462,32 @@ __global__ void __launch_bounds__(AT_THREADS, HD <= 128 ? 2 : 1) paged_attend_ke
             if (w < warp) off += s_sum[w];
             all += s_sum[w];
         }
-        pre += off - sum;                              /* quanta per unit before b0 */
+        pre += off - sum;                              /* a unit's worth of the time before b0 */
         const long long total = all * U;
-        const long long ncta = max(1ll, min((long long)gridDim.x, (total + a.min_quanta - 1) / a.min_quanta));
-        const long long lo = blockIdx.x < ncta ? share_lo(blockIdx.x, ncta, total) : total;
-        const long long hi = blockIdx.x < ncta ? share_lo(blockIdx.x + 1, ncta, total) : total;
+        const long long ncta = max(1ll, min((long long)gridDim.x, total / a.min_share));
+        const bool on = blockIdx.x < ncta;
+        const long long lo = on ? share_lo(blockIdx.x, ncta, total) : total;
+        const long long hi = on ? share_lo(blockIdx.x + 1, ncta, total) : total;
         if (lo < hi && lo >= pre * U && lo < (pre + sum) * U) {
             long long at = pre;
             int b = b0;
             for (; b < b1; b++) {
-                int f;
                 bool bad;
-                const int n = seq_span(a, b, f, bad), nq = (n - f + QP - 1) / QP;
-                if (lo < (at + nq) * U) break;
-                at += nq;
+                const int t = unit_time(b, bad);
+                if (lo < (at + t) * U) break;
+                at += t;
             }
             s_b = b;
             s_base = at * U;
-            s_lo = lo;
         }
         if (tid == 0) {
-            s_cnt = (int)(hi - lo);
+            s_lo = lo;
+            s_hi = hi;
             s_ncta = (int)ncta;
             s_total = total;
         }
         __syncthreads();
     }
-    const int cnt = s_cnt;
     /* sequences without positions: zeros */
     for (int b = blockIdx.x; b < a.n_seqs; b += gridDim.x) {
         int f;
@@ -423,49 +495,68 @@ __global__ void __launch_bounds__(AT_THREADS, HD <= 128 ? 2 : 1) paged_attend_ke
         if (seq_span(a, b, f, bad) == 0)
             for (int i = tid; i < a.n_heads * a.kv.hd; i += AT_THREADS) a.out[b * a.ldo + i] = 0.0f;
     }
-    if (cnt == 0) {
-        if (tid == 0) a.desc[blockIdx.x] = make_int4(-1, 0, 0, 0);
-        return;
-    }
+    if (s_lo >= s_hi) return;
 
     /* ---- the loader's place: sequence, unit of it, quantum of that ---- */
     int lb = s_b, first, len, nq, lu, lq;
+    long long ubase;                                   /* where the loader's unit begins */
+    int left;                                          /* time to the share's end */
     bool bad_;
     len = seq_span(a, lb, first, bad_);
     nq = (len - first + QP - 1) / QP;
     {
         const long long rel = s_lo - s_base;
-        lu = (int)(rel / nq);
-        lq = (int)(rel - (long long)lu * nq);
+        lu = (int)(rel / (nq + W));
+        const int off = (int)(rel - (long long)lu * (nq + W));
+        lq = max(0, off - W);
+        ubase = s_lo - off;
+        left = (int)(s_hi - ubase) - W - lq;
     }
-    const int b0_ = lb, u0_ = lu, lq0 = lq;                                /* the first unit's quanta before this share */
-    const long long unit0_at = s_base + (long long)lu * nq;   /* where the first unit begins */
-    int left = cnt;
-    const int prow = lane & (TP - 1);                  /* the tile row whose page this lane looks up */
-    int pg = -1, pslot = 0;
-    bool pin = false;
-    auto look = [&]() {                                /* page of the lane's row of the loader's tile */
-        const int p = first + (lq * AT_WARPS + warp) * TP + prow;
-        pin = p < len;
-        if (pin) {
-            const int pi = p / a.kv.page;
-            pslot = p - pi * a.kv.page;
-            pg = __ldg(a.kv.table + (size_t)lb * a.kv.ld_table + pi);
+    if (left <= 0) return;
+    const bool whole0 = lq == 0;                       /* the first unit begins in this share */
+    const int nq0 = nq;
+    const long long ubase0 = ubase;
+    const int prow = lane & (RW - 1);
+    int pg[LK], pslot[LK];
+    bool pin[LK];
+    auto look = [&]() {                                /* pages of the lane's rows of the loader's tile */
+#pragma unroll
+        for (int k = 0; k < LK; k++) {
+            const int p = first + (lq * AT_WARPS + warp) * TP + k * RW + prow;
+            pin[k] = p < len;
+            pg[k] = -1;
+            pslot[k] = 0;
+            if (pin[k]) {
+                const int pi = p / a.kv.page;
+                pslot[k] = p - pi * a.kv.page;
+                pg[k] = __ldg(a.kv.table + (size_t)lb * a.kv.ld_table + pi);
+            }
         }
     };
+    enum { LAST_OF_UNIT = 1 << 28, LAST_OF_SHARE = 1 << 29 };
+    int issued = 0;
     auto issue = [&](int stage) {
         const int g = lu / a.chunks;
-        const bool ok = pin && pg >= 0 && pg < a.kv.n_pages;
-        if (pin && !ok) atomicOr(a.err, (unsigned)SE_PAGE);
-        const unsigned live = __ballot_sync(0xffffffffu, ok) & (unsigned)((1ull << TP) - 1);
-        const unsigned row = ok ? (unsigned)(((size_t)pg * a.kv.n_kv + g) * a.kv.page + pslot) : 0u;
-        const uint32_t sk = ring_s + stage * SLOT, sv = sk + 32 * HD;
-        const size_t rowb = (size_t)a.kv.hd * ES;
+        issued++;
+        unsigned live[LK], row[LK];
+        const uint32_t sk = ring_s + stage * SLOT;
 #pragma unroll
-        for (int e = 0; e < HD / 16; e++) {
-            const int idx = lane + 32 * e, t = idx / CPR, ch = idx % CPR;
-            const unsigned rr = __shfl_sync(0xffffffffu, row, t);
-            const bool lv = ((live >> t) & 1u) && ch * 16 < (int)rowb;
+        for (int k = 0; k < LK; k++) {
+            const bool ok = pin[k] && pg[k] >= 0 && pg[k] < a.kv.n_pages;
+            if (pin[k] && !ok) atomicOr(a.err, (unsigned)SE_PAGE);
+            live[k] = __ballot_sync(0xffffffffu, ok) & (unsigned)((1ull << RW) - 1);
+            row[k] = ok ? (unsigned)(((size_t)pg[k] * a.kv.n_kv + g) * a.kv.page + pslot[k]) : 0u;
+            if constexpr (KV == KC_Q8_0) {
+                cp_async4z(sk + DOFF + (k * 32 + lane) * 4, a.kv.kd + row[k], ok);
+                cp_async4z(sk + DOFF + (TP + k * 32 + lane) * 4, a.kv.vd + row[k], ok);
+            }
+        }
+        const unsigned rowb = (unsigned)a.kv.hd * ES;
+#pragma unroll
+        for (int e = 0; e < TP * CPR / 32; e++) {
+            const int idx = lane + 32 * e, t = idx / CPR, ch = idx % CPR, k = (32 * e / CPR) / RW;
+            const unsigned rr = __shfl_sync(0xffffffffu, row[k], t & (RW - 1));
+            const bool lv = ((live[k] >> (t & (RW - 1))) & 1u) && ch * 16 < (int)rowb;
             const size_t off = (size_t)rr * rowb + (lv ? ch * 16 : 0);
             int kx, vx;                                /* swizzles: which of 8 bank groups a row starts at */
             if constexpr (KV == KC_F32) {
@@ -475,18 +566,20 @@ __global__ void __launch_bounds__(AT_THREADS, HD <= 128 ? 2 : 1) paged_attend_ke
                 kx = vx = CPR >= 8 ? (t & 7) : ((t >> 1) & 3);
             }
             cp_async16z(sk + t * PITCH + ((ch ^ kx) << 4), a.kv.k + off, lv);
-            cp_async16z(sv + t * PITCH + ((ch ^ vx) << 4), a.kv.v + off, lv);
+            cp_async16z(sk + VOFF + t * PITCH + ((ch ^ vx) << 4), a.kv.v + off, lv);
         }
-        if constexpr (KV == KC_Q8_0) {
-            cp_async4z(sk + 64 * HD + lane * 4, a.kv.kd + row, ok);
-            cp_async4z(sk + 64 * HD + 128 + lane * 4, a.kv.vd + row, ok);
+        if (lane == 0) {
+            const bool eu = lq == nq - 1;
+            const int f = (eu ? LAST_OF_UNIT : 0) | (left <= (eu ? 1 + W : 1) ? LAST_OF_SHARE : 0);
+            info[stage] = make_int4(lb, lu | f, (int)live[0], LK > 1 ? (int)live[LK - 1] : 0);
         }
-        if (lane == 0) info[stage] = make_int4(lb, lu, (int)live, (lq == nq - 1 || left == 1) ? (lq == nq - 1 ? 3 : 1) : 0);
     };
     auto advance = [&]() {
-        left--;
-        if (left == 0) return;
-        if (++lq == nq) {
+        const bool eu = lq == nq - 1;
+        left -= eu ? 1 + W : 1;
+        if (left <= 0) return;
+        if (eu) {
+            ubase += nq + W;
             lq = 0;
             if (++lu == U) {
                 lu = 0;
@@ -499,6 +592,8 @@ __global__ void __launch_bounds__(AT_THREADS, HD <= 128 ? 2 : 1) paged_attend_ke
                     nq = (len - first + QP - 1) / QP;
                 } while (nq == 0);
             }
+        } else {
+            lq++;
         }
         look();
     };
@@ -511,6 +606,7 @@ __global__ void __launch_bounds__(AT_THREADS, HD <= 128 ? 2 : 1) paged_attend_ke
         }
         cp_async_commit();
     }
+    __syncwarp();
 
     /* ---- the compute side ---- */
     constexpr int QR = KV == KC_F32 ? HD / 8 * 4 : (KV == KC_F16 ? HD / 16 * 4 : HD / 32 * 2);
@@ -520,7 +616,7 @@ __global__ void __launch_bounds__(AT_THREADS, HD <= 128 ? 2 : 1) paged_attend_ke
     float acc[MT][NACC], m[MT], l[MT];
     const float LOG2E = 1.4426950408889634f;
     int cu_b = -1, cu_u = -1;
-    bool fresh = true;                                 /* the unit of the next tile begins in this share */
+    bool fresh = true;                                 /* the current unit begins in this share */
 
     auto load_q = [&](int b, int u) {
         const int g = u / a.chunks, h0 = (u - g * a.chunks) * HC, nh = min(HC, a.group - h0);
@@ -603,8 +699,8 @@ __global__ void __launch_bounds__(AT_THREADS, HD <= 128 ? 2 : 1) paged_attend_ke
     };
 
     /* one tile of TP positions in ring slot `stage` */
-    auto compute = [&](int stage, unsigned live) {
-        const uint32_t sk = ring_s + stage * SLOT, sv = sk + 32 * HD;
+    auto compute = [&](int stage, const unsigned (&live)[LK]) {
+        const uint32_t sk = ring_s + stage * SLOT, sv = sk + VOFF;
         float s[MT][NT][2];
         if constexpr (KV == KC_F16) {
             float d[MT][NT][4];
@@ -638,36 +734,42 @@ __global__ void __launch_bounds__(AT_THREADS, HD <= 128 ? 2 : 1) paged_attend_ke
                     s[mt][nt][1] = (d[mt][nt][1] + d[mt][nt][3]) * qc[mt];
                 }
         } else if constexpr (KV == KC_F32) {
-            float dh[MT][4], dl[MT][4];
+            float dh[MT][NT][4], dl[MT][NT][4];
 #pragma unroll
             for (int mt = 0; mt < MT; mt++)
 #pragma unroll
-                for (int i = 0; i < 4; i++) dh[mt][i] = dl[mt][i] = 0.0f;
+                for (int nt = 0; nt < NT; nt++)
+#pragma unroll
+                    for (int i = 0; i < 4; i++) dh[mt][nt][i] = dl[mt][nt][i] = 0.0f;
             const uint32_t kb = sk + r * PITCH;
             const int x = c ^ (((r & 1) << 2) | (r >> 1));
 #pragma unroll
-            for (int jj = 0; jj < HD / 16; jj++) {
-                const float4 t = lds4(kb + (((4 * jj) ^ x) << 4));
-                unsigned h[4], w[4];
-                split_tf32(t.x, h[0], w[0]);
-                split_tf32(t.y, h[1], w[1]);
-                split_tf32(t.z, h[2], w[2]);
-                split_tf32(t.w, h[3], w[3]);
+            for (int jj = 0; jj < HD / 16; jj++)
 #pragma unroll
-                for (int mt = 0; mt < MT; mt++) {
-                    const unsigned a0[4] = { qf[mt][8 * jj], qf[mt][8 * jj + 1], qf[mt][8 * jj + 2], qf[mt][8 * jj + 3] };
-                    const unsigned a1[4] = { qf[mt][8 * jj + 4], qf[mt][8 * jj + 5], qf[mt][8 * jj + 6], qf[mt][8 * jj + 7] };
-                    mma_tf32(dh[mt], a0, h[0], h[1]);
-                    mma_tf32(dl[mt], a0, w[0], w[1]);
-                    mma_tf32(dh[mt], a1, h[2], h[3]);
-                    mma_tf32(dl[mt], a1, w[2], w[3]);
+                for (int nt = 0; nt < NT; nt++) {
+                    const float4 t = lds4(kb + nt * 8 * PITCH + (((4 * jj) ^ x) << 4));
+                    unsigned h[4], w[4];
+                    split_tf32(t.x, h[0], w[0]);
+                    split_tf32(t.y, h[1], w[1]);
+                    split_tf32(t.z, h[2], w[2]);
+                    split_tf32(t.w, h[3], w[3]);
+#pragma unroll
+                    for (int mt = 0; mt < MT; mt++) {
+                        const unsigned a0[4] = { qf[mt][8 * jj], qf[mt][8 * jj + 1], qf[mt][8 * jj + 2], qf[mt][8 * jj + 3] };
+                        const unsigned a1[4] = { qf[mt][8 * jj + 4], qf[mt][8 * jj + 5], qf[mt][8 * jj + 6], qf[mt][8 * jj + 7] };
+                        mma_tf32(dh[mt][nt], a0, h[0], h[1]);
+                        mma_tf32(dl[mt][nt], a0, w[0], w[1]);
+                        mma_tf32(dh[mt][nt], a1, h[2], h[3]);
+                        mma_tf32(dl[mt][nt], a1, w[2], w[3]);
+                    }
                 }
-            }
 #pragma unroll
-            for (int mt = 0; mt < MT; mt++) {
-                s[mt][0][0] = ((dh[mt][0] + dh[mt][2]) + (dl[mt][0] + dl[mt][2])) * qc[mt];
-                s[mt][0][1] = ((dh[mt][1] + dh[mt][3]) + (dl[mt][1] + dl[mt][3])) * qc[mt];
-            }
+            for (int mt = 0; mt < MT; mt++)
+#pragma unroll
+                for (int nt = 0; nt < NT; nt++) {
+                    s[mt][nt][0] = ((dh[mt][nt][0] + dh[mt][nt][2]) + (dl[mt][nt][0] + dl[mt][nt][2])) * qc[mt];
+                    s[mt][nt][1] = ((dh[mt][nt][1] + dh[mt][nt][3]) + (dl[mt][nt][1] + dl[mt][nt][3])) * qc[mt];
+                }
         } else {
             int d[MT][NT][4];
 #pragma unroll
@@ -690,7 +792,7 @@ __global__ void __launch_bounds__(AT_THREADS, HD <= 128 ? 2 : 1) paged_attend_ke
                         mma_s8(d[mt][nt], qf[mt][4 * jj + 2], qf[mt][4 * jj + 3], b[2], b[3]);
                     }
                 }
-            const float *kd = (const float *)(ring + stage * SLOT + 64 * HD);
+            const float *kd = (const float *)(ring + stage * SLOT + DOFF);
 #pragma unroll
             for (int nt = 0; nt < NT; nt++) {
                 const float2 e = *(const float2 *)(kd + nt * 8 + 2 * c);
@@ -713,7 +815,7 @@ __global__ void __launch_bounds__(AT_THREADS, HD <= 128 ? 2 : 1) paged_attend_ke
                 for (int i = 0; i < 2; i++) {
                     float v = s[mt][nt][i];
                     if (a.softcap > 0.0f) v = a.softcap * tanhf(__fdiv_rn(v, a.softcap)) * LOG2E;
-                    v = (live >> (nt * 8 + 2 * c + i)) & 1u ? v : -INFINITY;
+                    v = (live[nt * 8 / RW] >> ((nt * 8) % RW + 2 * c + i)) & 1u ? v : -INFINITY;
                     s[mt][nt][i] = v;
                     mx = fmaxf(mx, v);
                 }
@@ -735,67 +837,99 @@ __global__ void __launch_bounds__(AT_THREADS, HD <= 128 ? 2 : 1) paged_attend_ke
         }
         /* the weighted sum of V's rows */
         if constexpr (KV == KC_F16) {
-            unsigned w[MT][4];
+            constexpr int KS = TP / 16;
+            unsigned w[MT][KS][4];
 #pragma unroll
-            for (int mt = 0; mt < MT; mt++) {
-                split_f16(s[mt][0][0], s[mt][0][1], w[mt][0], w[mt][1]);
-                split_f16(s[mt][1][0], s[mt][1][1], w[mt][2], w[mt][3]);
-            }
+            for (int mt = 0; mt < MT; mt++)
+#pragma unroll
+                for (int nt = 0; nt < NT; nt++)
+                    split_f16(s[mt][nt][0], s[mt][nt][1], w[mt][nt >> 1][2 * (nt & 1)], w[mt][nt >> 1][2 * (nt & 1) + 1]);
             const uint32_t vb = sv + ((lane & 7) + (lane & 8)) * PITCH;
             const int x = (lane >> 4) ^ (lane & 7);
 #pragma unroll
             for (int jj = 0; jj < HD / 16; jj++) {
-                unsigned b[4];
-                ldsm4t(b, vb + (((2 * jj) ^ x) << 4));
+                float d[MT][2][4];
+#pragma unroll
+                for (int mt = 0; mt < MT; mt++)
+#pragma unroll
+                    for (int i = 0; i < 4; i++) d[mt][0][i] = d[mt][1][i] = 0.0f;
+#pragma unroll
+                for (int ks = 0; ks < KS; ks++) {
+                    unsigned b[4];
+                    ldsm4t(b, vb + ks * 16 * PITCH + (((2 * jj) ^ x) << 4));
+#pragma unroll
+                    for (int mt = 0; mt < MT; mt++) {
+                        mma_f16(d[mt][0], w[mt][ks], b[0], b[1]);
+                        mma_f16(d[mt][1], w[mt][ks], b[2], b[3]);
+                    }
+                }
 #pragma unroll
                 for (int mt = 0; mt < MT; mt++) {
-                    float d0[4] = { 0.0f, 0.0f, 0.0f, 0.0f }, d1[4] = { 0.0f, 0.0f, 0.0f, 0.0f };
-                    mma_f16(d0, w[mt], b[0], b[1]);
-                    mma_f16(d1, w[mt], b[2], b[3]);
                     float *o = &acc[mt][4 * jj];
-                    o[0] = o[0] * corr[mt] + (d0[0] + d0[2]);
-                    o[1] = o[1] * corr[mt] + (d0[1] + d0[3]);
-                    o[2] = o[2] * corr[mt] + (d1[0] + d1[2]);
-                    o[3] = o[3] * corr[mt] + (d1[1] + d1[3]);
+                    o[0] = o[0] * corr[mt] + (d[mt][0][0] + d[mt][0][2]);
+                    o[1] = o[1] * corr[mt] + (d[mt][0][1] + d[mt][0][3]);
+                    o[2] = o[2] * corr[mt] + (d[mt][1][0] + d[mt][1][2]);
+                    o[3] = o[3] * corr[mt] + (d[mt][1][1] + d[mt][1][3]);
                 }
             }
         } else if constexpr (KV == KC_F32) {
-            unsigned w[MT][4];
+            unsigned w[MT][NT][4];
 #pragma unroll
-            for (int mt = 0; mt < MT; mt++) {
-                split_tf32(s[mt][0][0], w[mt][0], w[mt][1]);
-                split_tf32(s[mt][0][1], w[mt][2], w[mt][3]);
-            }
+            for (int mt = 0; mt < MT; mt++)
+#pragma unroll
+                for (int nt = 0; nt < NT; nt++) {
+                    split_tf32(s[mt][nt][0], w[mt][nt][0], w[mt][nt][1]);
+                    split_tf32(s[mt][nt][1], w[mt][nt][2], w[mt][nt][3]);
+                }
             const uint32_t v0 = sv + (2 * c) * PITCH, v1 = v0 + PITCH;
             const int x0 = r ^ (2 * c), x1 = r ^ (2 * c + 1);
 #pragma unroll
             for (int j = 0; j < HD / 32; j++) {
-                const float4 ya = lds4(v0 + (((8 * j) ^ x0) << 4)), yb = lds4(v1 + (((8 * j) ^ x1) << 4));
-                const float y0[4] = { ya.x, ya.y, ya.z, ya.w }, y1[4] = { yb.x, yb.y, yb.z, yb.w };
+                float d[MT][4][4];
 #pragma unroll
-                for (int i = 0; i < 4; i++) {
-                    unsigned h0, h1, g0, g1;
-                    split_tf32(y0[i], h0, g0);
-                    split_tf32(y1[i], h1, g1);
+                for (int mt = 0; mt < MT; mt++)
 #pragma unroll
-                    for (int mt = 0; mt < MT; mt++) {
-                        float d0[4] = { 0.0f, 0.0f, 0.0f, 0.0f };
-                        mma_tf32(d0, w[mt], g0, g1);
-                        mma_tf32(d0, w[mt], h0, h1);
-                        float *o = &acc[mt][8 * j + i];
-                        o[0] = o[0] * corr[mt] + (d0[0] + d0[2]);
-                        o[4] = o[4] * corr[mt] + (d0[1] + d0[3]);
+                    for (int i = 0; i < 4; i++)
+#pragma unroll
+                        for (int k = 0; k < 4; k++) d[mt][i][k] = 0.0f;
+#pragma unroll
+                for (int nt = 0; nt < NT; nt++) {
+                    const float4 ya = lds4(v0 + nt * 8 * PITCH + (((8 * j) ^ x0) << 4));
+                    const float4 yb = lds4(v1 + nt * 8 * PITCH + (((8 * j) ^ x1) << 4));
+                    const float y0[4] = { ya.x, ya.y, ya.z, ya.w }, y1[4] = { yb.x, yb.y, yb.z, yb.w };
+#pragma unroll
+                    for (int i = 0; i < 4; i++) {
+                        unsigned h0, h1, g0, g1;
+                        split_tf32(y0[i], h0, g0);
+                        split_tf32(y1[i], h1, g1);
+#pragma unroll
+                        for (int mt = 0; mt < MT; mt++) {
+                            mma_tf32(d[mt][i], w[mt][nt], g0, g1);
+                            mma_tf32(d[mt][i], w[mt][nt], h0, h1);
+                        }
                     }
                 }
+#pragma unroll
+                for (int mt = 0; mt < MT; mt++)
+#pragma unroll
+                    for (int i = 0; i < 4; i++) {
+                        float *o = &acc[mt][8 * j + i];
+                        o[0] = o[0] * corr[mt] + (d[mt][i][0] + d[mt][i][2]);
+                        o[4] = o[4] * corr[mt] + (d[mt][i][1] + d[mt][i][3]);
+                    }
             }
         } else {
             /* the rows' scales join the weights; a power of two keeps the product in f16's range */
-            const float *vd = (const float *)(ring + stage * SLOT + 64 * HD + 128);
-            const float top = warp_max(fabsf(vd[lane]));
+            constexpr int KS = TP / 16;
+            const float *vd = (const float *)(ring + stage * SLOT + DOFF) + TP;
+            float top = fabsf(vd[lane]);
+#pragma unroll
+            for (int k = 1; k < LK; k++) top = fmaxf(top, fabsf(vd[k * 32 + lane]));
+            top = warp_max(top);
             int ex = (int)((__float_as_uint(top) >> 23) & 255) - 127;
             ex = min(max(ex, -100), 100);
             const float dn = __uint_as_float((unsigned)(127 - 1 - ex) << 23), upf = __uint_as_float((unsigned)(127 + 1 + ex) << 23);
-            unsigned w[MT][2][4];
+            unsigned w[MT][KS][4];
 #pragma unroll
             for (int nt = 0; nt < NT; nt++) {
                 const float2 e = *(const float2 *)(vd + nt * 8 + 2 * c);
@@ -824,7 +958,7 @@ __global__ void __launch_bounds__(AT_THREADS, HD <= 128 ? 2 : 1) paged_attend_ke
 #pragma unroll
                         for (int i = 0; i < 4; i++) d[mt][k][i] = 0.0f;
 #pragma unroll
-                for (int ks = 0; ks < 2; ks++) {
+                for (int ks = 0; ks < KS; ks++) {
                     unsigned b[4];
                     ldsm4t(b, vb + ks * 16 * PITCH + (((2 * jj) ^ x) << 4));
                     unsigned e0, o0, e1, o1;
@@ -938,21 +1072,35 @@ __global__ void __launch_bounds__(AT_THREADS, HD <= 128 ? 2 : 1) paged_attend_ke
         }
     };
 
-    bool join = false, first_unit = true;
-    for (int it = 0; it < cnt; it++) {
-        cp_async_wait_but<S - 2>();
-        __syncwarp();
-        if (left > 0) {
-            issue((it + S - 1) % S);
-            advance();
+    __shared__ int s_c0, s_c1;
+    auto leave = [&](int b, int u) {                   /* the unit's piece is written: join them if it was the last */
+        __threadfence();
+        __syncthreads();
+        if (tid == 0) {
+            /* a unit that is not fresh is the share's first, one that is left unfinished its last */
+            const long long x = (fresh ? ubase : ubase0) + W;
+            const int c0 = share_owner(x, s_ncta, s_total);
+            const int c1 = share_owner(x + (fresh ? nq : nq0) - 1, s_ncta, s_total);
+            const unsigned n = atomicAdd(a.count + c1, 1u);
+            s_last = n == (unsigned)(c1 - c0);
+            if (s_last) a.count[c1] = 0u;
+            s_c0 = c0;
+            s_c1 = c1;
+            __threadfence();
         }
-        cp_async_commit();
+        __syncthreads();
+        if (s_last) join_pieces<HD, MT>(a, b, u, s_c0, s_c1);
+    };
+
+    for (int it = 0; it < issued; it++) {
         const int stage = it % S;
-        const int4 f = info[stage];
-        if (f.x != cu_b || f.y != cu_u) {
+        const int4 f = info[stage];                    /* written when the slot's copies were issued */
+        const int fu = f.y & (LAST_OF_UNIT - 1);
+        if (f.x != cu_b || fu != cu_u) {
+            /* a new unit: its queries are on their way while the tile arrives */
             cu_b = f.x;
-            cu_u = f.y;
-            fresh = it > 0 || lq0 == 0;
+            cu_u = fu;
+            fresh = it > 0 || whole0;
             load_q(cu_b, cu_u);
 #pragma unroll
             for (int mt = 0; mt < MT; mt++) {
@@ -962,64 +1110,21 @@ __global__ void __launch_bounds__(AT_THREADS, HD <= 128 ? 2 : 1) paged_attend_ke
                 for (int i = 0; i < NACC; i++) acc[mt][i] = 0.0f;
             }
         }
-        if (f.z) compute(stage, (unsigned)f.z);
-        if (f.w & 1) {
-            if (first_unit) join = !fresh && (f.w & 2);
-            first_unit = false;
-            finish(cu_b, cu_u, fresh && (f.w & 2));
+        cp_async_wait_but<S - 2>();
+        __syncwarp();
+        if (left > 0) {
+            issue((it + S - 1) % S);
+            advance();
         }
-    }
-    /* the first unit began in another CTA's share and ends in this one: from which CTA on it is to be joined
-     * (the last whose share begins at or before the unit) */
-    if (tid == 0)
-        a.desc[blockIdx.x] =
-            join ? make_int4(b0_, u0_, (int)(((unit0_at + 1) * s_ncta - 1) / s_total), 0) : make_int4(-1, 0, 0, 0);
-}
-
-/* The pieces of units that more than one CTA's share holds, summed in the
- * CTAs' order: block i joins the unit whose last piece is CTA i's, a warp per
- * head. Few and small: its time is a launch's latency, part of which the
- * programmatic launch hides. */
-constexpr int JN_THREADS = 256;
-template <int HD, int MT>
-__global__ void __launch_bounds__(JN_THREADS) paged_join_kernel(const __grid_constant__ AttendArgs a) {
-    cudaGridDependencySynchronize();
-    const int4 d = a.desc[blockIdx.x];
-    if (d.x < 0) return;
-    constexpr int HC = 8 * MT, PF = part_floats<HD, MT>(), NV = HD > 128 ? 2 : 1;
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, c1 = blockIdx.x;
-    const int g = d.y / a.chunks, h0 = (d.y - g * a.chunks) * HC, nh = min(HC, a.group - h0);
-    auto piece = [&](int c) { return a.part + ((size_t)2 * c + (c == d.z ? 1 : 0)) * PF; };
-    for (int h = warp; h < nh; h += JN_THREADS / 32) {
-        float M = -INFINITY;
-        for (int k = d.z + lane; k <= c1; k += 32) M = fmaxf(M, piece(k)[HC * HD + h]);
-        M = warp_max(M);
-        const float base = M == -INFINITY ? 0.0f : M;
-        float4 o[NV];
-        float L = 0.0f;
-#pragma unroll
-        for (int j = 0; j < NV; j++) o[j] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-#pragma unroll 4
-        for (int k = d.z; k <= c1; k++) {
-            const float *p = piece(k);
-            const float f = exp2f(p[HC * HD + h] - base);
-            L += f * p[HC * HD + HC + h];
-#pragma unroll
-            for (int j = 0; j < NV; j++) {
-                const int e = 4 * lane + 128 * j;
-                if (e < HD) {
-                    const float4 t = *(const float4 *)(p + h * HD + e);
-                    o[j].x += f * t.x;
-                    o[j].y += f * t.y;
-                    o[j].z += f * t.z;
-                    o[j].w += f * t.w;
-                }
-            }
-        }
-#pragma unroll
-        for (int j = 0; j < NV; j++) {
-            const int e = 4 * lane + 128 * j;
-            if (e < a.kv.hd) *(float4 *)(a.out + d.x * a.ldo + (size_t)(g * a.group + h0 + h) * a.kv.hd + e) = over(o[j], L);
+        cp_async_commit();
+        unsigned live[LK];
+        live[0] = (unsigned)f.z;
+        if constexpr (LK > 1) live[1] = (unsigned)f.w;
+        if (f.z | f.w) compute(stage, live);
+        if (f.y & (LAST_OF_UNIT | LAST_OF_SHARE)) {
+            const bool complete = fresh && (f.y & LAST_OF_UNIT);
+            finish(cu_b, cu_u, complete);
+            if (!complete) leave(cu_b, cu_u);
         }
     }
 }

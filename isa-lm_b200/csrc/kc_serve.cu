@@ -139,8 +139,9 @@ static int take_cache(const kc_paged_kv *kv, const ServeDev &d, PagedKV &o) {
 template <int KV>
 static void launch_append(const AppendArgs &a, cudaStream_t st) {
     const int hd = a.kv.hd, lph = hd <= 32 ? 8 : (hd <= 64 ? 16 : 32);
-    const long long items = (long long)a.rows * (a.n_heads + 2 * a.kv.n_kv), per = AP_THREADS / lph;
-    const unsigned grid = (unsigned)((items + per - 1) / per);
+    const int hw = AP_HEADS * (32 / lph);
+    const long long warps = (long long)a.rows * ((a.n_heads + hw - 1) / hw + 2 * ((a.kv.n_kv + hw - 1) / hw));
+    const unsigned grid = (unsigned)((warps + AP_THREADS / 32 - 1) / (AP_THREADS / 32));
     if (lph == 8) append_kernel<KV, 8, 1><<<grid, AP_THREADS, 0, st>>>(a);
     else if (lph == 16) append_kernel<KV, 16, 1><<<grid, AP_THREADS, 0, st>>>(a);
     else if (hd <= 128) append_kernel<KV, 32, 1><<<grid, AP_THREADS, 0, st>>>(a);
@@ -149,32 +150,32 @@ static void launch_append(const AppendArgs &a, cudaStream_t st) {
 
 /* ------------------------------------------------------------ attention */
 
-/* One instance: its kernels, shared memory, and on each device the CTAs that fit. */
+/* The workspace: a counter for each CTA of any instance, zero between calls, and the pieces. */
+constexpr int AT_MAX_CTAS = 2048;
+
+/* One instance: its kernel, shared memory, and on each device the CTAs that fit. */
 struct AttendVariant {
     void (*attend)(const AttendArgs);
-    void (*join)(const AttendArgs);
-    int smem, part, quantum;
+    int smem, part;
     int ctas[SV_MAX_DEVICES];
 };
 
-template <int KV, int HD, int MT, int S>
+template <int KV, int HD, int TM, int MT, int S, int OCC>
 static AttendVariant make_variant() {
     AttendVariant v{};
-    v.attend = paged_attend_kernel<KV, HD, MT, S>;
-    v.join = paged_join_kernel<HD, MT>;
-    v.smem = attend_smem<KV, HD, MT, S>();
+    v.attend = paged_attend_kernel<KV, HD, TM, MT, S, OCC>;
+    v.smem = attend_smem<KV, HD, TM, MT, S>();
     v.part = part_floats<HD, MT>();
-    v.quantum = AT_WARPS * AttType<KV>::TP;
     return v;
 }
 
 template <int KV>
 static AttendVariant *variants_of(int hd, int group, int &mt) {
-    static AttendVariant v64 = make_variant<KV, 64, 1, 6>(), v128 = make_variant<KV, 128, 1, 3>(),
-                         v256 = make_variant<KV, 256, 1, 3>();
+    static AttendVariant v64 = make_variant<KV, 64, 2, 1, 3, 2>(), v128 = make_variant<KV, 128, 1, 1, 3, 2>(),
+                         v256 = make_variant<KV, 256, 1, 1, 3, 1>();
     if constexpr (KV != KC_F32) {
         /* more than 8 heads share a KV head: 16 at a time, so that the cache is read once */
-        static AttendVariant w64 = make_variant<KV, 64, 2, 6>(), w128 = make_variant<KV, 128, 2, 3>();
+        static AttendVariant w64 = make_variant<KV, 64, 2, 2, 3, 2>(), w128 = make_variant<KV, 128, 1, 2, 3, 2>();
         if (group > 8 && hd <= 128) {
             mt = 2;
             return hd <= 64 ? &w64 : &w128;
@@ -199,13 +200,13 @@ static int attend_variant(const kc_paged_kv *kv, int n_heads, const ServeDev &d,
             set_error("attend: no CTA fits an SM");
             return KC_E_IO;
         }
-        v->ctas[d.dev] = n * d.sms;
+        v->ctas[d.dev] = std::min(n * d.sms, AT_MAX_CTAS);
     }
     return KC_OK;
 }
 
 static size_t ws_bytes(const AttendVariant *v, int ctas) {
-    return (size_t)ctas * (sizeof(int4) + 2 * sizeof(float) * (size_t)v->part);
+    return sizeof(unsigned) * AT_MAX_CTAS + 2 * sizeof(float) * (size_t)v->part * (size_t)ctas;
 }
 
 }  // namespace kc
@@ -242,8 +243,8 @@ extern "C" int kc_paged_append_dev(const kc_paged_kv *kv, const kc_append_args *
     PTR(x->pos, 4);
     if (x->seqs) PTR(x->seqs, 4);
     if (x->q_norm) {
-        PTR(x->q_norm, 4);
-        PTR(x->k_norm, 4);
+        PTR(x->q_norm, 16);
+        PTR(x->k_norm, 16);
     }
     a.q = x->q; a.k = x->k; a.v = x->v; a.q_out = x->q_out;
     a.ldq = x->ldq; a.ldk = x->ldk; a.ldv = x->ldv; a.ldo = x->ldo;
@@ -259,6 +260,7 @@ extern "C" int kc_paged_append_dev(const kc_paged_kv *kv, const kc_append_args *
 
 static int check_heads(const kc_paged_kv *kv, int n_heads) {
     if (n_heads < 1 || n_heads % kv->n_kv_heads) return refuse("n_heads must be a multiple of n_kv_heads");
+    if (n_heads > 65536) return refuse("n_heads must be at most 65536");
     return KC_OK;
 }
 
@@ -275,6 +277,17 @@ extern "C" int kc_paged_attend_ws(const kc_paged_kv *kv, int n_heads, size_t *by
     if (rc != KC_OK) return rc;
     *bytes = ws_bytes(v, v->ctas[d.dev]);
     return KC_OK;
+}
+
+extern "C" int kc_paged_attend_ws_init(void *ws, size_t bytes) {
+    clear_error();
+    ServeDev d;
+    const int rc = serve_device(d);
+    if (rc != KC_OK) return rc;
+    PTR(ws, 16);
+    if (bytes < sizeof(unsigned) * AT_MAX_CTAS) return refuse("workspace too small (kc_paged_attend_ws)");
+    SK(cudaMemsetAsync(ws, 0, sizeof(unsigned) * AT_MAX_CTAS, nullptr), "workspace");
+    return sv_cuda(cudaStreamSynchronize(nullptr), "workspace");
 }
 
 extern "C" int kc_paged_attend_dev(const kc_paged_kv *kv, const kc_attend_args *x, void *stream) {
@@ -312,26 +325,13 @@ extern "C" int kc_paged_attend_dev(const kc_paged_kv *kv, const kc_attend_args *
     a.q = x->q; a.out = x->out; a.ldq = x->ldq; a.ldo = x->ldo; a.lens = x->lens;
     a.n_seqs = x->n_seqs; a.n_heads = x->n_heads; a.group = x->n_heads / kv->n_kv_heads;
     a.window = x->window; a.scale = x->scale; a.softcap = x->softcap;
-    a.min_quanta = 1;
-    a.desc = (int4 *)x->ws;
-    a.part = (float *)((char *)x->ws + sizeof(int4) * (size_t)ctas);
+    a.unit_cost = 2;
+    a.min_share = 1;
+    a.count = (unsigned *)x->ws;
+    a.part = (float *)((char *)x->ws + sizeof(unsigned) * AT_MAX_CTAS);
     a.err = d.err;
-    const cudaStream_t st = (cudaStream_t)stream;
-    v->attend<<<ctas, AT_THREADS, v->smem, st>>>(a);
-    SK(cudaGetLastError(), "attend");
-    /* a sequence of one quantum is never shared out: nothing to join */
-    if ((long long)kv->ld_table * kv->page_size <= v->quantum) return KC_OK;
-    cudaLaunchConfig_t cfg{};
-    cfg.gridDim = dim3((unsigned)ctas);
-    cfg.blockDim = dim3(JN_THREADS);
-    cfg.stream = st;
-    cudaLaunchAttribute at{};
-    at.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    at.val.programmaticStreamSerializationAllowed = 1;
-    cfg.attrs = &at;
-    cfg.numAttrs = 1;
-    SK(cudaLaunchKernelEx(&cfg, v->join, a), "attend join");
-    return KC_OK;
+    v->attend<<<ctas, AT_THREADS, v->smem, (cudaStream_t)stream>>>(a);
+    return sv_cuda(cudaGetLastError(), "attend");
 }
 
 /* ------------------------------------------------------------ logits */
@@ -372,7 +372,7 @@ extern "C" int kc_logits_process_dev(const kc_logits_args *x, void *stream) {
     LogitsArgs a{};
     a.in = x->in; a.out = x->out; a.ld_in = x->ld_in; a.ld_out = x->ld_out; a.vocab = x->vocab;
     a.hist = x->history; a.hist_len = x->history_len; a.ld_hist = x->ld_history; a.hist_cap = x->history_cap;
-    a.repeat = x->repeat; a.presence = x->presence; a.frequency = x->frequency; a.repeat1 = 1.0f;
+    a.repeat = x->repeat; a.presence = x->presence; a.frequency = x->frequency;
     a.bias_off = x->bias_off; a.bias_ids = x->bias_ids; a.bias_vals = x->bias_vals; a.n_bias = x->n_bias;
     a.mask = x->mask; a.ld_mask = x->ld_mask;
     a.err = d.err;

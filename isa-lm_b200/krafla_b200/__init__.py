@@ -19,6 +19,7 @@ Status codes and their meaning are the reference's ml_status (core/ml.h:7-14).
 """
 import ctypes as C
 import os
+import struct
 import sys
 
 import numpy as np
@@ -105,6 +106,7 @@ def lib():
             "kc_debug_ffn_split": (I, [I]),
             "kc_rope_tables": (I, [P, I, I, P, P]), "kc_paged_append_dev": (I, [P, P, P]),
             "kc_paged_attend_dev": (I, [P, P, P]), "kc_paged_attend_ws": (I, [P, I, C.POINTER(S)]),
+            "kc_paged_attend_ws_init": (I, [P, S]),
             "kc_logits_process_dev": (I, [P, P]),
         }
         for name, (res, args) in sig.items():
@@ -434,6 +436,12 @@ class DevArray(DevBuf):
     def data_ptr(self):
         return self.ptr
 
+    def is_contiguous(self):
+        return True
+
+    def numel(self):
+        return int(np.prod(self.shape, dtype=np.int64))
+
     def stride(self):
         return tuple(int(np.prod(self.shape[i + 1:], dtype=np.int64)) for i in range(len(self.shape)))
 
@@ -441,7 +449,18 @@ class DevArray(DevBuf):
         return self.get(self.dtype, int(np.prod(self.shape, dtype=np.int64))).reshape(self.shape)
 
 
-_TYPE_NAMES = {}      # dtype object (numpy's or torch's) -> "float32", "int32", ...
+class _Types:
+    """Names of the types that an argument may have, and the dtype objects (numpy's or torch's) known to be one."""
+
+    def __init__(self, *names):
+        self.names, self.known = names, set()
+
+    def check(self, dt, name):
+        if dt not in self.known:
+            t = str(dt).replace("torch.", "")
+            if t not in self.names:
+                raise _shape_error(f"{name} is {t}, not {' or '.join(self.names)}")
+            self.known.add(dt)
 
 
 def _shape_error(msg):
@@ -450,23 +469,20 @@ def _shape_error(msg):
     return e
 
 
-def _array(x, types, name):
-    """Checks an array's type; its shape."""
-    dt = x.dtype
-    t = _TYPE_NAMES.get(dt)
-    if t is None:
-        t = _TYPE_NAMES[dt] = str(dt).replace("torch.", "")
-    if t not in types:
-        raise _shape_error(f"{name} is {t}, not {' or '.join(types)}")
-    return x.shape
-
-
-_F, _I, _W = ("float32",), ("int32",), ("int32", "uint32")
+_F, _I, _W = _Types("float32"), _Types("int32"), _Types("int32", "uint32")
+_H, _B = _Types("float16"), _Types("int8")
 
 
 def _rows(x, types, n, width, name):
-    """Rows of `width` values, [n, width] or [n, ...] with contiguous rows: the row stride."""
-    shape, st = _array(x, types, name), x.stride()
+    """Rows of `width` values, [n, width] or [n, ...] with contiguous rows: the row stride.
+    (The first test settles the common case in a microsecond's third; the rest explains refusals.)"""
+    try:
+        if x.dtype in types.known and x.is_contiguous() and x.shape[0] == n and x.numel() == n * width:
+            return width
+    except (AttributeError, IndexError):
+        pass
+    types.check(x.dtype, name)
+    shape, st = x.shape, x.stride()
     size, at = 1, 1
     for i in range(len(shape) - 1, 0, -1):
         if st[i] != at and shape[i] != 1:
@@ -479,10 +495,16 @@ def _rows(x, types, n, width, name):
 
 
 def _flat(x, types, shape, name):
-    """A contiguous array of this shape: its address (None passes)."""
+    """A contiguous array of this shape: its address (None passes, as 0)."""
     if x is None:
-        return None
-    s = _array(x, types, name)
+        return 0
+    try:
+        if x.dtype in types.known and x.shape == shape and x.is_contiguous():
+            return x.data_ptr()
+    except AttributeError:
+        pass
+    types.check(x.dtype, name)
+    s = x.shape
     if tuple(s) != shape:
         raise _shape_error(f"{name} is {list(s)}, not {list(shape)}")
     st, at = x.stride(), 1
@@ -498,24 +520,19 @@ class _PagedKV(C.Structure):
         (n, C.c_int) for n in ("n_seqs", "ld_table", "n_pages", "page_size", "n_kv_heads", "head_dim", "kv_type")]
 
 
-class _AppendArgs(C.Structure):
-    _fields_ = [(n, C.c_void_p) for n in ("q", "k", "v", "q_out")] + [
-        (n, C.c_longlong) for n in ("ldq", "ldk", "ldv", "ldo")] + [
-        (n, C.c_void_p) for n in ("cos", "sin", "q_norm", "k_norm", "seqs", "pos")] + [
-        (n, C.c_int) for n in ("rows", "n_heads", "n_pos")] + [("eps", C.c_float)]
+class _Args:
+    """One of the C entries' argument structs, packed in their fields' order (a call's cost is the host's:
+    a packed struct takes half the time of a ctypes one). P pointer, q long long, i int, f float, N size_t."""
+
+    def __init__(self, fields):
+        self.names = tuple(f[1:] for f in fields.split())
+        self.pack = struct.Struct("@" + "".join(f[0] for f in fields.split())).pack
 
 
-class _AttendArgs(C.Structure):
-    _fields_ = [("q", C.c_void_p), ("out", C.c_void_p), ("ldq", C.c_longlong), ("ldo", C.c_longlong),
-                ("lens", C.c_void_p), ("n_seqs", C.c_int), ("n_heads", C.c_int), ("window", C.c_int),
-                ("scale", C.c_float), ("softcap", C.c_float), ("ws", C.c_void_p), ("ws_bytes", C.c_size_t)]
-
-
-class _LogitsArgs(C.Structure):
-    _fields_ = [("inp", C.c_void_p), ("out", C.c_void_p), ("ld_in", C.c_longlong), ("ld_out", C.c_longlong),
-                ("history", C.c_void_p), ("history_len", C.c_void_p), ("ld_history", C.c_longlong)] + [
-        (n, C.c_void_p) for n in ("repeat", "presence", "frequency", "bias_off", "bias_ids", "bias_vals", "mask")] + [
-        ("ld_mask", C.c_longlong)] + [(n, C.c_int) for n in ("rows", "vocab", "history_cap", "n_bias")]
+_APPEND = _Args("Pq Pk Pv Pq_out qldq qldk qldv qldo Pcos Psin Pq_norm Pk_norm Pseqs Ppos irows in_heads in_pos feps")
+_ATTEND = _Args("Pq Pout qldq qldo Plens in_seqs in_heads iwindow fscale fsoftcap Pws Nws_bytes")
+_LOGITS = _Args("Pin Pout qld_in qld_out Phistory Phistory_len qld_history Prepeat Ppresence Pfrequency Pbias_off "
+                "Pbias_ids Pbias_vals Pmask qld_mask irows ivocab ihistory_cap in_bias")
 
 
 def rope_tables(config, n_pos, local=False):
@@ -545,16 +562,18 @@ class PagedKV:
     is a CUDA stream's handle (None: the default stream); nothing is waited for."""
 
     def __init__(self, k, v, table, kv_type, kd=None, vd=None, n_heads=None):
-        types = {F32: _F, F16: ("float16",), Q8_0: ("int8",)}.get(kv_type)
+        types = {F32: _F, F16: _H, Q8_0: _B}.get(kv_type)
         if types is None:
             raise _shape_error("kv_type must be F32, F16 or Q8_0")
-        shape = tuple(_array(k, types, "k"))
+        types.check(k.dtype, "k")
+        shape = tuple(k.shape)
         if len(shape) != 4:
             raise _shape_error(f"k is {list(shape)}, not [n_pages, n_kv_heads, page_size, head_dim]")
         self.n_heads = int(n_heads or shape[1])
         if (kv_type == Q8_0) != (kd is not None and vd is not None) or (kd is None) != (vd is None):
             raise _shape_error("an int8 cache has the scales kd and vd, another has none")
-        ts = tuple(_array(table, _I, "table"))
+        _I.check(table.dtype, "table")
+        ts = tuple(table.shape)
         if len(ts) != 2:
             raise _shape_error(f"table is {list(ts)}, not [n_seqs, pages]")
         self.kv_type, self.n_seqs, self.head_dim = kv_type, ts[0], shape[3]
@@ -568,10 +587,12 @@ class PagedKV:
         self._ws = self.workspace()
 
     def workspace(self):
-        """Scratch for the attention calls of one stream."""
+        """Scratch for attention calls that do not overlap in time (ready when this returns)."""
         n = C.c_size_t()
         _check(lib().kc_paged_attend_ws(self._ref, self.n_heads, C.byref(n)), "attend workspace")
-        return DevBuf(n.value)
+        ws = DevBuf(n.value)
+        _check(lib().kc_paged_attend_ws_init(ws.ptr, ws.nbytes), "attend workspace")
+        return ws
 
     def append(self, qkv, pos, cos, sin, q_out, seqs=None, q_norm=None, k_norm=None, eps=1e-5, stream=None):
         """kc_paged_append_dev: rows of q|k|v ([rows, (n_heads + 2 n_kv_heads) head_dim], or the
@@ -586,11 +607,11 @@ class PagedKV:
             pq = qkv.data_ptr()
             pk, pv = pq + 4 * self._q, pq + 4 * (self._q + kw)
         n_pos = cos.shape[0]
-        a = _AppendArgs(pq, pk, pv, q_out.data_ptr(), ldq, ldk, ldv, _rows(q_out, _F, n, self._q, "q_out"),
-                        _flat(cos, _F, (n_pos, hd // 2), "cos"), _flat(sin, _F, (n_pos, hd // 2), "sin"),
-                        _flat(q_norm, _F, (hd,), "q_norm"), _flat(k_norm, _F, (hd,), "k_norm"),
-                        _flat(seqs, _I, (n,), "seqs"), _flat(pos, _I, (n,), "pos"), n, self.n_heads, n_pos, eps)
-        st = lib().kc_paged_append_dev(self._ref, C.byref(a), stream)
+        a = _APPEND.pack(pq, pk, pv, q_out.data_ptr(), ldq, ldk, ldv, _rows(q_out, _F, n, self._q, "q_out"),
+                         _flat(cos, _F, (n_pos, hd // 2), "cos"), _flat(sin, _F, (n_pos, hd // 2), "sin"),
+                         _flat(q_norm, _F, (hd,), "q_norm"), _flat(k_norm, _F, (hd,), "k_norm"),
+                         _flat(seqs, _I, (n,), "seqs"), _flat(pos, _I, (n,), "pos"), n, self.n_heads, n_pos, eps)
+        st = _lib.kc_paged_append_dev(self._ref, a, stream)
         if st:
             raise KraflaError(st, "append")
         return q_out
@@ -599,12 +620,11 @@ class PagedKV:
         """kc_paged_attend_dev: query rows [n, n_heads, head_dim] of the first n sequences
         against their cached positions (the last `window` of lens[i]; 0: all) into out."""
         n = q.shape[0]
-        ldq = _rows(q, _F, n, self._q, "q")
         w = ws or self._ws
-        a = _AttendArgs(q.data_ptr(), out.data_ptr(), ldq, _rows(out, _F, n, self._q, "out"),
-                        _flat(lens, _I, (n,), "lens"), n, self.n_heads, window,
-                        self.head_dim ** -0.5 if scale is None else scale, softcap, w.ptr, w.nbytes)
-        st = lib().kc_paged_attend_dev(self._ref, C.byref(a), stream)
+        a = _ATTEND.pack(q.data_ptr(), out.data_ptr(), _rows(q, _F, n, self._q, "q"), _rows(out, _F, n, self._q, "out"),
+                         _flat(lens, _I, (n,), "lens"), n, self.n_heads, window,
+                         self.head_dim ** -0.5 if scale is None else scale, softcap, w.ptr, w.nbytes)
+        st = _lib.kc_paged_attend_dev(self._ref, a, stream)
         if st:
             raise KraflaError(st, "attend")
         return out
@@ -616,31 +636,31 @@ def process_logits(out, logits, history=None, history_len=None, repeat=None, pre
     logits [rows, vocab] into out (which may be logits). history [rows, cap] int32 with
     history_len [rows]; repeat, presence, frequency [rows]; bias_off [rows + 1] into bias_ids
     and bias_vals; mask [rows, words] with bit v % 32 of word v / 32 set where v is allowed."""
-    shape = _array(logits, _F, "logits")
+    shape = logits.shape
     if len(shape) != 2:
         raise _shape_error(f"logits is {list(shape)}, not [rows, vocab]")
     n, v = shape
-    ld_h, cap, ld_m = 0, 0, 0
-    if history is None and not (repeat is presence is frequency is history_len is None):
-        raise _shape_error("penalties need the rows' history")
+    ld_h = cap = ld_m = n_bias = hist = bits = 0
     if history is not None:
         cap = history.shape[-1]
         ld_h = _rows(history, _I, n, cap, "history")
+        hist = history.data_ptr() if cap else 0
+    elif not (repeat is presence is frequency is history_len is None):
+        raise _shape_error("penalties need the rows' history")
     if mask is not None:
         words = mask.shape[-1]
         if words < (v + 31) // 32:
             raise _shape_error(f"mask has {words} words a row for {v} tokens")
         ld_m = _rows(mask, _W, n, words, "mask")
-    n_bias = 0
+        bits = mask.data_ptr()
     if bias_ids is not None:
         n_bias = bias_ids.shape[0]
-    a = _LogitsArgs(logits.data_ptr(), out.data_ptr(), _rows(logits, _F, n, v, "logits"), _rows(out, _F, n, v, "out"),
-                    history.data_ptr() if cap else None, _flat(history_len, _I, (n,), "history_len"), ld_h,
-                    _flat(repeat, _F, (n,), "repeat"), _flat(presence, _F, (n,), "presence"),
-                    _flat(frequency, _F, (n,), "frequency"), _flat(bias_off, _I, (n + 1,), "bias_off"),
-                    _flat(bias_ids, _I, (n_bias,), "bias_ids"), _flat(bias_vals, _F, (n_bias,), "bias_vals"),
-                    mask.data_ptr() if mask is not None else None, ld_m, n, v, cap, n_bias)
-    st = lib().kc_logits_process_dev(C.byref(a), stream)
+    a = _LOGITS.pack(logits.data_ptr(), out.data_ptr(), _rows(logits, _F, n, v, "logits"), _rows(out, _F, n, v, "out"),
+                     hist, _flat(history_len, _I, (n,), "history_len"), ld_h, _flat(repeat, _F, (n,), "repeat"),
+                     _flat(presence, _F, (n,), "presence"), _flat(frequency, _F, (n,), "frequency"),
+                     _flat(bias_off, _I, (n + 1,), "bias_off"), _flat(bias_ids, _I, (n_bias,), "bias_ids"),
+                     _flat(bias_vals, _F, (n_bias,), "bias_vals"), bits, ld_m, n, v, cap, n_bias)
+    st = lib().kc_logits_process_dev(a, stream)
     if st:
         raise KraflaError(st, "process logits")
     return out

@@ -25,7 +25,7 @@ def cache(**kw):
 
 
 def refused(fn, *structs):
-    st = fn(*[C.byref(s) for s in structs], None)
+    st = fn(*[s if isinstance(s, bytes) else C.byref(s) for s in structs], None)
     return st == kb.E_SHAPE and kb.what_detail()
 
 
@@ -35,7 +35,7 @@ def refused(fn, *structs):
     (dict(n_pages=1 << 26, page_size=64), "2^32"), (dict(ld_table=1 << 28), "2^31"), (dict(n_seqs=0), "n_seqs")])
 def test_cache_sizes_are_refused(kw, word):
     L = kb.lib()
-    for fn, a in ((L.kc_paged_append_dev, kb._AppendArgs()), (L.kc_paged_attend_dev, kb._AttendArgs())):
+    for fn, a in ((L.kc_paged_append_dev, bytes(256)), (L.kc_paged_attend_dev, bytes(256))):
         assert word in refused(fn, cache(**kw), a)
     n = C.c_size_t()
     assert L.kc_paged_attend_ws(C.byref(cache(**kw)), 4, C.byref(n)) == kb.E_SHAPE
@@ -44,7 +44,7 @@ def test_cache_sizes_are_refused(kw, word):
 def attend_args(**kw):
     d = dict(q=P, out=P, ldq=256, ldo=256, lens=P, n_seqs=4, n_heads=4, window=0, scale=0.1, softcap=0.0, ws=P, ws_bytes=0)
     d.update(kw)
-    return kb._AttendArgs(*[d[n] for n, _ in kb._AttendArgs._fields_])
+    return kb._ATTEND.pack(*[d[n] for n in kb._ATTEND.names])
 
 
 @pytest.mark.parametrize("kw,word", [
@@ -56,27 +56,25 @@ def test_attend_is_refused(kw, word):
 
 
 def append_args(**kw):
-    d = dict(q=P, k=P, v=P, q_out=P, ldq=512, ldk=512, ldv=512, ldo=256, cos=P, sin=P, q_norm=None, k_norm=None, seqs=P,
+    d = dict(q=P, k=P, v=P, q_out=P, ldq=512, ldk=512, ldv=512, ldo=256, cos=P, sin=P, q_norm=0, k_norm=0, seqs=P,
              pos=P, rows=9, n_heads=4, n_pos=100, eps=1e-5)
     d.update(kw)
-    return kb._AppendArgs(*[d[n] for n, _ in kb._AppendArgs._fields_])
+    return kb._APPEND.pack(*[d[n] for n in kb._APPEND.names])
 
 
 @pytest.mark.parametrize("kw,word", [
     (dict(rows=-1), "rows"), (dict(n_heads=0), "n_heads"), (dict(n_pos=0), "n_pos"), (dict(ldk=130), "multiples of 4"),
     (dict(ldv=64), "shorter"), (dict(q_norm=P), "together"), (dict(eps=float("nan")), "eps"), (dict(eps=-1.0), "eps"),
-    (dict(seqs=None), "more rows"), (dict(rows=1 << 30), "too many")])
+    (dict(seqs=0), "more rows"), (dict(rows=1 << 30), "too many")])
 def test_append_is_refused(kw, word):
     assert word in refused(kb.lib().kc_paged_append_dev, cache(), append_args(**kw))
 
 
 def logits_args(**kw):
-    a = kb._LogitsArgs()
-    d = dict(inp=P, out=P, ld_in=100, ld_out=100, rows=3, vocab=100)
+    d = dict({n: 0 for n in kb._LOGITS.names}, out=P, ld_in=100, ld_out=100, rows=3, vocab=100)
+    d["in"] = P
     d.update(kw)
-    for n, x in d.items():
-        setattr(a, n, x)
-    return a
+    return kb._LOGITS.pack(*[d[n] for n in kb._LOGITS.names])
 
 
 @pytest.mark.parametrize("kw,word", [

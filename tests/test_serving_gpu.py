@@ -374,9 +374,9 @@ def test_logits_bad_offsets_and_lengths():
 def test_refused_pointers():
     """Host memory and wrong types never reach a kernel."""
     a = np.zeros((2, 64), np.float32)
-    x = kb._LogitsArgs(a.ctypes.data, a.ctypes.data, 64, 64)
-    x.rows, x.vocab = 2, 64
-    assert kb.lib().kc_logits_process_dev(kb.C.byref(x), None) == kb.E_SHAPE
+    x = dict({n: 0 for n in kb._LOGITS.names}, out=a.ctypes.data, ld_in=64, ld_out=64, rows=2, vocab=64)
+    x["in"] = a.ctypes.data
+    assert kb.lib().kc_logits_process_dev(kb._LOGITS.pack(*x.values()), None) == kb.E_SHAPE
     assert "not device memory" in kb.what_detail()
     with pytest.raises(kb.KraflaError, match="float32"):
         kb.process_logits(kb.DevArray((2, 64), np.float32), kb.DevArray((2, 64), np.float16))
