@@ -8,7 +8,7 @@
  *   z = -inf where v's bit of the row's mask is 0
  * every operation IEEE round to nearest in 32 bits, in this order.
  *
- * Bound by memory: 8 bytes a logit, an eighth for the mask. A CTA takes 4096
+ * Bound by memory: 8 bytes a logit, an eighth for the mask. A CTA takes 8192
  * logits of one row; it requests them first, then counts the row's history
  * tokens that fall into its stretch in shared memory while they arrive. */
 #pragma once
@@ -18,9 +18,9 @@
 
 namespace kc {
 
-constexpr int LG_THREADS = 256;
+constexpr int LG_THREADS = 512;
 constexpr int LG_VEC = 4;                              /* float4 per thread */
-constexpr int LG_HIST = 8;                             /* history tokens a thread requests at once */
+constexpr int LG_HIST = 4;                             /* history tokens a thread requests at once */
 constexpr int LG_CHUNK = LG_THREADS * LG_VEC * 4;      /* logits per CTA */
 
 struct LogitsArgs {
@@ -40,10 +40,15 @@ struct LogitsArgs {
     unsigned *err;
 };
 
+/* Shared memory: for each logit of the chunk the times its token is in the
+ * history, and the last list entry that names it (-1: none). */
+template <bool HIST, bool BIAS>
+constexpr int logits_smem() { return ((HIST ? 4 : 0) + (BIAS ? 4 : 0)) * LG_CHUNK; }
+
 template <bool HIST, bool BIAS>
 __global__ void __launch_bounds__(LG_THREADS) logits_kernel(const LogitsArgs a) {
-    __shared__ __align__(16) int s_count[HIST ? LG_CHUNK : 1];
-    __shared__ __align__(16) int s_bias[BIAS ? LG_CHUNK : 1];        /* the last list entry of each token, -1 none */
+    extern __shared__ __align__(16) int lg_smem[];
+    int *s_count = lg_smem, *s_bias = lg_smem + (HIST ? LG_CHUNK : 0);
     const int tid = threadIdx.x, V = a.vocab;
     const long long row = blockIdx.x;
     const float *in = a.in + row * a.ld_in;
@@ -52,7 +57,27 @@ __global__ void __launch_bounds__(LG_THREADS) logits_kernel(const LogitsArgs a) 
     const int sh = (int)(((uintptr_t)in >> 2) & 3);
     const bool same = (int)(((uintptr_t)out >> 2) & 3) == sh;
     const int e0 = (int)blockIdx.y * LG_CHUNK - sh;    /* the chunk's first element (below 0: none) */
+    /* everything that comes from memory is requested before anything waits */
+    int t0[HIST ? LG_HIST : 1], n = 0, b0 = 0, b1 = 0, i0 = -1;
+    const int *h = a.hist + row * a.ld_hist;
+    float rep = 1.0f, pres = 0.0f, freq = 0.0f;
+    if constexpr (BIAS) {
+        b0 = __ldg(a.bias_off + row);
+        b1 = __ldg(a.bias_off + row + 1);
+    }
+    if constexpr (HIST) {
+        n = a.hist_len ? __ldg(a.hist_len + row) : a.hist_cap;
+#pragma unroll
+        for (int k = 0; k < LG_HIST; k++) {
+            const int i = tid + k * LG_THREADS;
+            t0[k] = i < a.hist_cap ? __ldg(h + i) : -1;
+        }
+        if (a.repeat) rep = __ldg(a.repeat + row);
+        if (a.presence) pres = __ldg(a.presence + row);
+        if (a.frequency) freq = __ldg(a.frequency + row);
+    }
     float z[LG_VEC][4];
+    uint32_t ma[LG_VEC], mb[LG_VEC];                   /* the mask words that hold bits e .. e + 3 of each vector */
 #pragma unroll
     for (int k = 0; k < LG_VEC; k++) {
         const int e = e0 + 4 * (tid + k * LG_THREADS);
@@ -63,61 +88,46 @@ __global__ void __launch_bounds__(LG_THREADS) logits_kernel(const LogitsArgs a) 
 #pragma unroll
             for (int i = 0; i < 4; i++) z[k][i] = e + i >= 0 && e + i < V ? in[e + i] : 0.0f;
         }
-    }
-    /* the words that hold bits e .. e + 3 of each vector */
-    uint32_t ma[LG_VEC], mb[LG_VEC];
-#pragma unroll
-    for (int k = 0; k < LG_VEC; k++) {
         ma[k] = mb[k] = 0xffffffffu;
-        const int e = e0 + 4 * (tid + k * LG_THREADS), w = e >> 5;
         if (a.mask && e + 3 >= 0 && e < V) {
             const uint32_t *mask = a.mask + row * a.ld_mask;
-            if (w >= 0) ma[k] = mb[k] = __ldg(mask + w);
-            if (((e + 3) >> 5) != w && ((e + 3) >> 5) <= (V - 1) >> 5) mb[k] = __ldg(mask + ((e + 3) >> 5));
+            const int wa = e >> 5, wb = (e + 3) >> 5;  /* (e below 0: word -1, whose bits no logit has) */
+            if (wa >= 0) ma[k] = mb[k] = __ldg(mask + wa);
+            if (wb != wa && wb <= (V - 1) >> 5) mb[k] = __ldg(mask + wb);
         }
     }
-    float rep = 1.0f, pres = 0.0f, freq = 0.0f;
     if constexpr (HIST || BIAS) {
-        const int *h = a.hist + row * a.ld_hist;
-        int t0[HIST ? LG_HIST : 1], n = 0;
-        if constexpr (HIST) {
-#pragma unroll
-            for (int k = 0; k < LG_HIST; k++) {
-                const int i = tid + k * LG_THREADS;
-                t0[k] = i < a.hist_cap ? __ldg(h + i) : -1;
+        if constexpr (BIAS) {
+            if (b0 < 0 || b1 < b0 || b1 > a.n_bias) {
+                if (tid == 0 && blockIdx.y == 0) atomicOr(a.err, 2u);
+                b0 = b1 = 0;
             }
-            n = a.hist_len ? a.hist_len[row] : a.hist_cap;
-            rep = a.repeat ? a.repeat[row] : 1.0f;
-            if (a.presence) pres = a.presence[row];
-            if (a.frequency) freq = a.frequency[row];
+            if (b0 + tid < b1) i0 = __ldg(a.bias_ids + b0 + tid);
         }
         for (int i = tid; i < LG_CHUNK / 4; i += LG_THREADS) {
             if constexpr (HIST) ((int4 *)s_count)[i] = make_int4(0, 0, 0, 0);
             if constexpr (BIAS) ((int4 *)s_bias)[i] = make_int4(-1, -1, -1, -1);
         }
         __syncthreads();
+        auto here = [&](int t) { return (unsigned)t < (unsigned)V && (unsigned)(t - e0) < (unsigned)LG_CHUNK; };
         if constexpr (HIST) {
             if (n > a.hist_cap) {
                 if (tid == 0 && blockIdx.y == 0) atomicOr(a.err, 1u);
                 n = a.hist_cap;
             }
-            auto seen = [&](int t) {
-                if (t >= 0 && t < V && t >= e0 && t - e0 < LG_CHUNK) atomicAdd(&s_count[t - e0], 1);
-            };
 #pragma unroll
             for (int k = 0; k < LG_HIST; k++)
-                if (tid + k * LG_THREADS < n) seen(t0[k]);
-            for (int i = tid + LG_HIST * LG_THREADS; i < n; i += LG_THREADS) seen(__ldg(h + i));
+                if (tid + k * LG_THREADS < n && here(t0[k])) atomicAdd(&s_count[t0[k] - e0], 1);
+            for (int i = tid + LG_HIST * LG_THREADS; i < n; i += LG_THREADS) {
+                const int t = __ldg(h + i);
+                if (here(t)) atomicAdd(&s_count[t - e0], 1);
+            }
         }
         if constexpr (BIAS) {
-            int b0 = a.bias_off[row], b1 = a.bias_off[row + 1];
-            if (b0 < 0 || b1 < b0 || b1 > a.n_bias) {
-                if (tid == 0 && blockIdx.y == 0) atomicOr(a.err, 2u);
-                b0 = b1 = 0;
-            }
-            for (int i = b0 + tid; i < b1; i += LG_THREADS) {
-                const int t = a.bias_ids[i];
-                if (t >= 0 && t < V && t >= e0 && t - e0 < LG_CHUNK) atomicMax(&s_bias[t - e0], i);
+            if (i0 >= 0 && here(i0)) atomicMax(&s_bias[i0 - e0], b0 + tid);
+            for (int i = b0 + tid + LG_THREADS; i < b1; i += LG_THREADS) {
+                const int t = __ldg(a.bias_ids + i);
+                if (here(t)) atomicMax(&s_bias[t - e0], i);
             }
         }
         __syncthreads();
@@ -126,29 +136,33 @@ __global__ void __launch_bounds__(LG_THREADS) logits_kernel(const LogitsArgs a) 
     for (int k = 0; k < LG_VEC; k++) {
         const int o = 4 * (tid + k * LG_THREADS), e = e0 + o;
         if (e + 3 < 0 || e >= V) continue;
-        /* the vector's mask bits, from its two words (elements before the row have e < 0: any bit will do) */
-        const unsigned bits = __funnelshift_r(ma[k], mb[k], (unsigned)e & 31u);
-        int4 cn = make_int4(0, 0, 0, 0), bn = make_int4(-1, -1, -1, -1);
-        if constexpr (HIST) cn = *(const int4 *)(s_count + o);
-        if constexpr (BIAS) bn = *(const int4 *)(s_bias + o);
-        const int cc[4] = { cn.x, cn.y, cn.z, cn.w }, bb[4] = { bn.x, bn.y, bn.z, bn.w };
+        /* few logits have a history or a bias: four at a time are looked at */
+        if constexpr (HIST) {
+            const int4 t = *(const int4 *)(s_count + o);
+            if (t.x | t.y | t.z | t.w) {
+                const int c[4] = { t.x, t.y, t.z, t.w };
 #pragma unroll
-        for (int i = 0; i < 4; i++) {
-            float x = z[k][i];
-            if constexpr (HIST) {
-                const int c = cc[i];
-                if (c > 0) {
-                    x = x > 0.0f ? __fdiv_rn(x, rep) : __fmul_rn(x, rep);
-                    x = __fsub_rn(x, __fmul_rn(freq, (float)c));
-                    x = __fsub_rn(x, pres);
-                }
+                for (int i = 0; i < 4; i++)
+                    if (c[i] > 0) {
+                        float x = z[k][i];
+                        x = x > 0.0f ? __fdiv_rn(x, rep) : __fmul_rn(x, rep);
+                        x = __fsub_rn(x, __fmul_rn(freq, (float)c[i]));
+                        z[k][i] = __fsub_rn(x, pres);
+                    }
             }
-            if constexpr (BIAS) {
-                const int b = bb[i];
-                if (b >= 0) x = __fadd_rn(x, a.bias_vals[b]);
-            }
-            z[k][i] = (bits >> i) & 1u ? x : -INFINITY;
         }
+        if constexpr (BIAS) {
+            const int4 t = *(const int4 *)(s_bias + o);
+            if ((t.x & t.y & t.z & t.w) >= 0) {
+                const int b[4] = { t.x, t.y, t.z, t.w };
+#pragma unroll
+                for (int i = 0; i < 4; i++)
+                    if (b[i] >= 0) z[k][i] = __fadd_rn(z[k][i], a.bias_vals[b[i]]);
+            }
+        }
+        const unsigned bits = __funnelshift_r(ma[k], mb[k], (unsigned)e & 31u);
+#pragma unroll
+        for (int i = 0; i < 4; i++) z[k][i] = (bits >> i) & 1u ? z[k][i] : -INFINITY;
         if (same && e >= 0 && e <= V - 4) {
             __stcs((float4 *)(out + e), make_float4(z[k][0], z[k][1], z[k][2], z[k][3]));
         } else {

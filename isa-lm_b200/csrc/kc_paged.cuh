@@ -9,7 +9,9 @@
  * where they are read, and a bad one is skipped and flagged, never followed. */
 #pragma once
 #include <cuda_fp16.h>
+#include <climits>
 #include <cstdint>
+#include <type_traits>
 
 #include "kc_kernels.cuh"
 #include "krafla_cuda.h"
@@ -24,6 +26,10 @@ struct PagedKV {
     float *kd, *vd;
     const int *table;
     int n_seqs, ld_table, n_pages, page, n_kv, hd;
+    unsigned page_mul;
+    int page_shift;
+    /* p / page for 0 <= p < 2^31 */
+    __device__ __forceinline__ int page_of(int p) const { return page_mul ? (int)(__umulhi((unsigned)p, page_mul) >> page_shift) : p; }
 };
 
 /* ------------------------------------------------------------ append */
@@ -126,7 +132,7 @@ __global__ void __launch_bounds__(AP_THREADS) append_kernel(const AppendArgs a) 
             if (h < nh && d < hd) t = __ldcs((const float4 *)(src + (size_t)h * hd + d));
             x[k][j][0] = t.x; x[k][j][1] = t.y; x[k][j][2] = t.z; x[k][j][3] = t.w;
         }
-    const int pi = p >= 0 ? p / a.kv.page : 0, slot = p - pi * a.kv.page;
+    const int pi = p >= 0 ? a.kv.page_of(p) : 0, slot = p - pi * a.kv.page;
     bool ok = seq < a.kv.n_seqs && p >= 0 && p < a.n_pos && pi < a.kv.ld_table;
     int page = 0;
     if (ok) {
@@ -243,6 +249,7 @@ __global__ void __launch_bounds__(AP_THREADS) append_kernel(const AppendArgs a) 
  * per tile and are carried in f32. */
 constexpr int AT_WARPS = 4;
 constexpr int AT_THREADS = AT_WARPS * 32;
+constexpr int AT_SHORT = 3;               /* quanta of a unit that is not worth sharing out */
 constexpr int AT_COMB = 4;                /* heads that the warps of a CTA put together at a time */
 
 template <int KV>
@@ -259,9 +266,10 @@ struct AttendArgs {
     const int *lens;
     int n_seqs, n_heads, group, chunks;   /* chunks: head chunks per KV head */
     int window;
-    float scale, softcap;
+    float scale, softcap, inv_softcap;
     int unit_cost;                        /* a unit's own time, in quanta */
     int min_share;                        /* least such time of a CTA's share */
+    int near;                             /* a tile's pages lie within 32 entries of its table row */
     unsigned *count;                      /* [CTAs] pieces that have come, of the unit that ends there; 0 between calls */
     float *part;                          /* [2 * CTAs] pieces */
     unsigned *err;
@@ -271,6 +279,9 @@ struct AttendArgs {
 template <int HD, int MT>
 constexpr int part_floats() { return 8 * MT * (HD + 2); }
 
+__device__ __forceinline__ void cp_async16s(uint32_t dst, const void *src) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src));
+}
 __device__ __forceinline__ void cp_async16z(uint32_t dst, const void *src, bool live) {
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(live ? 16 : 0));
 }
@@ -298,6 +309,17 @@ __device__ __forceinline__ void mma_f16(float (&c)[4], const unsigned (&a)[4], u
                  : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
                  : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
+/* the product alone, without a sum to add it to */
+__device__ __forceinline__ void mma_f16_first(float (&c)[4], const unsigned (&a)[4], unsigned b0, unsigned b1) {
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%10, %10, %10, %10};"
+                 : "=f"(c[0]), "=f"(c[1]), "=f"(c[2]), "=f"(c[3])
+                 : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(0.0f));
+}
+__device__ __forceinline__ void mma_tf32_first(float (&c)[4], const unsigned (&a)[4], unsigned b0, unsigned b1) {
+    asm volatile("mma.sync.aligned.m16n8k8.row.col.f32.tf32.tf32.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%10, %10, %10, %10};"
+                 : "=f"(c[0]), "=f"(c[1]), "=f"(c[2]), "=f"(c[3])
+                 : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(0.0f));
+}
 __device__ __forceinline__ void mma_tf32(float (&c)[4], const unsigned (&a)[4], unsigned b0, unsigned b1) {
     asm volatile("mma.sync.aligned.m16n8k8.row.col.f32.tf32.tf32.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
                  : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
@@ -317,14 +339,41 @@ __device__ __forceinline__ void split_f16(float a, float b, unsigned &hi, unsign
     hi = h2u(h);
     lo = h2u(__floats2half2_rn(a - f.x, b - f.y));
 }
-__device__ __forceinline__ unsigned to_tf32(float a) {
-    unsigned r;
-    asm("cvt.rna.tf32.f32 %0, %1;" : "=r"(r) : "f"(a));
+/* a float as two tf32: the nearest above or below, and what it leaves (|.| <= 2^-10 of it, of which
+ * 11 bits are kept); integer operations, since the conversion instruction runs at a fraction of their rate */
+__device__ __forceinline__ void split_tf32(float a, unsigned &hi, unsigned &lo) {
+    hi = __float_as_uint(a) & 0xffffe000u;
+    lo = (__float_as_uint(a - __uint_as_float(hi)) + 0x1000u) & 0xffffe000u;
+}
+/* 2^x, 0 below 2^-126 (relative error 2^-22) */
+__device__ __forceinline__ float ex2(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+/* two f32 at once */
+__device__ __forceinline__ float2 add2(float2 a, float2 b) {
+    float2 r;
+    asm("{\n .reg .b64 x, y, z;\n mov.b64 x, {%2, %3};\n mov.b64 y, {%4, %5};\n add.rn.f32x2 z, x, y;\n mov.b64 {%0, %1}, z;\n}"
+        : "=f"(r.x), "=f"(r.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
     return r;
 }
-__device__ __forceinline__ void split_tf32(float a, unsigned &hi, unsigned &lo) {
-    hi = to_tf32(a);
-    lo = to_tf32(a - __uint_as_float(hi));
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+    float2 r;
+    asm("{\n .reg .b64 x, y, z, w;\n mov.b64 x, {%2, %3};\n mov.b64 y, {%4, %5};\n mov.b64 z, {%6, %7};\n"
+        " fma.rn.f32x2 w, x, y, z;\n mov.b64 {%0, %1}, w;\n}"
+        : "=f"(r.x), "=f"(r.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
+    return r;
+}
+__device__ __forceinline__ float2 mul2(float2 a, float b) {
+    float2 r;
+    asm("{\n .reg .b64 x, y, z;\n mov.b64 x, {%2, %3};\n mov.b64 y, {%4, %4};\n mul.rn.f32x2 z, x, y;\n mov.b64 {%0, %1}, z;\n}"
+        : "=f"(r.x), "=f"(r.y) : "f"(a.x), "f"(a.y), "f"(b));
+    return r;
+}
+/* o = o * corr + (rows 0-7 and 8-15 of a product) */
+__device__ __forceinline__ void carry(float2 &o, float2 corr, const float (&d)[4]) {
+    o = fma2(o, corr, add2(make_float2(d[0], d[1]), make_float2(d[2], d[3])));
 }
 
 /* Positions [first, len) of sequence b, quanta of QP positions, clamped to what the table can hold. */
@@ -348,62 +397,89 @@ constexpr int attend_smem() {
     return AT_WARPS * (S * (slot_bytes<KV, HD, TM>() + 16) + AT_COMB * HD * 4 + 2 * 8 * MT * 4);
 }
 
-/* The share of CTA i of n of `total`: [i total / n, (i + 1) total / n); the owner of x. */
-__device__ __forceinline__ long long share_lo(long long i, long long n, long long total) { return i * total / n; }
-__device__ __forceinline__ int share_owner(long long x, long long n, long long total) {
-    return (int)(((x + 1) * n - 1) / total);
-}
-
 /* sum / weights; nothing attended gives zeros */
 __device__ __forceinline__ float4 over(float4 o, float l) {
     const float inv = l == 0.0f ? 0.0f : __fdiv_rn(1.0f, l);
     return make_float4(o.x * inv, o.y * inv, o.z * inv, o.w * inv);
 }
 
-/* The pieces of CTAs c0..c1 of one unit, in that order, into the output. */
+/* The pieces of CTAs c0..c1 of one unit into the output: every four outputs by
+ * as many threads as there are to spare, each of which takes a run of the
+ * pieces, 16 requested at once; the runs meet in shared memory (`red`, 8 floats
+ * a thread) in their order. */
 template <int HD, int MT>
-__device__ __noinline__ void join_pieces(const AttendArgs &a, int b, int u, int c0, int c1) {
-    constexpr int HC = 8 * MT, PF = part_floats<HD, MT>(), UN = 8;
-    const int g = u / a.chunks, h0 = (u - g * a.chunks) * HC, nh = min(HC, a.group - h0);
-    auto piece = [&](int c) { return a.part + ((size_t)2 * c + (c == c0 ? 1 : 0)) * PF; };
-    for (int idx = threadIdx.x; idx < nh * (HD / 4); idx += AT_THREADS) {
+__device__ __noinline__ void join_pieces(const AttendArgs &a, int b, int u, int c0, int c1, float *red) {
+    constexpr int HC = 8 * MT, PF = part_floats<HD, MT>(), UN = 16;
+    const int g = u / a.chunks, h0 = (u - g * a.chunks) * HC, nh = min(HC, a.group - h0), outs = nh * (HD / 4);
+    int runs = 1;
+    while (2 * runs * outs <= AT_THREADS) runs *= 2;
+    const int per = (c1 - c0 + runs) / runs;
+    for (int i0 = 0; i0 < outs; i0 += AT_THREADS / runs) {
+        const int idx = i0 + (int)threadIdx.x / runs, run = threadIdx.x % runs;
         const int h = idx / (HD / 4), e = 4 * (idx - h * (HD / 4));
         float M = -INFINITY, L = 0.0f;
         float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-        for (int k0 = c0; k0 <= c1; k0 += UN) {
-            float m[UN], l[UN];
-            float4 t[UN];
+        if (idx < outs) {
+            const int k1 = min(c0 + (run + 1) * per, c1 + 1);
+            for (int k0 = c0 + run * per; k0 < k1; k0 += UN) {
+                float m[UN], l[UN];
+                float4 t[UN];
 #pragma unroll
-            for (int i = 0; i < UN; i++) {
-                m[i] = -INFINITY;
-                l[i] = 0.0f;
-                t[i] = o;
-                if (k0 + i <= c1) {
-                    const float *p = piece(k0 + i);
-                    m[i] = __ldcg(p + HC * HD + h);
-                    l[i] = __ldcg(p + HC * HD + HC + h);
-                    t[i] = __ldcg((const float4 *)(p + h * HD + e));
+                for (int i = 0; i < UN; i++) {
+                    m[i] = -INFINITY;
+                    l[i] = 0.0f;
+                    t[i] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+                    if (k0 + i < k1) {
+                        const float *p = a.part + ((size_t)2 * (k0 + i) + (k0 + i == c0 ? 1 : 0)) * PF;
+                        m[i] = __ldcg(p + HC * HD + h);
+                        l[i] = __ldcg(p + HC * HD + HC + h);
+                        t[i] = __ldcg((const float4 *)(p + h * HD + e));
+                    }
                 }
-            }
-            float mn = M;
+                float mn = M;
 #pragma unroll
-            for (int i = 0; i < UN; i++) mn = fmaxf(mn, m[i]);
-            const float base = mn == -INFINITY ? 0.0f : mn, f0 = exp2f(M - base);
-            M = mn;
-            L *= f0;
-            o = make_float4(o.x * f0, o.y * f0, o.z * f0, o.w * f0);
+                for (int i = 0; i < UN; i++) mn = fmaxf(mn, m[i]);
+                const float base = mn == -INFINITY ? 0.0f : mn, f0 = ex2(M - base);
+                M = mn;
+                L *= f0;
+                o = make_float4(o.x * f0, o.y * f0, o.z * f0, o.w * f0);
 #pragma unroll
-            for (int i = 0; i < UN; i++)
-                if (k0 + i <= c1) {
-                    const float f = exp2f(m[i] - base);
+                for (int i = 0; i < UN; i++) {
+                    const float f = ex2(m[i] - base);
                     L += f * l[i];
                     o.x += f * t[i].x;
                     o.y += f * t[i].y;
                     o.z += f * t[i].z;
                     o.w += f * t[i].w;
                 }
+            }
         }
-        if (e < a.kv.hd) *(float4 *)(a.out + b * a.ldo + (size_t)(g * a.group + h0 + h) * a.kv.hd + e) = over(o, L);
+        if (runs > 1) {
+            __syncthreads();
+            float *w = red + 8 * threadIdx.x;
+            *(float4 *)w = o;
+            w[4] = M;
+            w[5] = L;
+            __syncthreads();
+            if (run == 0) {
+                float mn = M;
+                for (int i = 1; i < runs; i++) mn = fmaxf(mn, w[8 * i + 4]);
+                const float base = mn == -INFINITY ? 0.0f : mn, f0 = ex2(M - base);
+                L *= f0;
+                o = make_float4(o.x * f0, o.y * f0, o.z * f0, o.w * f0);
+                for (int i = 1; i < runs; i++) {
+                    const float f = ex2(w[8 * i + 4] - base);
+                    const float4 t = *(const float4 *)(w + 8 * i);
+                    L += f * w[8 * i + 5];
+                    o.x += f * t.x;
+                    o.y += f * t.y;
+                    o.z += f * t.z;
+                    o.w += f * t.w;
+                }
+            }
+        }
+        if (idx < outs && run == 0 && e < a.kv.hd)
+            *(float4 *)(a.out + b * a.ldo + (size_t)(g * a.group + h0 + h) * a.kv.hd + e) = over(o, L);
     }
 }
 
@@ -427,25 +503,28 @@ __global__ void __launch_bounds__(AT_THREADS, OCC) paged_attend_kernel(const __g
     const int U = a.kv.n_kv * a.chunks;                /* units per sequence */
     const int W = a.unit_cost;
 
-    /* ---- this CTA's share ---- */
+    /* ---- this CTA's share: [i chunk, (i + 1) chunk) of the units' times, laid end to end ---- */
     __shared__ long long s_sum[AT_WARPS];
-    __shared__ long long s_lo, s_hi, s_total;
-    __shared__ int s_b, s_ncta, s_last;
-    __shared__ long long s_base;                       /* the time of the sequences before s_b */
+    __shared__ long long s_at;
+    __shared__ int s_b, s_len, s_first, s_last;
+    long long lo, hi, chunk;
     {
         const int per = (a.n_seqs + AT_THREADS - 1) / AT_THREADS;
         const int b0 = min(tid * per, a.n_seqs), b1 = min(b0 + per, a.n_seqs);
+        int len = 0, first = 0;                        /* (of the only sequence of a thread, if it has one) */
         auto unit_time = [&](int b, bool &bad) {
-            int f;
-            const int n = seq_span(a, b, f, bad);
-            return n > 0 ? (n - f + QP - 1) / QP + W : 0;
+            len = seq_span(a, b, first, bad);
+            return len > 0 ? (len - first + QP - 1) / QP + W : 0;
         };
         long long sum = 0;
-        bool any_bad = false;
+        bool any_bad = false, none = false, far = (long long)a.n_seqs * U > gridDim.x;
         for (int b = b0; b < b1; b++) {
             bool bad;
-            sum += unit_time(b, bad);
+            const int t = unit_time(b, bad);
+            sum += t;
+            far |= t > AT_SHORT + W;
             any_bad |= bad;
+            none |= t == 0;
         }
         if (any_bad && blockIdx.x == 0) atomicOr(a.err, (unsigned)SE_LEN);
         long long pre = sum;
@@ -455,82 +534,112 @@ __global__ void __launch_bounds__(AT_THREADS, OCC) paged_attend_kernel(const __g
             if (lane >= o) pre += t;
         }
         if (lane == 31) s_sum[warp] = pre;
-        __syncthreads();
-        long long off = 0, all = 0;
+        none = __syncthreads_or(none);
+        far = __syncthreads_or(far);
+        long long all = 0;
+        pre -= sum;
 #pragma unroll
         for (int w = 0; w < AT_WARPS; w++) {
-            if (w < warp) off += s_sum[w];
+            if (w < warp) pre += s_sum[w];             /* a unit's worth of the time before b0 */
             all += s_sum[w];
         }
-        pre += off - sum;                              /* a unit's worth of the time before b0 */
         const long long total = all * U;
-        const long long ncta = max(1ll, min((long long)gridDim.x, total / a.min_share));
-        const bool on = blockIdx.x < ncta;
-        const long long lo = on ? share_lo(blockIdx.x, ncta, total) : total;
-        const long long hi = on ? share_lo(blockIdx.x + 1, ncta, total) : total;
+        /* total / CTAs, rounded up; a quotient below 2^42 is at least 2^-11 from the next integer or one itself */
+        if (!far) {
+            /* short sequences, a CTA for each unit: joining would take longer than it saved */
+            const int b = blockIdx.x / U;
+            if (b0 <= b && b < b1) {
+                bool bad;
+                if (per > 1) unit_time(b, bad);
+                s_b = b;
+                s_len = len;
+                s_first = first;
+                s_at = 0;
+            }
+            chunk = 1ll << 40;
+            lo = hi = 0;
+        } else {
+        chunk = (long long)((double)total / (double)gridDim.x);
+        chunk = max(chunk + (chunk * gridDim.x < total), (long long)a.min_share);
+        lo = min(blockIdx.x * chunk, total);
+        hi = min(lo + chunk, total);
         if (lo < hi && lo >= pre * U && lo < (pre + sum) * U) {
             long long at = pre;
             int b = b0;
-            for (; b < b1; b++) {
-                bool bad;
-                const int t = unit_time(b, bad);
-                if (lo < (at + t) * U) break;
-                at += t;
-            }
+            if (per > 1)
+                for (; b < b1; b++) {
+                    bool bad;
+                    const int t = unit_time(b, bad);
+                    if (lo < (at + t) * U) break;
+                    at += t;
+                }
             s_b = b;
-            s_base = at * U;
+            s_len = len;
+            s_first = first;
+            s_at = at * U;
         }
-        if (tid == 0) {
-            s_lo = lo;
-            s_hi = hi;
-            s_ncta = (int)ncta;
-            s_total = total;
         }
         __syncthreads();
+        /* sequences without positions: zeros */
+        if (none)
+            for (int b = blockIdx.x; b < a.n_seqs; b += gridDim.x) {
+                int f;
+                bool bad;
+                if (seq_span(a, b, f, bad) == 0)
+                    for (int i = tid; i < a.n_heads * a.kv.hd; i += AT_THREADS) a.out[b * a.ldo + i] = 0.0f;
+            }
+        if (!far) {
+            if (blockIdx.x >= a.n_seqs * U || s_len == 0) return;
+            const int t = (s_len - s_first + QP - 1) / QP + W;
+            lo = (long long)(blockIdx.x % U) * t;
+            hi = lo + t;
+        }
+        if (lo >= hi) return;
     }
-    /* sequences without positions: zeros */
-    for (int b = blockIdx.x; b < a.n_seqs; b += gridDim.x) {
-        int f;
-        bool bad;
-        if (seq_span(a, b, f, bad) == 0)
-            for (int i = tid; i < a.n_heads * a.kv.hd; i += AT_THREADS) a.out[b * a.ldo + i] = 0.0f;
-    }
-    if (s_lo >= s_hi) return;
 
     /* ---- the loader's place: sequence, unit of it, quantum of that ---- */
-    int lb = s_b, first, len, nq, lu, lq;
+    int lb = s_b, first = s_first, len = s_len, lu, lq;
+    int nq = (len - first + QP - 1) / QP;
     long long ubase;                                   /* where the loader's unit begins */
     int left;                                          /* time to the share's end */
     bool bad_;
-    len = seq_span(a, lb, first, bad_);
-    nq = (len - first + QP - 1) / QP;
     {
-        const long long rel = s_lo - s_base;
-        lu = (int)(rel / (nq + W));
+        const long long rel = lo - s_at;
+        lu = rel >> 31 ? (int)(rel / (nq + W)) : (int)((unsigned)rel / (unsigned)(nq + W));
         const int off = (int)(rel - (long long)lu * (nq + W));
         lq = max(0, off - W);
-        ubase = s_lo - off;
-        left = (int)(s_hi - ubase) - W - lq;
+        ubase = lo - off;
+        left = (int)min(hi - ubase, 1ll << 30) - W - lq;
     }
     if (left <= 0) return;
+    const int b0_ = lb, u0_ = lu;
     const bool whole0 = lq == 0;                       /* the first unit begins in this share */
     const int nq0 = nq;
     const long long ubase0 = ubase;
     const int prow = lane & (RW - 1);
     int pg[LK], pslot[LK];
     bool pin[LK];
+    /* 32 entries of the sequence's table row from tb0 on, an entry a lane; a tile's are among them unless
+     * pages are so short that it may span more (a.near 0), where each row's entry is loaded */
+    int tab = -1, tb0 = 0, tbn = 0;
     auto look = [&]() {                                /* pages of the lane's rows of the loader's tile */
+        const int p0 = first + (lq * AT_WARPS + warp) * TP;
+        if (a.near && p0 < len) {
+            const int i0 = a.kv.page_of(p0), i1 = min(p0 + TP, len) - 1;
+            if (i0 < tb0 || i1 >= tbn) {
+                tb0 = i0;
+                tbn = (int)min((long long)(tb0 + 32) * a.kv.page, (long long)INT_MAX);
+                tab = tb0 + lane < a.kv.ld_table ? __ldg(a.kv.table + (size_t)lb * a.kv.ld_table + tb0 + lane) : -1;
+            }
+        }
 #pragma unroll
         for (int k = 0; k < LK; k++) {
-            const int p = first + (lq * AT_WARPS + warp) * TP + k * RW + prow;
+            const int p = p0 + k * RW + prow;
             pin[k] = p < len;
-            pg[k] = -1;
-            pslot[k] = 0;
-            if (pin[k]) {
-                const int pi = p / a.kv.page;
-                pslot[k] = p - pi * a.kv.page;
-                pg[k] = __ldg(a.kv.table + (size_t)lb * a.kv.ld_table + pi);
-            }
+            const int pi = pin[k] ? a.kv.page_of(p) : tb0;
+            pslot[k] = p - pi * a.kv.page;
+            if (a.near) pg[k] = __shfl_sync(0xffffffffu, tab, (pi - tb0) & 31);
+            else pg[k] = pin[k] ? __ldg(a.kv.table + (size_t)lb * a.kv.ld_table + pi) : -1;
         }
     };
     enum { LAST_OF_UNIT = 1 << 28, LAST_OF_SHARE = 1 << 29 };
@@ -552,22 +661,36 @@ __global__ void __launch_bounds__(AT_THREADS, OCC) paged_attend_kernel(const __g
             }
         }
         const unsigned rowb = (unsigned)a.kv.hd * ES;
+        bool full = rowb == PITCH;                     /* every row of the tile is there, and as long as the slot's */
 #pragma unroll
-        for (int e = 0; e < TP * CPR / 32; e++) {
-            const int idx = lane + 32 * e, t = idx / CPR, ch = idx % CPR, k = (32 * e / CPR) / RW;
-            const unsigned rr = __shfl_sync(0xffffffffu, row[k], t & (RW - 1));
-            const bool lv = ((live[k] >> (t & (RW - 1))) & 1u) && ch * 16 < (int)rowb;
-            const size_t off = (size_t)rr * rowb + (lv ? ch * 16 : 0);
-            int kx, vx;                                /* swizzles: which of 8 bank groups a row starts at */
-            if constexpr (KV == KC_F32) {
-                kx = ((t & 1) << 2) | ((t >> 1) & 3);
-                vx = t & 7;
-            } else {
-                kx = vx = CPR >= 8 ? (t & 7) : ((t >> 1) & 3);
+        for (int k = 0; k < LK; k++) full &= live[k] == (unsigned)((1ull << RW) - 1);
+        auto rows = [&](auto all) {
+#pragma unroll
+            for (int e = 0; e < TP * CPR / 32; e++) {
+                const int idx = lane + 32 * e, t = idx / CPR, ch = idx % CPR, k = (32 * e / CPR) / RW;
+                const unsigned rr = __shfl_sync(0xffffffffu, row[k], t & (RW - 1));
+                int kx, vx;                            /* swizzles: which of 8 bank groups a row starts at */
+                if constexpr (KV == KC_F32) {
+                    kx = ((t & 1) << 2) | ((t >> 1) & 3);
+                    vx = t & 7;
+                } else {
+                    kx = vx = CPR >= 8 ? (t & 7) : ((t >> 1) & 3);
+                }
+                const uint32_t dk = sk + t * PITCH + ((ch ^ kx) << 4), dv = sk + VOFF + t * PITCH + ((ch ^ vx) << 4);
+                if constexpr (decltype(all)::value) {
+                    const size_t off = (size_t)rr * PITCH + ch * 16;
+                    cp_async16s(dk, a.kv.k + off);
+                    cp_async16s(dv, a.kv.v + off);
+                } else {
+                    const bool lv = ((live[k] >> (t & (RW - 1))) & 1u) && ch * 16 < (int)rowb;
+                    const size_t off = (size_t)rr * rowb + (lv ? ch * 16 : 0);
+                    cp_async16z(dk, a.kv.k + off, lv);
+                    cp_async16z(dv, a.kv.v + off, lv);
+                }
             }
-            cp_async16z(sk + t * PITCH + ((ch ^ kx) << 4), a.kv.k + off, lv);
-            cp_async16z(sk + VOFF + t * PITCH + ((ch ^ vx) << 4), a.kv.v + off, lv);
-        }
+        };
+        if (full) rows(std::true_type{});
+        else rows(std::false_type{});
         if (lane == 0) {
             const bool eu = lq == nq - 1;
             const int f = (eu ? LAST_OF_UNIT : 0) | (left <= (eu ? 1 + W : 1) ? LAST_OF_SHARE : 0);
@@ -591,12 +714,43 @@ __global__ void __launch_bounds__(AT_THREADS, OCC) paged_attend_kernel(const __g
                     len = seq_span(a, lb, first, bad_);
                     nq = (len - first + QP - 1) / QP;
                 } while (nq == 0);
+                tbn = 0;                               /* another table row */
             }
         } else {
             lq++;
         }
         look();
     };
+    /* the lane's part of a unit's query rows, as loaded */
+    float xq[MT][HD / 4];
+    auto fetch_q = [&](int b, int u) {
+        const int g = u / a.chunks, h0 = (u - g * a.chunks) * HC, nh = min(HC, a.group - h0);
+        const float *qb = a.q + b * a.ldq + (size_t)(g * a.group + h0) * a.kv.hd;
+#pragma unroll
+        for (int mt = 0; mt < MT; mt++) {
+            const bool on = mt * 8 + r < nh;
+            const float *qh = qb + (size_t)(mt * 8 + r) * a.kv.hd;
+#pragma unroll
+            for (int j = 0; j < HD / 16; j++) {
+                if constexpr (KV == KC_F16) {          /* dims 16 j + 2 c + {0, 1, 8, 9} */
+#pragma unroll
+                    for (int i = 0; i < 2; i++) {
+                        const int d = 16 * j + 8 * i + 2 * c;
+                        float2 t = make_float2(0.0f, 0.0f);
+                        if (on && d < a.kv.hd) t = __ldg((const float2 *)(qh + d));
+                        xq[mt][4 * j + 2 * i] = t.x;
+                        xq[mt][4 * j + 2 * i + 1] = t.y;
+                    }
+                } else {                               /* dims 16 j + 4 c + {0, 1, 2, 3} */
+                    const int d = 16 * j + 4 * c;
+                    float4 t = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+                    if (on && d < a.kv.hd) t = __ldg((const float4 *)(qh + d));
+                    xq[mt][4 * j] = t.x; xq[mt][4 * j + 1] = t.y; xq[mt][4 * j + 2] = t.z; xq[mt][4 * j + 3] = t.w;
+                }
+            }
+        }
+    };
+    fetch_q(lb, lu);
     look();
 #pragma unroll
     for (int s = 0; s < S - 1; s++) {
@@ -611,89 +765,57 @@ __global__ void __launch_bounds__(AT_THREADS, OCC) paged_attend_kernel(const __g
     /* ---- the compute side ---- */
     constexpr int QR = KV == KC_F32 ? HD / 8 * 4 : (KV == KC_F16 ? HD / 16 * 4 : HD / 32 * 2);
     unsigned qf[MT][QR];                               /* the query fragments */
-    float qc[MT];                                      /* score of a raw product, times log2 e without a soft-cap */
+    float qc[MT];                                      /* score of a raw product, times log2 e, or over the soft-cap */
     constexpr int NACC = HD / 4;
-    float acc[MT][NACC], m[MT], l[MT];
+    float2 acc[MT][NACC / 2];                          /* see finish for which dimensions */
+    float m[MT], l[MT];                                /* running maxima, and the lane's part of the weights' sums */
     const float LOG2E = 1.4426950408889634f;
-    int cu_b = -1, cu_u = -1;
-    bool fresh = true;                                 /* the current unit begins in this share */
+    int cu_b = b0_, cu_u = u0_;                        /* the current unit */
+    bool fresh = whole0;                               /* it begins in this share */
 
-    auto load_q = [&](int b, int u) {
-        const int g = u / a.chunks, h0 = (u - g * a.chunks) * HC, nh = min(HC, a.group - h0);
-        const float *qb = a.q + b * a.ldq + (size_t)(g * a.group + h0) * a.kv.hd;
+    /* the fragments of the query rows in xq */
+    auto set_q = [&]() {
+        const float post = a.softcap > 0.0f ? a.inv_softcap : LOG2E;
 #pragma unroll
         for (int mt = 0; mt < MT; mt++) {
-            const bool on = mt * 8 + r < nh;
-            const float *qh = qb + (size_t)(mt * 8 + r) * a.kv.hd;
-            const float post = a.softcap > 0.0f ? 1.0f : LOG2E;
-            if constexpr (KV == KC_F16) {
-                float x[HD / 4];
-                float mx = 0.0f;
+            const float *x = xq[mt];
+            if constexpr (KV == KC_F32) {
 #pragma unroll
-                for (int j = 0; j < HD / 16; j++)
-#pragma unroll
-                    for (int i = 0; i < 2; i++) {
-                        const int d = 16 * j + 8 * i + 2 * c;
-                        float2 t = make_float2(0.0f, 0.0f);
-                        if (on && d < a.kv.hd) t = __ldg((const float2 *)(qh + d));
-                        x[4 * j + 2 * i] = t.x;
-                        x[4 * j + 2 * i + 1] = t.y;
-                        mx = fmaxf(mx, fmaxf(fabsf(t.x), fabsf(t.y)));
-                    }
-                mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
-                mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
-                /* the largest |q| of the head is brought to [2^12, 2^13), a power of two exactly, so
-                 * that the low parts of all but vanishing values stay normal f16 */
-                int ex = (int)((__float_as_uint(mx) >> 23) & 255) - 127;
-                ex = min(max(ex, -100), 100);
-                const float up = __uint_as_float((unsigned)(127 + 12 - ex) << 23);
-                qc[mt] = a.scale * __uint_as_float((unsigned)(127 - 12 + ex) << 23) * post;
-#pragma unroll
-                for (int j = 0; j < HD / 16; j++)
-#pragma unroll
-                    for (int i = 0; i < 2; i++)
-                        split_f16(x[4 * j + 2 * i] * up, x[4 * j + 2 * i + 1] * up, qf[mt][4 * j + 2 * i],
-                                  qf[mt][4 * j + 2 * i + 1]);
-            } else if constexpr (KV == KC_F32) {
-#pragma unroll
-                for (int j = 0; j < HD / 16; j++) {
-                    const int d = 16 * j + 4 * c;
-                    float4 t = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-                    if (on && d < a.kv.hd) t = __ldg((const float4 *)(qh + d));
-                    split_tf32(t.x, qf[mt][8 * j], qf[mt][8 * j + 1]);
-                    split_tf32(t.y, qf[mt][8 * j + 2], qf[mt][8 * j + 3]);
-                    split_tf32(t.z, qf[mt][8 * j + 4], qf[mt][8 * j + 5]);
-                    split_tf32(t.w, qf[mt][8 * j + 6], qf[mt][8 * j + 7]);
-                }
+                for (int i = 0; i < HD / 4; i++) split_tf32(x[i], qf[mt][2 * i], qf[mt][2 * i + 1]);
                 qc[mt] = a.scale * post;
             } else {
-                /* the query head quantized as a cache row is (ops/ops.c:229-233) */
-                float x[HD / 4];
-                float mx = 0.0f;
+                float mx = 0.0f;                       /* of the head, whose values the four lanes of a row hold */
 #pragma unroll
-                for (int j = 0; j < HD / 16; j++) {
-                    const int d = 16 * j + 4 * c;
-                    float4 t = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-                    if (on && d < a.kv.hd) t = __ldg((const float4 *)(qh + d));
-                    x[4 * j] = t.x; x[4 * j + 1] = t.y; x[4 * j + 2] = t.z; x[4 * j + 3] = t.w;
-                    mx = fmaxf(mx, fmaxf(fmaxf(fabsf(t.x), fabsf(t.y)), fmaxf(fabsf(t.z), fabsf(t.w))));
-                }
+                for (int i = 0; i < HD / 4; i++) mx = fmaxf(mx, fabsf(x[i]));
                 mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
                 mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
-                const bool tiny = mx < 1e-30f;
-                const float id = tiny ? 0.0f : __fdiv_rn(127.0f, mx), qd = tiny ? 0.0f : __fdiv_rn(mx, 127.0f);
+                if constexpr (KV == KC_F16) {
+                    /* the largest |q| of the head is brought to [2^12, 2^13), a power of two exactly, so
+                     * that the low parts of all but vanishing values stay normal f16 */
+                    int ex = (int)((__float_as_uint(mx) >> 23) & 255) - 127;
+                    ex = min(max(ex, -100), 100);
+                    const float up = __uint_as_float((unsigned)(127 + 12 - ex) << 23);
+                    qc[mt] = a.scale * __uint_as_float((unsigned)(127 - 12 + ex) << 23) * post;
 #pragma unroll
-                for (int j = 0; j < HD / 16; j++) {
-                    unsigned w = 0;
+                    for (int i = 0; i < HD / 8; i++)
+                        split_f16(x[2 * i] * up, x[2 * i + 1] * up, qf[mt][2 * i], qf[mt][2 * i + 1]);
+                } else {
+                    /* the query head quantized as a cache row is (ops/ops.c:229-233) */
+                    const bool tiny = mx < 1e-30f;
+                    const float id = tiny ? 0.0f : __fdiv_rn(127.0f, mx), qd = tiny ? 0.0f : __fdiv_rn(mx, 127.0f);
 #pragma unroll
-                    for (int i = 0; i < 4; i++) {
-                        const float u = truncf(__fadd_rn(__fmul_rn(x[4 * j + i], id), copysignf(0.5f, x[4 * j + i])));
-                        const int qi = tiny ? 0 : (int)fminf(fmaxf(u, -127.0f), 127.0f);
-                        w |= ((unsigned)qi & 0xffu) << (8 * i);
+                    for (int j = 0; j < HD / 16; j++) {
+                        unsigned w = 0;
+#pragma unroll
+                        for (int i = 0; i < 4; i++) {
+                            const float u = truncf(__fadd_rn(__fmul_rn(x[4 * j + i], id), copysignf(0.5f, x[4 * j + i])));
+                            const int qi = tiny ? 0 : (int)fminf(fmaxf(u, -127.0f), 127.0f);
+                            w |= ((unsigned)qi & 0xffu) << (8 * i);
+                        }
+                        qf[mt][j] = w;
                     }
-                    qf[mt][j] = w;
+                    qc[mt] = __fmul_rn(qd, a.scale) * post;
                 }
-                qc[mt] = __fmul_rn(qd, a.scale) * post;
             }
         }
     };
@@ -704,12 +826,6 @@ __global__ void __launch_bounds__(AT_THREADS, OCC) paged_attend_kernel(const __g
         float s[MT][NT][2];
         if constexpr (KV == KC_F16) {
             float d[MT][NT][4];
-#pragma unroll
-            for (int mt = 0; mt < MT; mt++)
-#pragma unroll
-                for (int nt = 0; nt < NT; nt++)
-#pragma unroll
-                    for (int i = 0; i < 4; i++) d[mt][nt][i] = 0.0f;
             const uint32_t kb = sk + (lane & 7) * PITCH;
             const int x = (lane >> 3) ^ (lane & 7);
 #pragma unroll
@@ -722,7 +838,8 @@ __global__ void __launch_bounds__(AT_THREADS, OCC) paged_attend_kernel(const __g
                     for (int mt = 0; mt < MT; mt++) {
                         const unsigned a0[4] = { qf[mt][8 * jj], qf[mt][8 * jj + 1], qf[mt][8 * jj + 2], qf[mt][8 * jj + 3] };
                         const unsigned a1[4] = { qf[mt][8 * jj + 4], qf[mt][8 * jj + 5], qf[mt][8 * jj + 6], qf[mt][8 * jj + 7] };
-                        mma_f16(d[mt][nt], a0, b[0], b[1]);
+                        if (jj == 0) mma_f16_first(d[mt][nt], a0, b[0], b[1]);
+                        else mma_f16(d[mt][nt], a0, b[0], b[1]);
                         mma_f16(d[mt][nt], a1, b[2], b[3]);
                     }
                 }
@@ -735,12 +852,6 @@ __global__ void __launch_bounds__(AT_THREADS, OCC) paged_attend_kernel(const __g
                 }
         } else if constexpr (KV == KC_F32) {
             float dh[MT][NT][4], dl[MT][NT][4];
-#pragma unroll
-            for (int mt = 0; mt < MT; mt++)
-#pragma unroll
-                for (int nt = 0; nt < NT; nt++)
-#pragma unroll
-                    for (int i = 0; i < 4; i++) dh[mt][nt][i] = dl[mt][nt][i] = 0.0f;
             const uint32_t kb = sk + r * PITCH;
             const int x = c ^ (((r & 1) << 2) | (r >> 1));
 #pragma unroll
@@ -757,8 +868,13 @@ __global__ void __launch_bounds__(AT_THREADS, OCC) paged_attend_kernel(const __g
                     for (int mt = 0; mt < MT; mt++) {
                         const unsigned a0[4] = { qf[mt][8 * jj], qf[mt][8 * jj + 1], qf[mt][8 * jj + 2], qf[mt][8 * jj + 3] };
                         const unsigned a1[4] = { qf[mt][8 * jj + 4], qf[mt][8 * jj + 5], qf[mt][8 * jj + 6], qf[mt][8 * jj + 7] };
-                        mma_tf32(dh[mt][nt], a0, h[0], h[1]);
-                        mma_tf32(dl[mt][nt], a0, w[0], w[1]);
+                        if (jj == 0) {
+                            mma_tf32_first(dh[mt][nt], a0, h[0], h[1]);
+                            mma_tf32_first(dl[mt][nt], a0, w[0], w[1]);
+                        } else {
+                            mma_tf32(dh[mt][nt], a0, h[0], h[1]);
+                            mma_tf32(dl[mt][nt], a0, w[0], w[1]);
+                        }
                         mma_tf32(dh[mt][nt], a1, h[2], h[3]);
                         mma_tf32(dl[mt][nt], a1, w[2], w[3]);
                     }
@@ -777,7 +893,7 @@ __global__ void __launch_bounds__(AT_THREADS, OCC) paged_attend_kernel(const __g
 #pragma unroll
                 for (int nt = 0; nt < NT; nt++)
 #pragma unroll
-                    for (int i = 0; i < 4; i++) d[mt][nt][i] = 0;
+                    for (int i = 0; i < 4; i++) d[mt][nt][i] = 0x4b400000;   /* 1.5 * 2^23: the sums come out as its floats */
             const uint32_t kb = sk + (lane & 7) * PITCH;
             const int x = (lane >> 3) ^ (CPR >= 8 ? (lane & 7) : ((lane >> 1) & 3));
 #pragma unroll
@@ -798,42 +914,52 @@ __global__ void __launch_bounds__(AT_THREADS, OCC) paged_attend_kernel(const __g
                 const float2 e = *(const float2 *)(kd + nt * 8 + 2 * c);
 #pragma unroll
                 for (int mt = 0; mt < MT; mt++) {
-                    s[mt][nt][0] = (float)d[mt][nt][0] * qc[mt] * e.x;
-                    s[mt][nt][1] = (float)d[mt][nt][1] * qc[mt] * e.y;
+                    s[mt][nt][0] = (__int_as_float(d[mt][nt][0]) - 12582912.0f) * qc[mt] * e.x;
+                    s[mt][nt][1] = (__int_as_float(d[mt][nt][1]) - 12582912.0f) * qc[mt] * e.y;
                 }
             }
         }
         /* soft-cap, mask, running softmax in base 2 */
         constexpr float LIFT = KV == KC_F32 ? 0.0f : 15.0f;   /* weights in (0, 2^15]: small ones stay normal f16 */
-        float corr[MT];
+        float2 corr[MT];
+        bool all = true;
+#pragma unroll
+        for (int k = 0; k < LK; k++) all &= live[k] == (unsigned)((1ull << RW) - 1);
 #pragma unroll
         for (int mt = 0; mt < MT; mt++) {
-            float mx = -INFINITY;
+            if (a.softcap > 0.0f) {
 #pragma unroll
-            for (int nt = 0; nt < NT; nt++)
+                for (int nt = 0; nt < NT; nt++)
 #pragma unroll
-                for (int i = 0; i < 2; i++) {
-                    float v = s[mt][nt][i];
-                    if (a.softcap > 0.0f) v = a.softcap * tanhf(__fdiv_rn(v, a.softcap)) * LOG2E;
-                    v = (live[nt * 8 / RW] >> ((nt * 8) % RW + 2 * c + i)) & 1u ? v : -INFINITY;
-                    s[mt][nt][i] = v;
-                    mx = fmaxf(mx, v);
-                }
+                    for (int i = 0; i < 2; i++)
+                        s[mt][nt][i] = a.softcap * LOG2E * tanhf(s[mt][nt][i]);
+            }
+            if (!all) {
+#pragma unroll
+                for (int nt = 0; nt < NT; nt++)
+#pragma unroll
+                    for (int i = 0; i < 2; i++)
+                        if (!((live[nt * 8 / RW] >> ((nt * 8) % RW + 2 * c + i)) & 1u)) s[mt][nt][i] = -INFINITY;
+            }
+            float mx = fmaxf(s[mt][0][0], s[mt][0][1]);
+#pragma unroll
+            for (int nt = 1; nt < NT; nt++) mx = fmaxf(mx, fmaxf(s[mt][nt][0], s[mt][nt][1]));
             mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
             mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
-            const float mn = fmaxf(m[mt], mx), base = mn == -INFINITY ? 0.0f : mn;
-            corr[mt] = exp2f(m[mt] - base);
+            const float mn = fmaxf(m[mt], mx), base = mn == -INFINITY ? 0.0f : mn, sub = base - LIFT;
+            const float cr = ex2(m[mt] - base);
+            corr[mt] = make_float2(cr, cr);
             m[mt] = mn;
             float sum = 0.0f;
 #pragma unroll
             for (int nt = 0; nt < NT; nt++)
 #pragma unroll
                 for (int i = 0; i < 2; i++) {
-                    const float p = exp2f(s[mt][nt][i] - base + LIFT);
+                    const float p = ex2(s[mt][nt][i] - sub);
                     s[mt][nt][i] = p;
                     sum += p;
                 }
-            l[mt] = l[mt] * corr[mt] + sum;
+            l[mt] = l[mt] * cr + sum;
         }
         /* the weighted sum of V's rows */
         if constexpr (KV == KC_F16) {
@@ -850,26 +976,24 @@ __global__ void __launch_bounds__(AT_THREADS, OCC) paged_attend_kernel(const __g
             for (int jj = 0; jj < HD / 16; jj++) {
                 float d[MT][2][4];
 #pragma unroll
-                for (int mt = 0; mt < MT; mt++)
-#pragma unroll
-                    for (int i = 0; i < 4; i++) d[mt][0][i] = d[mt][1][i] = 0.0f;
-#pragma unroll
                 for (int ks = 0; ks < KS; ks++) {
                     unsigned b[4];
                     ldsm4t(b, vb + ks * 16 * PITCH + (((2 * jj) ^ x) << 4));
 #pragma unroll
                     for (int mt = 0; mt < MT; mt++) {
-                        mma_f16(d[mt][0], w[mt][ks], b[0], b[1]);
-                        mma_f16(d[mt][1], w[mt][ks], b[2], b[3]);
+                        if (ks == 0) {
+                            mma_f16_first(d[mt][0], w[mt][ks], b[0], b[1]);
+                            mma_f16_first(d[mt][1], w[mt][ks], b[2], b[3]);
+                        } else {
+                            mma_f16(d[mt][0], w[mt][ks], b[0], b[1]);
+                            mma_f16(d[mt][1], w[mt][ks], b[2], b[3]);
+                        }
                     }
                 }
 #pragma unroll
                 for (int mt = 0; mt < MT; mt++) {
-                    float *o = &acc[mt][4 * jj];
-                    o[0] = o[0] * corr[mt] + (d[mt][0][0] + d[mt][0][2]);
-                    o[1] = o[1] * corr[mt] + (d[mt][0][1] + d[mt][0][3]);
-                    o[2] = o[2] * corr[mt] + (d[mt][1][0] + d[mt][1][2]);
-                    o[3] = o[3] * corr[mt] + (d[mt][1][1] + d[mt][1][3]);
+                    carry(acc[mt][2 * jj], corr[mt], d[mt][0]);
+                    carry(acc[mt][2 * jj + 1], corr[mt], d[mt][1]);
                 }
             }
         } else if constexpr (KV == KC_F32) {
@@ -887,12 +1011,6 @@ __global__ void __launch_bounds__(AT_THREADS, OCC) paged_attend_kernel(const __g
             for (int j = 0; j < HD / 32; j++) {
                 float d[MT][4][4];
 #pragma unroll
-                for (int mt = 0; mt < MT; mt++)
-#pragma unroll
-                    for (int i = 0; i < 4; i++)
-#pragma unroll
-                        for (int k = 0; k < 4; k++) d[mt][i][k] = 0.0f;
-#pragma unroll
                 for (int nt = 0; nt < NT; nt++) {
                     const float4 ya = lds4(v0 + nt * 8 * PITCH + (((8 * j) ^ x0) << 4));
                     const float4 yb = lds4(v1 + nt * 8 * PITCH + (((8 * j) ^ x1) << 4));
@@ -904,7 +1022,8 @@ __global__ void __launch_bounds__(AT_THREADS, OCC) paged_attend_kernel(const __g
                         split_tf32(y1[i], h1, g1);
 #pragma unroll
                         for (int mt = 0; mt < MT; mt++) {
-                            mma_tf32(d[mt][i], w[mt][nt], g0, g1);
+                            if (nt == 0) mma_tf32_first(d[mt][i], w[mt][nt], g0, g1);
+                            else mma_tf32(d[mt][i], w[mt][nt], g0, g1);
                             mma_tf32(d[mt][i], w[mt][nt], h0, h1);
                         }
                     }
@@ -912,11 +1031,7 @@ __global__ void __launch_bounds__(AT_THREADS, OCC) paged_attend_kernel(const __g
 #pragma unroll
                 for (int mt = 0; mt < MT; mt++)
 #pragma unroll
-                    for (int i = 0; i < 4; i++) {
-                        float *o = &acc[mt][8 * j + i];
-                        o[0] = o[0] * corr[mt] + (d[mt][i][0] + d[mt][i][2]);
-                        o[4] = o[4] * corr[mt] + (d[mt][i][1] + d[mt][i][3]);
-                    }
+                    for (int i = 0; i < 4; i++) carry(acc[mt][4 * j + i], corr[mt], d[mt][i]);
             }
         } else {
             /* the rows' scales join the weights; a power of two keeps the product in f16's range */
@@ -952,12 +1067,6 @@ __global__ void __launch_bounds__(AT_THREADS, OCC) paged_attend_kernel(const __g
             for (int jj = 0; jj < HD / 32; jj++) {
                 float d[MT][4][4];
 #pragma unroll
-                for (int mt = 0; mt < MT; mt++)
-#pragma unroll
-                    for (int k = 0; k < 4; k++)
-#pragma unroll
-                        for (int i = 0; i < 4; i++) d[mt][k][i] = 0.0f;
-#pragma unroll
                 for (int ks = 0; ks < KS; ks++) {
                     unsigned b[4];
                     ldsm4t(b, vb + ks * 16 * PITCH + (((2 * jj) ^ x) << 4));
@@ -966,27 +1075,34 @@ __global__ void __launch_bounds__(AT_THREADS, OCC) paged_attend_kernel(const __g
                     bytes(b[1], e1, o1);
 #pragma unroll
                     for (int mt = 0; mt < MT; mt++) {
-                        mma_f16(d[mt][0], w[mt][ks], e0, e1);
-                        mma_f16(d[mt][1], w[mt][ks], o0, o1);
+                        if (ks == 0) {
+                            mma_f16_first(d[mt][0], w[mt][ks], e0, e1);
+                            mma_f16_first(d[mt][1], w[mt][ks], o0, o1);
+                        } else {
+                            mma_f16(d[mt][0], w[mt][ks], e0, e1);
+                            mma_f16(d[mt][1], w[mt][ks], o0, o1);
+                        }
                     }
                     bytes(b[2], e0, o0);
                     bytes(b[3], e1, o1);
 #pragma unroll
                     for (int mt = 0; mt < MT; mt++) {
-                        mma_f16(d[mt][2], w[mt][ks], e0, e1);
-                        mma_f16(d[mt][3], w[mt][ks], o0, o1);
+                        if (ks == 0) {
+                            mma_f16_first(d[mt][2], w[mt][ks], e0, e1);
+                            mma_f16_first(d[mt][3], w[mt][ks], o0, o1);
+                        } else {
+                            mma_f16(d[mt][2], w[mt][ks], e0, e1);
+                            mma_f16(d[mt][3], w[mt][ks], o0, o1);
+                        }
                     }
                 }
 #pragma unroll
                 for (int mt = 0; mt < MT; mt++)
 #pragma unroll
-                    for (int k = 0; k < 2; k++) {
-                        float *o = &acc[mt][8 * jj + 4 * k];
-                        o[0] = o[0] * corr[mt] + (d[mt][2 * k][0] + d[mt][2 * k][2]) * upf;
-                        o[1] = o[1] * corr[mt] + (d[mt][2 * k + 1][0] + d[mt][2 * k + 1][2]) * upf;
-                        o[2] = o[2] * corr[mt] + (d[mt][2 * k][1] + d[mt][2 * k][3]) * upf;
-                        o[3] = o[3] * corr[mt] + (d[mt][2 * k + 1][1] + d[mt][2 * k + 1][3]) * upf;
-                    }
+                    for (int k = 0; k < 4; k++)
+                        acc[mt][4 * jj + k] = fma2(acc[mt][4 * jj + k], corr[mt],
+                                                   mul2(add2(make_float2(d[mt][k][0], d[mt][k][1]),
+                                                             make_float2(d[mt][k][2], d[mt][k][3])), upf));
             }
         }
     };
@@ -1015,23 +1131,21 @@ __global__ void __launch_bounds__(AT_THREADS, OCC) paged_attend_kernel(const __g
                 const int x = (r & 3) * 8;             /* rows start at different banks */
 #pragma unroll
                 for (int j = 0; j < HD / 32; j++) {
+                    const float2 *o = &acc[mt][4 * j];
                     if constexpr (KV == KC_F32) {
-                        /* acc[8 j + i]: dim 32 j + 8 c + i */
+                        /* o[i]: dims 32 j + 8 c + i and + 4 */
                         float *p = row + ((32 * j + 8 * c) ^ x);
-                        *(float4 *)p = make_float4(acc[mt][8 * j], acc[mt][8 * j + 1], acc[mt][8 * j + 2], acc[mt][8 * j + 3]);
-                        *(float4 *)(p + 4) =
-                            make_float4(acc[mt][8 * j + 4], acc[mt][8 * j + 5], acc[mt][8 * j + 6], acc[mt][8 * j + 7]);
+                        *(float4 *)p = make_float4(o[0].x, o[1].x, o[2].x, o[3].x);
+                        *(float4 *)(p + 4) = make_float4(o[0].y, o[1].y, o[2].y, o[3].y);
                     } else if constexpr (KV == KC_F16) {
 #pragma unroll
-                        for (int k = 0; k < 4; k++)    /* acc[2 n + i]: dim 8 n + 2 c + i, n = 4 j + k */
-                            *(float2 *)(row + ((32 * j + 8 * k + 2 * c) ^ x)) =
-                                make_float2(acc[mt][8 * j + 2 * k], acc[mt][8 * j + 2 * k + 1]);
+                        for (int k = 0; k < 4; k++)    /* o[k]: dims 32 j + 8 k + 2 c and + 1 */
+                            *(float2 *)(row + ((32 * j + 8 * k + 2 * c) ^ x)) = o[k];
                     } else {
 #pragma unroll
-                        for (int k = 0; k < 2; k++)    /* acc[4 n + i]: dim 16 n + 4 c + i, n = 2 j + k */
+                        for (int k = 0; k < 2; k++)    /* o[2 k], o[2 k + 1]: dims 32 j + 16 k + 4 c + {0, 2}, {1, 3} */
                             *(float4 *)(row + ((32 * j + 16 * k + 4 * c) ^ x)) =
-                                make_float4(acc[mt][8 * j + 4 * k], acc[mt][8 * j + 4 * k + 1],
-                                            acc[mt][8 * j + 4 * k + 2], acc[mt][8 * j + 4 * k + 3]);
+                                make_float4(o[2 * k].x, o[2 * k + 1].x, o[2 * k].y, o[2 * k + 1].y);
                     }
                 }
             }
@@ -1074,13 +1188,11 @@ __global__ void __launch_bounds__(AT_THREADS, OCC) paged_attend_kernel(const __g
 
     __shared__ int s_c0, s_c1;
     auto leave = [&](int b, int u) {                   /* the unit's piece is written: join them if it was the last */
-        __threadfence();
-        __syncthreads();
         if (tid == 0) {
+            __threadfence();                           /* finish's barrier is behind every thread's part of it */
             /* a unit that is not fresh is the share's first, one that is left unfinished its last */
             const long long x = (fresh ? ubase : ubase0) + W;
-            const int c0 = share_owner(x, s_ncta, s_total);
-            const int c1 = share_owner(x + (fresh ? nq : nq0) - 1, s_ncta, s_total);
+            const int c0 = (int)(x / chunk), c1 = (int)((x + (fresh ? nq : nq0) - 1) / chunk);
             const unsigned n = atomicAdd(a.count + c1, 1u);
             s_last = n == (unsigned)(c1 - c0);
             if (s_last) a.count[c1] = 0u;
@@ -1089,9 +1201,21 @@ __global__ void __launch_bounds__(AT_THREADS, OCC) paged_attend_kernel(const __g
             __threadfence();
         }
         __syncthreads();
-        if (s_last) join_pieces<HD, MT>(a, b, u, s_c0, s_c1);
+        if (s_last) join_pieces<HD, MT>(a, b, u, s_c0, s_c1, comb);
+        if (s_last) __syncthreads();                   /* (comb is the next unit's) */
     };
 
+    auto begin = [&]() {
+        set_q();
+#pragma unroll
+        for (int mt = 0; mt < MT; mt++) {
+            m[mt] = -INFINITY;
+            l[mt] = 0.0f;
+#pragma unroll
+            for (int i = 0; i < NACC / 2; i++) acc[mt][i] = make_float2(0.0f, 0.0f);
+        }
+    };
+    begin();
     for (int it = 0; it < issued; it++) {
         const int stage = it % S;
         const int4 f = info[stage];                    /* written when the slot's copies were issued */
@@ -1100,15 +1224,9 @@ __global__ void __launch_bounds__(AT_THREADS, OCC) paged_attend_kernel(const __g
             /* a new unit: its queries are on their way while the tile arrives */
             cu_b = f.x;
             cu_u = fu;
-            fresh = it > 0 || whole0;
-            load_q(cu_b, cu_u);
-#pragma unroll
-            for (int mt = 0; mt < MT; mt++) {
-                m[mt] = -INFINITY;
-                l[mt] = 0.0f;
-#pragma unroll
-                for (int i = 0; i < NACC; i++) acc[mt][i] = 0.0f;
-            }
+            fresh = true;
+            fetch_q(cu_b, cu_u);
+            begin();
         }
         cp_async_wait_but<S - 2>();
         __syncwarp();

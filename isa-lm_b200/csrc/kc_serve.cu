@@ -116,8 +116,8 @@ static int check_cache(const kc_paged_kv *kv) {
         return refuse("n_pages, page_size, n_kv_heads, n_seqs and ld_table must be at least 1");
     if ((double)kv->n_pages * kv->page_size * kv->n_kv_heads >= 4294967296.0)
         return refuse("the pool's rows (n_pages * page_size * n_kv_heads) must be fewer than 2^32");
-    if ((double)kv->ld_table * kv->page_size > 2147483647.0)
-        return refuse("a table row (ld_table * page_size) must hold fewer than 2^31 positions");
+    if ((double)kv->ld_table * kv->page_size > 2147483647.0 - 65536.0)
+        return refuse("a table row (ld_table * page_size) must hold fewer than 2^31 - 2^16 positions");
     return KC_OK;
 }
 
@@ -129,8 +129,13 @@ static int take_cache(const kc_paged_kv *kv, const ServeDev &d, PagedKV &o) {
         PTR(kv->kd, 4);
         PTR(kv->vd, 4);
     }
+    /* p / page_size as the high half of p * page_mul, shifted: with 2^(s-1) < page_size <= 2^s, page_mul =
+     * ceil(2^(31+s) / page_size) is off by less than 2^s / page_size / 2^31 of itself */
+    int s = 0;
+    while ((1ll << s) < kv->page_size) s++;
+    const unsigned mul = s ? (unsigned)(((1ull << (31 + s)) + kv->page_size - 1) / kv->page_size) : 0u;
     o = PagedKV{ (uint8_t *)kv->k, (uint8_t *)kv->v, kv->kd, kv->vd, kv->table, kv->n_seqs, kv->ld_table, kv->n_pages,
-                 kv->page_size, kv->n_kv_heads, kv->head_dim };
+                 kv->page_size, kv->n_kv_heads, kv->head_dim, mul, s - 1 };
     return KC_OK;
 }
 
@@ -156,7 +161,7 @@ constexpr int AT_MAX_CTAS = 2048;
 /* One instance: its kernel, shared memory, and on each device the CTAs that fit. */
 struct AttendVariant {
     void (*attend)(const AttendArgs);
-    int smem, part;
+    int smem, part, tile;
     int ctas[SV_MAX_DEVICES];
 };
 
@@ -166,6 +171,7 @@ static AttendVariant make_variant() {
     v.attend = paged_attend_kernel<KV, HD, TM, MT, S, OCC>;
     v.smem = attend_smem<KV, HD, TM, MT, S>();
     v.part = part_floats<HD, MT>();
+    v.tile = att_tp<KV, TM>();
     return v;
 }
 
@@ -325,6 +331,8 @@ extern "C" int kc_paged_attend_dev(const kc_paged_kv *kv, const kc_attend_args *
     a.q = x->q; a.out = x->out; a.ldq = x->ldq; a.ldo = x->ldo; a.lens = x->lens;
     a.n_seqs = x->n_seqs; a.n_heads = x->n_heads; a.group = x->n_heads / kv->n_kv_heads;
     a.window = x->window; a.scale = x->scale; a.softcap = x->softcap;
+    a.inv_softcap = x->softcap > 0.0f ? 1.0f / x->softcap : 0.0f;
+    a.near = (v->tile - 1) / kv->page_size + 2 <= 32;
     a.unit_cost = 2;
     a.min_share = 1;
     a.count = (unsigned *)x->ws;
@@ -379,9 +387,19 @@ extern "C" int kc_logits_process_dev(const kc_logits_args *x, void *stream) {
     const dim3 grid((unsigned)x->rows, (unsigned)((x->vocab + 3 + LG_CHUNK - 1) / LG_CHUNK));
     const cudaStream_t st = (cudaStream_t)stream;
     const bool hist = pen && x->history_cap > 0;
-    if (hist && bias) logits_kernel<true, true><<<grid, LG_THREADS, 0, st>>>(a);
-    else if (hist) logits_kernel<true, false><<<grid, LG_THREADS, 0, st>>>(a);
-    else if (bias) logits_kernel<false, true><<<grid, LG_THREADS, 0, st>>>(a);
-    else logits_kernel<false, false><<<grid, LG_THREADS, 0, st>>>(a);
+    if (hist && bias) {
+        /* beyond the static limit: the attribute belongs to the device */
+        static bool done[SV_MAX_DEVICES];
+        constexpr int smem = logits_smem<true, true>();
+        if (!done[d.dev]) SK(cudaFuncSetAttribute((const void *)logits_kernel<true, true>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem), "logits");
+        done[d.dev] = true;
+        logits_kernel<true, true><<<grid, LG_THREADS, smem, st>>>(a);
+    } else if (hist) {
+        logits_kernel<true, false><<<grid, LG_THREADS, logits_smem<true, false>(), st>>>(a);
+    } else if (bias) {
+        logits_kernel<false, true><<<grid, LG_THREADS, logits_smem<false, true>(), st>>>(a);
+    } else {
+        logits_kernel<false, false><<<grid, LG_THREADS, 0, st>>>(a);
+    }
     return sv_cuda(cudaGetLastError(), "logits");
 }

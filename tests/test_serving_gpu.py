@@ -118,6 +118,28 @@ def test_attend(kv, shape):
 
 
 @pytest.mark.parametrize("kv", ["f32", "f16", "q8"])
+@pytest.mark.parametrize("n,heads,hk,hd,top", [(90, 16, 8, 64, 300), (700, 2, 1, 64, 90), (41, 8, 8, 128, 700), (140, 3, 3, 32, 60)])
+def test_attend_many_sequences(kv, n, heads, hk, hd, top):
+    """More units (sequences times KV heads) than CTAs, more sequences than threads, ragged and empty ones."""
+    rng = np.random.default_rng(n + hd)
+    page = 16
+    lens = np.where(rng.random(n) < 0.1, 0, rng.integers(1, top, n)).tolist()
+    n_pages = sum(-(-m // page) for m in lens)
+    pools = make_pool(rng, kv, n_pages, hk, page, hd)
+    table = make_table(rng, lens, page, n_pages)
+    q = rng.standard_normal((n, heads, hd)).astype(np.float32)
+    c = handle(pools, table, kv, heads)
+    dq, dl = kb.DevArray.of(q), kb.DevArray.of(np.array(lens, np.int32))
+    k, v, kd, vd = pools
+    vmax = np.abs(v.astype(np.float64)).max() if kd is None else (127 * vd).max()
+    for window in (0, 33):
+        out = c.attend(dq, dl, kb.DevArray.of(np.full(q.shape, np.nan, np.float32)), window=window)
+        want, reach = ref.attend(q, k, v, table, lens, hd ** -0.5, window, 0.0, kd, vd)
+        check(out.numpy(), want, reach, vmax, hd, max(lens))
+    kb._check(kb.lib().kc_dev_sync(), "sync")
+
+
+@pytest.mark.parametrize("kv", ["f32", "f16", "q8"])
 def test_attend_long_is_split_and_repeatable(kv):
     rng = np.random.default_rng(5)
     lens, page, hk, hd, heads = [20011, 4096], 16, 2, 128, 8
