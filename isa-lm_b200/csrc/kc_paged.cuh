@@ -268,7 +268,7 @@ struct AttendArgs {
     int window;
     float scale, softcap, inv_softcap;
     int unit_cost;                        /* a unit's own time, in quanta */
-    int min_share;                        /* least such time of a CTA's share */
+    unsigned long long grid_inv;          /* 2^64 / CTAs, rounded up */
     int near;                             /* a tile's pages lie within 32 entries of its table row */
     unsigned *count;                      /* [CTAs] pieces that have come, of the unit that ends there; 0 between calls */
     float *part;                          /* [2 * CTAs] pieces */
@@ -305,29 +305,29 @@ __device__ __forceinline__ float4 lds4(uint32_t a) {
     return v;
 }
 __device__ __forceinline__ void mma_f16(float (&c)[4], const unsigned (&a)[4], unsigned b0, unsigned b1) {
-    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
                  : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
                  : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 /* the product alone, without a sum to add it to */
 __device__ __forceinline__ void mma_f16_first(float (&c)[4], const unsigned (&a)[4], unsigned b0, unsigned b1) {
-    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%10, %10, %10, %10};"
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%10, %10, %10, %10};"
                  : "=f"(c[0]), "=f"(c[1]), "=f"(c[2]), "=f"(c[3])
                  : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(0.0f));
 }
 __device__ __forceinline__ void mma_tf32_first(float (&c)[4], const unsigned (&a)[4], unsigned b0, unsigned b1) {
-    asm volatile("mma.sync.aligned.m16n8k8.row.col.f32.tf32.tf32.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%10, %10, %10, %10};"
+    asm("mma.sync.aligned.m16n8k8.row.col.f32.tf32.tf32.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%10, %10, %10, %10};"
                  : "=f"(c[0]), "=f"(c[1]), "=f"(c[2]), "=f"(c[3])
                  : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(0.0f));
 }
 __device__ __forceinline__ void mma_tf32(float (&c)[4], const unsigned (&a)[4], unsigned b0, unsigned b1) {
-    asm volatile("mma.sync.aligned.m16n8k8.row.col.f32.tf32.tf32.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+    asm("mma.sync.aligned.m16n8k8.row.col.f32.tf32.tf32.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
                  : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
                  : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 /* rows 8-15 of A are zero */
 __device__ __forceinline__ void mma_s8(int (&c)[4], unsigned a0, unsigned a2, unsigned b0, unsigned b1) {
-    asm volatile("mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 {%0, %1, %2, %3}, {%4, %5, %6, %5}, {%7, %8}, {%0, %1, %2, %3};"
+    asm("mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 {%0, %1, %2, %3}, {%4, %5, %6, %5}, {%7, %8}, {%0, %1, %2, %3};"
                  : "+r"(c[0]), "+r"(c[1]), "+r"(c[2]), "+r"(c[3]) : "r"(a0), "r"(0), "r"(a2), "r"(b0), "r"(b1));
 }
 
@@ -387,14 +387,16 @@ __device__ __forceinline__ int seq_span(const AttendArgs &a, int b, int &first, 
     return n;
 }
 
-/* Shared memory of a warp's ring slot: K rows, V rows, and (8-bit) their scales. */
-template <int KV, int HD, int TM>
-constexpr int slot_bytes() {
-    return 2 * 32 * TM * HD + (KV == KC_Q8_0 ? 2 * att_tp<KV, TM>() * 4 : 0);
-}
+/* Shared memory: a ring of S slots for each warp (a tile's K rows, then its V
+ * rows; on a boundary of 1024 bytes, so that a row's chunk is reached by an
+ * exclusive or on the address), their 8-bit rows' scales, what each slot holds,
+ * and finish's part. */
+template <int HD, int TM>
+constexpr int slot_bytes() { return 2 * 32 * TM * HD; }
 template <int KV, int HD, int TM, int MT, int S>
 constexpr int attend_smem() {
-    return AT_WARPS * (S * (slot_bytes<KV, HD, TM>() + 16) + AT_COMB * HD * 4 + 2 * 8 * MT * 4);
+    return 1024 + AT_WARPS * (S * (slot_bytes<HD, TM>() + (KV == KC_Q8_0 ? 8 * att_tp<KV, TM>() : 0) + 16) +
+                              AT_COMB * HD * 4 + 2 * 8 * MT * 4);
 }
 
 /* sum / weights; nothing attended gives zeros */
@@ -490,128 +492,93 @@ __global__ void __launch_bounds__(AT_THREADS, OCC) paged_attend_kernel(const __g
     constexpr int NT = TP / 8;                         /* 8-position column blocks of the scores */
     constexpr int LK = TP > 32 ? TP / 32 : 1;          /* tile rows whose page a lane looks up */
     constexpr int RW = TP / LK;
-    constexpr int SLOT = slot_bytes<KV, HD, TM>(), VOFF = TP * PITCH, DOFF = 2 * TP * PITCH;
+    constexpr int SLOT = slot_bytes<HD, TM>(), VOFF = TP * PITCH, SCALES = KV == KC_Q8_0 ? 2 * TP : 0;
     constexpr int HC = 8 * MT;
     extern __shared__ __align__(128) unsigned char at_raw[];
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const int r = lane >> 2, c = lane & 3;             /* fragment row (head) and column group */
-    unsigned char *ring = at_raw + (size_t)warp * S * SLOT;
-    int4 *info = (int4 *)(at_raw + AT_WARPS * S * SLOT) + warp * S;   /* what each slot holds */
-    float *comb = (float *)(at_raw + AT_WARPS * S * (SLOT + 16));     /* finish: the warps' sums */
-    float *cml = comb + AT_WARPS * AT_COMB * HD;                      /* and their maxima and weights' sums */
-    const uint32_t ring_s = smem_u32(ring);
+    unsigned char *slots = at_raw + (-smem_u32(at_raw) & 1023u);
+    const uint32_t ring_s = smem_u32(slots) + (uint32_t)(warp * S * SLOT);
+    float *scl = (float *)(slots + AT_WARPS * S * SLOT) + warp * S * SCALES;   /* K's and V's row scales of each slot */
+    int4 *info = (int4 *)(slots + AT_WARPS * S * (SLOT + SCALES * 4)) + warp * S;   /* what each slot holds */
+    float *comb = (float *)(slots + AT_WARPS * S * (SLOT + SCALES * 4 + 16));  /* finish: the warps' sums */
+    float *cml = comb + AT_WARPS * AT_COMB * HD;       /* and their maxima and weights' sums */
     const int U = a.kv.n_kv * a.chunks;                /* units per sequence */
     const int W = a.unit_cost;
 
-    /* ---- this CTA's share: [i chunk, (i + 1) chunk) of the units' times, laid end to end ---- */
-    __shared__ long long s_sum[AT_WARPS];
-    __shared__ long long s_at;
-    __shared__ int s_b, s_len, s_first, s_last;
-    long long lo, hi, chunk;
-    {
-        const int per = (a.n_seqs + AT_THREADS - 1) / AT_THREADS;
-        const int b0 = min(tid * per, a.n_seqs), b1 = min(b0 + per, a.n_seqs);
-        int len = 0, first = 0;                        /* (of the only sequence of a thread, if it has one) */
-        auto unit_time = [&](int b, bool &bad) {
-            len = seq_span(a, b, first, bad);
-            return len > 0 ? (len - first + QP - 1) / QP + W : 0;
-        };
-        long long sum = 0;
-        bool any_bad = false, none = false, far = (long long)a.n_seqs * U > gridDim.x;
-        for (int b = b0; b < b1; b++) {
-            bool bad;
-            const int t = unit_time(b, bad);
-            sum += t;
-            far |= t > AT_SHORT + W;
-            any_bad |= bad;
-            none |= t == 0;
-        }
-        if (any_bad && blockIdx.x == 0) atomicOr(a.err, (unsigned)SE_LEN);
-        long long pre = sum;
-#pragma unroll
-        for (int o = 1; o < 32; o <<= 1) {
-            const long long t = __shfl_up_sync(0xffffffffu, pre, o);
-            if (lane >= o) pre += t;
-        }
-        if (lane == 31) s_sum[warp] = pre;
-        none = __syncthreads_or(none);
-        far = __syncthreads_or(far);
-        long long all = 0;
-        pre -= sum;
-#pragma unroll
-        for (int w = 0; w < AT_WARPS; w++) {
-            if (w < warp) pre += s_sum[w];             /* a unit's worth of the time before b0 */
-            all += s_sum[w];
-        }
-        const long long total = all * U;
-        /* total / CTAs, rounded up; a quotient below 2^42 is at least 2^-11 from the next integer or one itself */
-        if (!far) {
-            /* short sequences, a CTA for each unit: joining would take longer than it saved */
-            const int b = blockIdx.x / U;
-            if (b0 <= b && b < b1) {
-                bool bad;
-                if (per > 1) unit_time(b, bad);
-                s_b = b;
-                s_len = len;
-                s_first = first;
-                s_at = 0;
-            }
-            chunk = 1ll << 40;
-            lo = hi = 0;
-        } else {
-        chunk = (long long)((double)total / (double)gridDim.x);
-        chunk = max(chunk + (chunk * gridDim.x < total), (long long)a.min_share);
-        lo = min(blockIdx.x * chunk, total);
-        hi = min(lo + chunk, total);
-        if (lo < hi && lo >= pre * U && lo < (pre + sum) * U) {
-            long long at = pre;
-            int b = b0;
-            if (per > 1)
-                for (; b < b1; b++) {
-                    bool bad;
-                    const int t = unit_time(b, bad);
-                    if (lo < (at + t) * U) break;
-                    at += t;
-                }
-            s_b = b;
-            s_len = len;
-            s_first = first;
-            s_at = at * U;
-        }
-        }
-        __syncthreads();
-        /* sequences without positions: zeros */
-        if (none)
-            for (int b = blockIdx.x; b < a.n_seqs; b += gridDim.x) {
-                int f;
-                bool bad;
-                if (seq_span(a, b, f, bad) == 0)
-                    for (int i = tid; i < a.n_heads * a.kv.hd; i += AT_THREADS) a.out[b * a.ldo + i] = 0.0f;
-            }
-        if (!far) {
-            if (blockIdx.x >= a.n_seqs * U || s_len == 0) return;
-            const int t = (s_len - s_first + QP - 1) / QP + W;
-            lo = (long long)(blockIdx.x % U) * t;
-            hi = lo + t;
-        }
-        if (lo >= hi) return;
-    }
-
-    /* ---- the loader's place: sequence, unit of it, quantum of that ---- */
-    int lb = s_b, first = s_first, len = s_len, lu, lq;
-    int nq = (len - first + QP - 1) / QP;
-    long long ubase;                                   /* where the loader's unit begins */
+    /* ---- this CTA's share: [i chunk, (i + 1) chunk) of the units' times, laid end to end; every warp
+     * finds it by itself, a run of sequences a lane ---- */
+    int lb, first, len, lu, lq, nq;                    /* the loader's place: sequence, unit of it, quantum of that */
+    long long ubase, chunk;                            /* where the loader's unit begins */
     int left;                                          /* time to the share's end */
     bool bad_;
     {
-        const long long rel = lo - s_at;
-        lu = rel >> 31 ? (int)(rel / (nq + W)) : (int)((unsigned)rel / (unsigned)(nq + W));
-        const int off = (int)(rel - (long long)lu * (nq + W));
-        lq = max(0, off - W);
-        ubase = lo - off;
-        left = (int)min(hi - ubase, 1ll << 30) - W - lq;
+        const int per = (a.n_seqs + 31) / 32, b0 = min(lane * per, a.n_seqs), b1 = min(b0 + per, a.n_seqs);
+        int sum = 0;                                   /* a unit's worth of the run's time (fewer than 2^31 in all) */
+        bool none = false, far = (long long)a.n_seqs * U > gridDim.x, any_bad = false;
+        for (int b = b0; b < b1; b++) {
+            len = seq_span(a, b, first, bad_);
+            const int t = len > 0 ? (len - first + QP - 1) / QP + W : 0;
+            sum += t;
+            none |= t == 0;
+            far |= t > AT_SHORT + W;
+            any_bad |= bad_;
+        }
+        if (any_bad && blockIdx.x == 0) atomicOr(a.err, (unsigned)SE_LEN);
+        int pre = sum;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const int t = __shfl_up_sync(0xffffffffu, pre, o);
+            if (lane >= o) pre += t;
+        }
+        const int all = __shfl_sync(0xffffffffu, pre, 31);
+        pre -= sum;
+        /* sequences without positions: zeros */
+        if (__any_sync(0xffffffffu, none))
+            for (int b = blockIdx.x; b < a.n_seqs; b += gridDim.x)
+                if (seq_span(a, b, first, bad_) == 0)
+                    for (int i = tid; i < a.n_heads * a.kv.hd; i += AT_THREADS) a.out[b * a.ldo + i] = 0.0f;
+        if (!__any_sync(0xffffffffu, far)) {
+            /* short sequences, a CTA for each unit: joining would take longer than it saved */
+            lb = blockIdx.x / U;
+            lu = blockIdx.x % U;
+            if (lb >= a.n_seqs) return;
+            len = seq_span(a, lb, first, bad_);
+            nq = (len - first + QP - 1) / QP;
+            lq = 0;
+            left = nq;
+            ubase = 0;
+            chunk = 1ll << 40;
+        } else {
+            const long long total = (long long)all * U;
+            /* total / CTAs rounded up: grid_inv is 2^64 / CTAs rounded up, so the product's high half is the
+             * quotient or one more */
+            long long q = (long long)__umul64hi((unsigned long long)total, a.grid_inv);
+            q -= q * gridDim.x > total;
+            chunk = q + (q * gridDim.x < total);
+            const long long lo = blockIdx.x * chunk, hi = min(lo + chunk, total);
+            if (lo >= hi) return;
+            /* the lane whose run holds lo, and the sequence in it */
+            const unsigned at = __ballot_sync(0xffffffffu, lo >= (long long)pre * U && lo < ((long long)pre + sum) * U);
+            const int own = __ffs(at) - 1;
+            int b = __shfl_sync(0xffffffffu, b0, own), p = __shfl_sync(0xffffffffu, pre, own);
+            for (;; b++) {
+                len = seq_span(a, b, first, bad_);
+                nq = (len - first + QP - 1) / QP;
+                const int t = nq > 0 ? nq + W : 0;
+                if (lo < ((long long)p + t) * U || b + 1 >= a.n_seqs) break;
+                p += t;
+            }
+            lb = b;
+            const long long rel = lo - (long long)p * U;
+            lu = rel >> 31 ? (int)(rel / (nq + W)) : (int)((unsigned)rel / (unsigned)(nq + W));
+            const int off = (int)(rel - (long long)lu * (nq + W));
+            lq = max(0, off - W);
+            ubase = lo - off;
+            left = (int)min(hi - ubase, 1ll << 30) - W - lq;
+        }
+        if (left <= 0) return;                         /* (the same for the CTA's warps) */
     }
-    if (left <= 0) return;
     const int b0_ = lb, u0_ = lu;
     const bool whole0 = lq == 0;                       /* the first unit begins in this share */
     const int nq0 = nq;
@@ -643,54 +610,61 @@ __global__ void __launch_bounds__(AT_THREADS, OCC) paged_attend_kernel(const __g
         }
     };
     enum { LAST_OF_UNIT = 1 << 28, LAST_OF_SHARE = 1 << 29 };
+    unsigned live[LK], row[LK];                        /* of the loader's tile: rows that are there, and where */
+    bool full;                                         /* all of them, and as long as the slot's */
+    /* Rows start at different bank groups, by an exclusive or of the 16-byte chunk's number with swz(row): for
+     * row-per-lane reads of eight rows (ldmatrix, and f32 V) the row's low bits, or the next ones where two rows
+     * share 128 bytes; for f32 K, read by four lanes a row and eight rows in turn, the low bits reversed. */
+    constexpr int SWV = CPR >= 8 ? 0 : 1, SWK = KV == KC_F32 ? 2 : SWV;
+    auto swz = [](int sw, int t) { return sw == 0 ? (t & 7) : (sw == 1 ? ((t >> 1) & 3) : (((t & 1) << 2) | ((t >> 1) & 3))); };
+    /* a lane's chunk of the warp's e-th 512 bytes: row te + tl, te a constant of e whose bits tl has not */
+    const int tl = CPR < 32 ? lane / CPR : 0, cl = lane % (CPR < 32 ? CPR : 32);
+    auto copy_rows = [&](uint32_t dst, const uint8_t *src, const int sw) {
+        const unsigned rowb = (unsigned)a.kv.hd * ES;
+        const uint32_t to = dst + tl * PITCH + ((cl ^ swz(sw, tl)) << 4);
+        constexpr int RE = CPR < 32 ? 32 / CPR : 1, WE = CPR > 32 ? CPR / 32 : 1;   /* rows per 512 bytes, or the other way round */
+        if (full) {
+#pragma unroll
+            for (int e = 0; e < TP * CPR / 32; e++) {
+                const int te = e / WE * RE, ce = 32 * (e % WE);
+                const unsigned rr = __shfl_sync(0xffffffffu, row[te / RW], (te + tl) & (RW - 1));
+                cp_async16s((to ^ (uint32_t)(swz(sw, te) << 4)) + te * PITCH + ce * 16, src + ((size_t)rr * PITCH + (cl + ce) * 16));
+            }
+        } else {
+#pragma unroll 1
+            for (int e = 0; e < TP * CPR / 32; e++) {
+                const int te = e / WE * RE, ce = 32 * (e % WE), t = (te + tl) & (RW - 1), k = te / RW;
+                const unsigned rr = __shfl_sync(0xffffffffu, k ? row[LK - 1] : row[0], t);
+                const bool lv = (((k ? live[LK - 1] : live[0]) >> t) & 1u) && (cl + ce) * 16 < (int)rowb;
+                cp_async16z((to ^ (uint32_t)(swz(sw, te) << 4)) + te * PITCH + ce * 16,
+                            src + ((size_t)rr * rowb + (lv ? (cl + ce) * 16 : 0)), lv);
+            }
+        }
+    };
+    auto copy_scales = [&](float *dst, const float *src) {
+#pragma unroll
+        for (int k = 0; k < LK; k++) cp_async4z(smem_u32(dst + k * 32 + lane), src + row[k], (live[k] >> lane) & 1u);
+    };
     int issued = 0;
     auto issue = [&](int stage) {
         const int g = lu / a.chunks;
         issued++;
-        unsigned live[LK], row[LK];
-        const uint32_t sk = ring_s + stage * SLOT;
+        full = a.kv.hd == HD;
 #pragma unroll
         for (int k = 0; k < LK; k++) {
             const bool ok = pin[k] && pg[k] >= 0 && pg[k] < a.kv.n_pages;
             if (pin[k] && !ok) atomicOr(a.err, (unsigned)SE_PAGE);
             live[k] = __ballot_sync(0xffffffffu, ok) & (unsigned)((1ull << RW) - 1);
+            full &= live[k] == (unsigned)((1ull << RW) - 1);
             row[k] = ok ? (unsigned)(((size_t)pg[k] * a.kv.n_kv + g) * a.kv.page + pslot[k]) : 0u;
-            if constexpr (KV == KC_Q8_0) {
-                cp_async4z(sk + DOFF + (k * 32 + lane) * 4, a.kv.kd + row[k], ok);
-                cp_async4z(sk + DOFF + (TP + k * 32 + lane) * 4, a.kv.vd + row[k], ok);
-            }
         }
-        const unsigned rowb = (unsigned)a.kv.hd * ES;
-        bool full = rowb == PITCH;                     /* every row of the tile is there, and as long as the slot's */
-#pragma unroll
-        for (int k = 0; k < LK; k++) full &= live[k] == (unsigned)((1ull << RW) - 1);
-        auto rows = [&](auto all) {
-#pragma unroll
-            for (int e = 0; e < TP * CPR / 32; e++) {
-                const int idx = lane + 32 * e, t = idx / CPR, ch = idx % CPR, k = (32 * e / CPR) / RW;
-                const unsigned rr = __shfl_sync(0xffffffffu, row[k], t & (RW - 1));
-                int kx, vx;                            /* swizzles: which of 8 bank groups a row starts at */
-                if constexpr (KV == KC_F32) {
-                    kx = ((t & 1) << 2) | ((t >> 1) & 3);
-                    vx = t & 7;
-                } else {
-                    kx = vx = CPR >= 8 ? (t & 7) : ((t >> 1) & 3);
-                }
-                const uint32_t dk = sk + t * PITCH + ((ch ^ kx) << 4), dv = sk + VOFF + t * PITCH + ((ch ^ vx) << 4);
-                if constexpr (decltype(all)::value) {
-                    const size_t off = (size_t)rr * PITCH + ch * 16;
-                    cp_async16s(dk, a.kv.k + off);
-                    cp_async16s(dv, a.kv.v + off);
-                } else {
-                    const bool lv = ((live[k] >> (t & (RW - 1))) & 1u) && ch * 16 < (int)rowb;
-                    const size_t off = (size_t)rr * rowb + (lv ? ch * 16 : 0);
-                    cp_async16z(dk, a.kv.k + off, lv);
-                    cp_async16z(dv, a.kv.v + off, lv);
-                }
-            }
-        };
-        if (full) rows(std::true_type{});
-        else rows(std::false_type{});
+        const uint32_t sk = ring_s + stage * SLOT;
+        copy_rows(sk, a.kv.k, SWK);
+        copy_rows(sk + VOFF, a.kv.v, SWV);
+        if constexpr (KV == KC_Q8_0) {
+            copy_scales(scl + stage * SCALES, a.kv.kd);
+            copy_scales(scl + stage * SCALES + TP, a.kv.vd);
+        }
         if (lane == 0) {
             const bool eu = lq == nq - 1;
             const int f = (eu ? LAST_OF_UNIT : 0) | (left <= (eu ? 1 + W : 1) ? LAST_OF_SHARE : 0);
@@ -752,15 +726,6 @@ __global__ void __launch_bounds__(AT_THREADS, OCC) paged_attend_kernel(const __g
     };
     fetch_q(lb, lu);
     look();
-#pragma unroll
-    for (int s = 0; s < S - 1; s++) {
-        if (left > 0) {
-            issue(s);
-            advance();
-        }
-        cp_async_commit();
-    }
-    __syncwarp();
 
     /* ---- the compute side ---- */
     constexpr int QR = KV == KC_F32 ? HD / 8 * 4 : (KV == KC_F16 ? HD / 16 * 4 : HD / 32 * 2);
@@ -805,13 +770,12 @@ __global__ void __launch_bounds__(AT_THREADS, OCC) paged_attend_kernel(const __g
                     const float id = tiny ? 0.0f : __fdiv_rn(127.0f, mx), qd = tiny ? 0.0f : __fdiv_rn(mx, 127.0f);
 #pragma unroll
                     for (int j = 0; j < HD / 16; j++) {
-                        unsigned w = 0;
+                        /* x 127 / max rounded half away from zero: at most 127.5 and a rounding, never 128 */
+                        int q[4];
 #pragma unroll
-                        for (int i = 0; i < 4; i++) {
-                            const float u = truncf(__fadd_rn(__fmul_rn(x[4 * j + i], id), copysignf(0.5f, x[4 * j + i])));
-                            const int qi = tiny ? 0 : (int)fminf(fmaxf(u, -127.0f), 127.0f);
-                            w |= ((unsigned)qi & 0xffu) << (8 * i);
-                        }
+                        for (int i = 0; i < 4; i++)
+                            q[i] = __float2int_rz(__fadd_rn(__fmul_rn(x[4 * j + i], id), copysignf(0.5f, x[4 * j + i])));
+                        const unsigned w = __byte_perm(__byte_perm(q[0], q[1], 0x0040), __byte_perm(q[2], q[3], 0x0040), 0x5410);
                         qf[mt][j] = w;
                     }
                     qc[mt] = __fmul_rn(qd, a.scale) * post;
@@ -820,20 +784,19 @@ __global__ void __launch_bounds__(AT_THREADS, OCC) paged_attend_kernel(const __g
         }
     };
 
-    /* one tile of TP positions in ring slot `stage` */
-    auto compute = [&](int stage, const unsigned (&live)[LK]) {
-        const uint32_t sk = ring_s + stage * SLOT, sv = sk + VOFF;
-        float s[MT][NT][2];
+    /* the scores of the tile of TP positions in ring slot `stage`: of head row r, positions 8 nt + 2 c and + 1 */
+    float s[MT][NT][2];
+    auto scores = [&](int stage) {
+        const uint32_t sk = ring_s + stage * SLOT;
         if constexpr (KV == KC_F16) {
             float d[MT][NT][4];
-            const uint32_t kb = sk + (lane & 7) * PITCH;
-            const int x = (lane >> 3) ^ (lane & 7);
+            const uint32_t kb = sk + (lane & 7) * PITCH + (((lane >> 3) ^ (lane & 7)) << 4);
 #pragma unroll
             for (int jj = 0; jj < HD / 32; jj++)
 #pragma unroll
                 for (int nt = 0; nt < NT; nt++) {
                     unsigned b[4];
-                    ldsm4(b, kb + nt * 8 * PITCH + (((4 * jj) ^ x) << 4));
+                    ldsm4(b, (kb ^ (64 * jj)) + nt * 8 * PITCH);
 #pragma unroll
                     for (int mt = 0; mt < MT; mt++) {
                         const unsigned a0[4] = { qf[mt][8 * jj], qf[mt][8 * jj + 1], qf[mt][8 * jj + 2], qf[mt][8 * jj + 3] };
@@ -852,13 +815,12 @@ __global__ void __launch_bounds__(AT_THREADS, OCC) paged_attend_kernel(const __g
                 }
         } else if constexpr (KV == KC_F32) {
             float dh[MT][NT][4], dl[MT][NT][4];
-            const uint32_t kb = sk + r * PITCH;
-            const int x = c ^ (((r & 1) << 2) | (r >> 1));
+            const uint32_t kb = sk + r * PITCH + ((c ^ swz(SWK, r)) << 4);
 #pragma unroll
             for (int jj = 0; jj < HD / 16; jj++)
 #pragma unroll
                 for (int nt = 0; nt < NT; nt++) {
-                    const float4 t = lds4(kb + nt * 8 * PITCH + (((4 * jj) ^ x) << 4));
+                    const float4 t = lds4((kb ^ (64 * jj)) + nt * 8 * PITCH);
                     unsigned h[4], w[4];
                     split_tf32(t.x, h[0], w[0]);
                     split_tf32(t.y, h[1], w[1]);
@@ -894,21 +856,20 @@ __global__ void __launch_bounds__(AT_THREADS, OCC) paged_attend_kernel(const __g
                 for (int nt = 0; nt < NT; nt++)
 #pragma unroll
                     for (int i = 0; i < 4; i++) d[mt][nt][i] = 0x4b400000;   /* 1.5 * 2^23: the sums come out as its floats */
-            const uint32_t kb = sk + (lane & 7) * PITCH;
-            const int x = (lane >> 3) ^ (CPR >= 8 ? (lane & 7) : ((lane >> 1) & 3));
+            const uint32_t kb = sk + (lane & 7) * PITCH + (((lane >> 3) ^ swz(SWK, lane & 7)) << 4);
 #pragma unroll
             for (int jj = 0; jj < HD / 64; jj++)
 #pragma unroll
                 for (int nt = 0; nt < NT; nt++) {
                     unsigned b[4];
-                    ldsm4(b, kb + nt * 8 * PITCH + (((4 * jj) ^ x) << 4));
+                    ldsm4(b, (kb ^ (64 * jj)) + nt * 8 * PITCH);
 #pragma unroll
                     for (int mt = 0; mt < MT; mt++) {
                         mma_s8(d[mt][nt], qf[mt][4 * jj], qf[mt][4 * jj + 1], b[0], b[1]);
                         mma_s8(d[mt][nt], qf[mt][4 * jj + 2], qf[mt][4 * jj + 3], b[2], b[3]);
                     }
                 }
-            const float *kd = (const float *)(ring + stage * SLOT + DOFF);
+            const float *kd = scl + stage * SCALES;
 #pragma unroll
             for (int nt = 0; nt < NT; nt++) {
                 const float2 e = *(const float2 *)(kd + nt * 8 + 2 * c);
@@ -919,9 +880,11 @@ __global__ void __launch_bounds__(AT_THREADS, OCC) paged_attend_kernel(const __g
                 }
             }
         }
-        /* soft-cap, mask, running softmax in base 2 */
+    };
+    /* soft-cap, mask, running softmax in base 2: the scores become weights */
+    float2 corr[MT];                                   /* what the sums so far are scaled by */
+    auto soften = [&](const unsigned (&live)[LK]) {
         constexpr float LIFT = KV == KC_F32 ? 0.0f : 15.0f;   /* weights in (0, 2^15]: small ones stay normal f16 */
-        float2 corr[MT];
         bool all = true;
 #pragma unroll
         for (int k = 0; k < LK; k++) all &= live[k] == (unsigned)((1ull << RW) - 1);
@@ -961,7 +924,10 @@ __global__ void __launch_bounds__(AT_THREADS, OCC) paged_attend_kernel(const __g
                 }
             l[mt] = l[mt] * cr + sum;
         }
-        /* the weighted sum of V's rows */
+    };
+    /* the weighted sum of V's rows */
+    auto weigh = [&](int stage) {
+        const uint32_t sv = ring_s + stage * SLOT + VOFF;
         if constexpr (KV == KC_F16) {
             constexpr int KS = TP / 16;
             unsigned w[MT][KS][4];
@@ -970,15 +936,14 @@ __global__ void __launch_bounds__(AT_THREADS, OCC) paged_attend_kernel(const __g
 #pragma unroll
                 for (int nt = 0; nt < NT; nt++)
                     split_f16(s[mt][nt][0], s[mt][nt][1], w[mt][nt >> 1][2 * (nt & 1)], w[mt][nt >> 1][2 * (nt & 1) + 1]);
-            const uint32_t vb = sv + ((lane & 7) + (lane & 8)) * PITCH;
-            const int x = (lane >> 4) ^ (lane & 7);
+            const uint32_t vb = sv + (lane & 15) * PITCH + (((lane >> 4) ^ (lane & 7)) << 4);
 #pragma unroll
             for (int jj = 0; jj < HD / 16; jj++) {
                 float d[MT][2][4];
 #pragma unroll
                 for (int ks = 0; ks < KS; ks++) {
                     unsigned b[4];
-                    ldsm4t(b, vb + ks * 16 * PITCH + (((2 * jj) ^ x) << 4));
+                    ldsm4t(b, (vb ^ (32 * jj)) + ks * 16 * PITCH);
 #pragma unroll
                     for (int mt = 0; mt < MT; mt++) {
                         if (ks == 0) {
@@ -1005,15 +970,14 @@ __global__ void __launch_bounds__(AT_THREADS, OCC) paged_attend_kernel(const __g
                     split_tf32(s[mt][nt][0], w[mt][nt][0], w[mt][nt][1]);
                     split_tf32(s[mt][nt][1], w[mt][nt][2], w[mt][nt][3]);
                 }
-            const uint32_t v0 = sv + (2 * c) * PITCH, v1 = v0 + PITCH;
-            const int x0 = r ^ (2 * c), x1 = r ^ (2 * c + 1);
+            const uint32_t v0 = sv + (2 * c) * PITCH + ((r ^ (2 * c)) << 4), v1 = sv + (2 * c + 1) * PITCH + ((r ^ (2 * c + 1)) << 4);
 #pragma unroll
             for (int j = 0; j < HD / 32; j++) {
                 float d[MT][4][4];
 #pragma unroll
                 for (int nt = 0; nt < NT; nt++) {
-                    const float4 ya = lds4(v0 + nt * 8 * PITCH + (((8 * j) ^ x0) << 4));
-                    const float4 yb = lds4(v1 + nt * 8 * PITCH + (((8 * j) ^ x1) << 4));
+                    const float4 ya = lds4((v0 ^ (128 * j)) + nt * 8 * PITCH);
+                    const float4 yb = lds4((v1 ^ (128 * j)) + nt * 8 * PITCH);
                     const float y0[4] = { ya.x, ya.y, ya.z, ya.w }, y1[4] = { yb.x, yb.y, yb.z, yb.w };
 #pragma unroll
                     for (int i = 0; i < 4; i++) {
@@ -1036,7 +1000,7 @@ __global__ void __launch_bounds__(AT_THREADS, OCC) paged_attend_kernel(const __g
         } else {
             /* the rows' scales join the weights; a power of two keeps the product in f16's range */
             constexpr int KS = TP / 16;
-            const float *vd = (const float *)(ring + stage * SLOT + DOFF) + TP;
+            const float *vd = scl + stage * SCALES + TP;
             float top = fabsf(vd[lane]);
 #pragma unroll
             for (int k = 1; k < LK; k++) top = fmaxf(top, fabsf(vd[k * 32 + lane]));
@@ -1053,8 +1017,7 @@ __global__ void __launch_bounds__(AT_THREADS, OCC) paged_attend_kernel(const __g
                     split_f16(s[mt][nt][0] * (e.x * dn), s[mt][nt][1] * (e.y * dn), w[mt][nt >> 1][2 * (nt & 1)],
                               w[mt][nt >> 1][2 * (nt & 1) + 1]);
             }
-            const uint32_t vb = sv + ((lane & 7) + (lane & 8)) * PITCH;
-            const int x = (lane >> 4) ^ (CPR >= 8 ? (lane & 7) : ((lane >> 1) & 3));
+            const uint32_t vb = sv + (lane & 15) * PITCH + (((lane >> 4) ^ swz(SWV, lane & 7)) << 4);
             const __half2 bias = __half2half2(__ushort_as_half(0x6480));   /* 1152 */
             auto bytes = [&](unsigned u, unsigned &even, unsigned &odd) {
                 /* signed bytes of two rows -> f16: 0x6400 | (v + 128) is 1024 + 128 + v */
@@ -1069,7 +1032,7 @@ __global__ void __launch_bounds__(AT_THREADS, OCC) paged_attend_kernel(const __g
 #pragma unroll
                 for (int ks = 0; ks < KS; ks++) {
                     unsigned b[4];
-                    ldsm4t(b, vb + ks * 16 * PITCH + (((2 * jj) ^ x) << 4));
+                    ldsm4t(b, (vb ^ (32 * jj)) + ks * 16 * PITCH);
                     unsigned e0, o0, e1, o1;
                     bytes(b[0], e0, o0);
                     bytes(b[1], e1, o1);
@@ -1186,23 +1149,24 @@ __global__ void __launch_bounds__(AT_THREADS, OCC) paged_attend_kernel(const __g
         }
     };
 
-    __shared__ int s_c0, s_c1;
-    auto leave = [&](int b, int u) {                   /* the unit's piece is written: join them if it was the last */
-        if (tid == 0) {
-            __threadfence();                           /* finish's barrier is behind every thread's part of it */
-            /* a unit that is not fresh is the share's first, one that is left unfinished its last */
-            const long long x = (fresh ? ubase : ubase0) + W;
-            const int c0 = (int)(x / chunk), c1 = (int)((x + (fresh ? nq : nq0) - 1) / chunk);
-            const unsigned n = atomicAdd(a.count + c1, 1u);
-            s_last = n == (unsigned)(c1 - c0);
-            if (s_last) a.count[c1] = 0u;
-            s_c0 = c0;
-            s_c1 = c1;
-            __threadfence();
-        }
-        __syncthreads();
-        if (s_last) join_pieces<HD, MT>(a, b, u, s_c0, s_c1, comb);
-        if (s_last) __syncthreads();                   /* (comb is the next unit's) */
+    /* a piece is written: was it the unit's last missing one? (A unit that is not fresh is the share's first,
+     * one that is left unfinished its last: at most two, and they are joined after the loop, which keeps the
+     * loop's registers out of a call.) */
+    __shared__ int s_join[2][4];
+    if (tid < 2) s_join[tid][0] = 0;
+    auto leave = [&](int b, int u) {
+        if (tid != 0) return;
+        __threadfence();                               /* finish's barrier is behind every thread's part of the piece */
+        const long long x = (fresh ? ubase : ubase0) + W;
+        const int c0 = (int)(x / chunk), c1 = (int)((x + (fresh ? nq : nq0) - 1) / chunk);
+        const unsigned n = atomicAdd(a.count + c1, 1u);
+        int *j = s_join[fresh];
+        j[0] = n == (unsigned)(c1 - c0) ? c1 + 1 : 0;
+        j[1] = c0;
+        j[2] = b;
+        j[3] = u;
+        if (j[0]) a.count[c1] = 0u;
+        __threadfence();
     };
 
     auto begin = [&]() {
@@ -1216,9 +1180,10 @@ __global__ void __launch_bounds__(AT_THREADS, OCC) paged_attend_kernel(const __g
         }
     };
     begin();
-    for (int it = 0; it < issued; it++) {
-        const int stage = it % S;
-        const int4 f = info[stage];                    /* written when the slot's copies were issued */
+    /* the first S passes only load */
+    for (int it = -S, stage = 0; it < issued; it++, stage = stage + 1 == S ? 0 : stage + 1) {
+        int4 f = make_int4(cu_b, cu_u, 0, 0);
+        if (it >= 0) f = info[stage];                  /* written when the slot's copies were issued */
         const int fu = f.y & (LAST_OF_UNIT - 1);
         if (f.x != cu_b || fu != cu_u) {
             /* a new unit: its queries are on their way while the tile arrives */
@@ -1228,23 +1193,35 @@ __global__ void __launch_bounds__(AT_THREADS, OCC) paged_attend_kernel(const __g
             fetch_q(cu_b, cu_u);
             begin();
         }
-        cp_async_wait_but<S - 2>();
+        const bool on = f.z | f.w;
+        cp_async_wait_but<S - 1>();
+        __syncwarp();
+        if (on) {
+            scores(stage);
+            unsigned here[LK];
+            here[0] = (unsigned)f.z;
+            if constexpr (LK > 1) here[1] = (unsigned)f.w;
+            soften(here);
+            weigh(stage);
+        }
         __syncwarp();
         if (left > 0) {
-            issue((it + S - 1) % S);
+            issue(stage);
             advance();
         }
         cp_async_commit();
-        unsigned live[LK];
-        live[0] = (unsigned)f.z;
-        if constexpr (LK > 1) live[1] = (unsigned)f.w;
-        if (f.z | f.w) compute(stage, live);
         if (f.y & (LAST_OF_UNIT | LAST_OF_SHARE)) {
             const bool complete = fresh && (f.y & LAST_OF_UNIT);
             finish(cu_b, cu_u, complete);
             if (!complete) leave(cu_b, cu_u);
         }
     }
+    __syncthreads();
+    for (int k = 0; k < 2; k++)
+        if (s_join[k][0]) {
+            join_pieces<HD, MT>(a, s_join[k][2], s_join[k][3], s_join[k][1], s_join[k][0] - 1, comb);
+            __syncthreads();                           /* (comb is the second's) */
+        }
 }
 
 }  // namespace kc

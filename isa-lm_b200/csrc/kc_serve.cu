@@ -155,6 +155,9 @@ static void launch_append(const AppendArgs &a, cudaStream_t st) {
 
 /* ------------------------------------------------------------ attention */
 
+/* A unit's own time beside its tiles', in quanta (queries, the warps' meeting, the output). */
+constexpr int AT_UNIT_COST = 2;
+
 /* The workspace: a counter for each CTA of any instance, zero between calls, and the pieces. */
 constexpr int AT_MAX_CTAS = 2048;
 
@@ -175,13 +178,21 @@ static AttendVariant make_variant() {
     return v;
 }
 
+/* The instance for a cache and group: a template of positions per tile, heads
+ * per chunk, ring slots and CTAs an SM. Two slots a warp are enough; what pays
+ * is a third CTA (12 warps an SM instead of 8) where the arithmetic, not the
+ * copies, fills a tile's time: narrow heads, f32 (both halves of every value are
+ * split) and so on. Where a tile is little more than its copies (f16, and 8-bit
+ * of head 128), more copies under way only slow the memory down: 64 sequences of
+ * 2048..8192 positions, f16, head 128: 206 us with 8 warps, 219 us with 12; 32 of
+ * 2048, f32, head 64: 57.7 and 53.4 us; 64 of 4096, 8-bit, head 64: 76 and 65 us. */
 template <int KV>
 static AttendVariant *variants_of(int hd, int group, int &mt) {
-    static AttendVariant v64 = make_variant<KV, 64, 2, 1, 3, 2>(), v128 = make_variant<KV, 128, 1, 1, 3, 2>(),
-                         v256 = make_variant<KV, 256, 1, 1, 3, 1>();
+    static AttendVariant v64 = make_variant<KV, 64, 2, 1, 2, 3>(), v128 = make_variant<KV, 128, 1, 1, 2, KV == KC_F32 ? 3 : 2>(),
+                         v256 = make_variant<KV, 256, 1, 1, 2, 1>();
     if constexpr (KV != KC_F32) {
         /* more than 8 heads share a KV head: 16 at a time, so that the cache is read once */
-        static AttendVariant w64 = make_variant<KV, 64, 2, 2, 3, 2>(), w128 = make_variant<KV, 128, 1, 2, 3, 2>();
+        static AttendVariant w64 = make_variant<KV, 64, 2, 2, 2, 2>(), w128 = make_variant<KV, 128, 1, 2, 2, 2>();
         if (group > 8 && hd <= 128) {
             mt = 2;
             return hd <= 64 ? &w64 : &w128;
@@ -319,6 +330,8 @@ extern "C" int kc_paged_attend_dev(const kc_paged_kv *kv, const kc_attend_args *
     rc = attend_variant(kv, x->n_heads, d, v, a.chunks);
     if (rc != KC_OK) return rc;
     const int ctas = v->ctas[d.dev];
+    if ((double)x->n_seqs * ((double)kv->ld_table * kv->page_size / (AT_WARPS * v->tile) + 2 + AT_UNIT_COST) >= 2147483648.0)
+        return refuse("n_seqs sequences of ld_table * page_size positions are too many for one call");
     if (x->ws_bytes < ws_bytes(v, ctas))
         return refuse("workspace of " + std::to_string(x->ws_bytes) + " bytes, " + std::to_string(ws_bytes(v, ctas)) +
                       " needed (kc_paged_attend_ws)");
@@ -333,8 +346,8 @@ extern "C" int kc_paged_attend_dev(const kc_paged_kv *kv, const kc_attend_args *
     a.window = x->window; a.scale = x->scale; a.softcap = x->softcap;
     a.inv_softcap = x->softcap > 0.0f ? 1.0f / x->softcap : 0.0f;
     a.near = (v->tile - 1) / kv->page_size + 2 <= 32;
-    a.unit_cost = 2;
-    a.min_share = 1;
+    a.unit_cost = AT_UNIT_COST;
+    a.grid_inv = ~0ull / (unsigned)ctas + 1;
     a.count = (unsigned *)x->ws;
     a.part = (float *)((char *)x->ws + sizeof(unsigned) * AT_MAX_CTAS);
     a.err = d.err;
