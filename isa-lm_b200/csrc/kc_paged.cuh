@@ -325,6 +325,11 @@ __device__ __forceinline__ void mma_tf32(float (&c)[4], const unsigned (&a)[4], 
                  : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
                  : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
+/* the same from four times `init`; rows 8-15 of A are zero */
+__device__ __forceinline__ void mma_s8_first(int (&c)[4], unsigned a0, unsigned a2, unsigned b0, unsigned b1, int init) {
+    asm("mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 {%0, %1, %2, %3}, {%4, %5, %6, %5}, {%7, %8}, {%9, %9, %9, %9};"
+        : "=r"(c[0]), "=r"(c[1]), "=r"(c[2]), "=r"(c[3]) : "r"(a0), "r"(0), "r"(a2), "r"(b0), "r"(b1), "r"(init));
+}
 /* rows 8-15 of A are zero */
 __device__ __forceinline__ void mma_s8(int (&c)[4], unsigned a0, unsigned a2, unsigned b0, unsigned b1) {
     asm("mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 {%0, %1, %2, %3}, {%4, %5, %6, %5}, {%7, %8}, {%0, %1, %2, %3};"
@@ -619,25 +624,28 @@ __global__ void __launch_bounds__(AT_THREADS, OCC) paged_attend_kernel(const __g
     auto swz = [](int sw, int t) { return sw == 0 ? (t & 7) : (sw == 1 ? ((t >> 1) & 3) : (((t & 1) << 2) | ((t >> 1) & 3))); };
     /* a lane's chunk of the warp's e-th 512 bytes: row te + tl, te a constant of e whose bits tl has not */
     const int tl = CPR < 32 ? lane / CPR : 0, cl = lane % (CPR < 32 ? CPR : 32);
-    auto copy_rows = [&](uint32_t dst, const uint8_t *src, const int sw) {
-        const unsigned rowb = (unsigned)a.kv.hd * ES;
-        const uint32_t to = dst + tl * PITCH + ((cl ^ swz(sw, tl)) << 4);
+    auto copy_rows = [&](uint32_t sk) {
         constexpr int RE = CPR < 32 ? 32 / CPR : 1, WE = CPR > 32 ? CPR / 32 : 1;   /* rows per 512 bytes, or the other way round */
+        const uint32_t tk = sk + tl * PITCH + ((cl ^ swz(SWK, tl)) << 4), tv = sk + VOFF + tl * PITCH + ((cl ^ swz(SWV, tl)) << 4);
         if (full) {
+            const uint8_t *ks = a.kv.k + cl * 16, *vs = a.kv.v + cl * 16;
 #pragma unroll
             for (int e = 0; e < TP * CPR / 32; e++) {
-                const int te = e / WE * RE, ce = 32 * (e % WE);
-                const unsigned rr = __shfl_sync(0xffffffffu, row[te / RW], (te + tl) & (RW - 1));
-                cp_async16s((to ^ (uint32_t)(swz(sw, te) << 4)) + te * PITCH + ce * 16, src + ((size_t)rr * PITCH + (cl + ce) * 16));
+                const int te = e / WE * RE, ce = 32 * (e % WE), to = te * PITCH + ce * 16;
+                const size_t off = (size_t)__shfl_sync(0xffffffffu, row[te / RW], (te + tl) & (RW - 1)) * PITCH;
+                cp_async16s((tk ^ (uint32_t)(swz(SWK, te) << 4)) + to, ks + off + ce * 16);
+                cp_async16s((tv ^ (uint32_t)(swz(SWV, te) << 4)) + to, vs + off + ce * 16);
             }
         } else {
+            const unsigned rowb = (unsigned)a.kv.hd * ES;
 #pragma unroll 1
             for (int e = 0; e < TP * CPR / 32; e++) {
-                const int te = e / WE * RE, ce = 32 * (e % WE), t = (te + tl) & (RW - 1), k = te / RW;
+                const int te = e / WE * RE, ce = 32 * (e % WE), t = (te + tl) & (RW - 1), k = te / RW, to = te * PITCH + ce * 16;
                 const unsigned rr = __shfl_sync(0xffffffffu, k ? row[LK - 1] : row[0], t);
                 const bool lv = (((k ? live[LK - 1] : live[0]) >> t) & 1u) && (cl + ce) * 16 < (int)rowb;
-                cp_async16z((to ^ (uint32_t)(swz(sw, te) << 4)) + te * PITCH + ce * 16,
-                            src + ((size_t)rr * rowb + (lv ? (cl + ce) * 16 : 0)), lv);
+                const size_t off = (size_t)rr * rowb + (lv ? (cl + ce) * 16 : 0);
+                cp_async16z((tk ^ (uint32_t)(swz(SWK, te) << 4)) + to, a.kv.k + off, lv);
+                cp_async16z((tv ^ (uint32_t)(swz(SWV, te) << 4)) + to, a.kv.v + off, lv);
             }
         }
     };
@@ -658,9 +666,7 @@ __global__ void __launch_bounds__(AT_THREADS, OCC) paged_attend_kernel(const __g
             full &= live[k] == (unsigned)((1ull << RW) - 1);
             row[k] = ok ? (unsigned)(((size_t)pg[k] * a.kv.n_kv + g) * a.kv.page + pslot[k]) : 0u;
         }
-        const uint32_t sk = ring_s + stage * SLOT;
-        copy_rows(sk, a.kv.k, SWK);
-        copy_rows(sk + VOFF, a.kv.v, SWV);
+        copy_rows(ring_s + stage * SLOT);
         if constexpr (KV == KC_Q8_0) {
             copy_scales(scl + stage * SCALES, a.kv.kd);
             copy_scales(scl + stage * SCALES + TP, a.kv.vd);
@@ -740,14 +746,17 @@ __global__ void __launch_bounds__(AT_THREADS, OCC) paged_attend_kernel(const __g
 
     /* the fragments of the query rows in xq */
     auto set_q = [&]() {
-        const float post = a.softcap > 0.0f ? a.inv_softcap : LOG2E;
+        /* qc is positive (its sign goes to the query): the largest product is the largest score, and one that is
+         * masked away, -inf, stays so */
+        const float post = fabsf(a.scale) * (a.softcap > 0.0f ? a.inv_softcap : LOG2E);
+        const float sign = copysignf(1.0f, a.scale);
 #pragma unroll
         for (int mt = 0; mt < MT; mt++) {
             const float *x = xq[mt];
             if constexpr (KV == KC_F32) {
 #pragma unroll
-                for (int i = 0; i < HD / 4; i++) split_tf32(x[i], qf[mt][2 * i], qf[mt][2 * i + 1]);
-                qc[mt] = a.scale * post;
+                for (int i = 0; i < HD / 4; i++) split_tf32(x[i] * sign, qf[mt][2 * i], qf[mt][2 * i + 1]);
+                qc[mt] = post;
             } else {
                 float mx = 0.0f;                       /* of the head, whose values the four lanes of a row hold */
 #pragma unroll
@@ -759,28 +768,29 @@ __global__ void __launch_bounds__(AT_THREADS, OCC) paged_attend_kernel(const __g
                      * that the low parts of all but vanishing values stay normal f16 */
                     int ex = (int)((__float_as_uint(mx) >> 23) & 255) - 127;
                     ex = min(max(ex, -100), 100);
-                    const float up = __uint_as_float((unsigned)(127 + 12 - ex) << 23);
-                    qc[mt] = a.scale * __uint_as_float((unsigned)(127 - 12 + ex) << 23) * post;
+                    const float up = sign * __uint_as_float((unsigned)(127 + 12 - ex) << 23);
+                    qc[mt] = __uint_as_float((unsigned)(127 - 12 + ex) << 23) * post;
 #pragma unroll
                     for (int i = 0; i < HD / 8; i++)
                         split_f16(x[2 * i] * up, x[2 * i + 1] * up, qf[mt][2 * i], qf[mt][2 * i + 1]);
                 } else {
                     /* the query head quantized as a cache row is (ops/ops.c:229-233) */
                     const bool tiny = mx < 1e-30f;
-                    const float id = tiny ? 0.0f : __fdiv_rn(127.0f, mx), qd = tiny ? 0.0f : __fdiv_rn(mx, 127.0f);
+                    const float id = tiny ? 0.0f : sign * __fdiv_rn(127.0f, mx), qd = tiny ? 0.0f : __fdiv_rn(mx, 127.0f);
 #pragma unroll
                     for (int j = 0; j < HD / 16; j++) {
                         /* x 127 / max rounded half away from zero: at most 127.5 and a rounding, never 128 */
                         int q[4];
 #pragma unroll
                         for (int i = 0; i < 4; i++)
-                            q[i] = __float2int_rz(__fadd_rn(__fmul_rn(x[4 * j + i], id), copysignf(0.5f, x[4 * j + i])));
+                            q[i] = __float2int_rz(__fadd_rn(__fmul_rn(x[4 * j + i], id), copysignf(0.5f, sign * x[4 * j + i])));
                         const unsigned w = __byte_perm(__byte_perm(q[0], q[1], 0x0040), __byte_perm(q[2], q[3], 0x0040), 0x5410);
                         qf[mt][j] = w;
                     }
-                    qc[mt] = __fmul_rn(qd, a.scale) * post;
+                    qc[mt] = qd * post;
                 }
             }
+            qc[mt] = fmaxf(qc[mt], 1.17549435e-38f);
         }
     };
 
@@ -810,8 +820,8 @@ __global__ void __launch_bounds__(AT_THREADS, OCC) paged_attend_kernel(const __g
             for (int mt = 0; mt < MT; mt++)
 #pragma unroll
                 for (int nt = 0; nt < NT; nt++) {
-                    s[mt][nt][0] = (d[mt][nt][0] + d[mt][nt][2]) * qc[mt];
-                    s[mt][nt][1] = (d[mt][nt][1] + d[mt][nt][3]) * qc[mt];
+                    s[mt][nt][0] = d[mt][nt][0] + d[mt][nt][2];
+                    s[mt][nt][1] = d[mt][nt][1] + d[mt][nt][3];
                 }
         } else if constexpr (KV == KC_F32) {
             float dh[MT][NT][4], dl[MT][NT][4];
@@ -845,17 +855,11 @@ __global__ void __launch_bounds__(AT_THREADS, OCC) paged_attend_kernel(const __g
             for (int mt = 0; mt < MT; mt++)
 #pragma unroll
                 for (int nt = 0; nt < NT; nt++) {
-                    s[mt][nt][0] = ((dh[mt][nt][0] + dh[mt][nt][2]) + (dl[mt][nt][0] + dl[mt][nt][2])) * qc[mt];
-                    s[mt][nt][1] = ((dh[mt][nt][1] + dh[mt][nt][3]) + (dl[mt][nt][1] + dl[mt][nt][3])) * qc[mt];
+                    s[mt][nt][0] = (dh[mt][nt][0] + dh[mt][nt][2]) + (dl[mt][nt][0] + dl[mt][nt][2]);
+                    s[mt][nt][1] = (dh[mt][nt][1] + dh[mt][nt][3]) + (dl[mt][nt][1] + dl[mt][nt][3]);
                 }
         } else {
-            int d[MT][NT][4];
-#pragma unroll
-            for (int mt = 0; mt < MT; mt++)
-#pragma unroll
-                for (int nt = 0; nt < NT; nt++)
-#pragma unroll
-                    for (int i = 0; i < 4; i++) d[mt][nt][i] = 0x4b400000;   /* 1.5 * 2^23: the sums come out as its floats */
+            int d[MT][NT][4];                          /* from 1.5 * 2^23: the sums come out as its floats */
             const uint32_t kb = sk + (lane & 7) * PITCH + (((lane >> 3) ^ swz(SWK, lane & 7)) << 4);
 #pragma unroll
             for (int jj = 0; jj < HD / 64; jj++)
@@ -865,7 +869,8 @@ __global__ void __launch_bounds__(AT_THREADS, OCC) paged_attend_kernel(const __g
                     ldsm4(b, (kb ^ (64 * jj)) + nt * 8 * PITCH);
 #pragma unroll
                     for (int mt = 0; mt < MT; mt++) {
-                        mma_s8(d[mt][nt], qf[mt][4 * jj], qf[mt][4 * jj + 1], b[0], b[1]);
+                        if (jj == 0) mma_s8_first(d[mt][nt], qf[mt][4 * jj], qf[mt][4 * jj + 1], b[0], b[1], 0x4b400000);
+                        else mma_s8(d[mt][nt], qf[mt][4 * jj], qf[mt][4 * jj + 1], b[0], b[1]);
                         mma_s8(d[mt][nt], qf[mt][4 * jj + 2], qf[mt][4 * jj + 3], b[2], b[3]);
                     }
                 }
@@ -875,27 +880,42 @@ __global__ void __launch_bounds__(AT_THREADS, OCC) paged_attend_kernel(const __g
                 const float2 e = *(const float2 *)(kd + nt * 8 + 2 * c);
 #pragma unroll
                 for (int mt = 0; mt < MT; mt++) {
-                    s[mt][nt][0] = (__int_as_float(d[mt][nt][0]) - 12582912.0f) * qc[mt] * e.x;
-                    s[mt][nt][1] = (__int_as_float(d[mt][nt][1]) - 12582912.0f) * qc[mt] * e.y;
+                    s[mt][nt][0] = (__int_as_float(d[mt][nt][0]) - 12582912.0f) * e.x;
+                    s[mt][nt][1] = (__int_as_float(d[mt][nt][1]) - 12582912.0f) * e.y;
                 }
             }
         }
     };
-    /* soft-cap, mask, running softmax in base 2: the scores become weights */
+    /* soft-cap, mask, running softmax in base 2: the scores become weights, lifted by a power of two that keeps
+     * the small ones normal f16 numbers: 2^15, and for 8-bit rows, whose scales join the weights, over the next
+     * power of two above the tile's largest scale (back: what the tile's sums are multiplied by) */
     float2 corr[MT];                                   /* what the sums so far are scaled by */
-    auto soften = [&](const unsigned (&live)[LK]) {
-        constexpr float LIFT = KV == KC_F32 ? 0.0f : 15.0f;   /* weights in (0, 2^15]: small ones stay normal f16 */
+    float back = 1.0f;
+    auto soften = [&](int stage, const unsigned (&live)[LK]) {
+        float lift = KV == KC_F32 ? 0.0f : 15.0f;
+        if constexpr (KV == KC_Q8_0) {
+            const float *vd = scl + stage * SCALES + TP;
+            float top = fabsf(vd[lane]);
+#pragma unroll
+            for (int k = 1; k < LK; k++) top = fmaxf(top, fabsf(vd[k * 32 + lane]));
+            top = warp_max(top);
+            int ex = (int)((__float_as_uint(top) >> 23) & 255) - 126;
+            ex = min(max(ex, -100), 100);
+            lift -= (float)ex;
+            back = __uint_as_float((unsigned)(127 + ex) << 23);
+        }
         bool all = true;
 #pragma unroll
         for (int k = 0; k < LK; k++) all &= live[k] == (unsigned)((1ull << RW) - 1);
 #pragma unroll
         for (int mt = 0; mt < MT; mt++) {
+            float qm = qc[mt];
             if (a.softcap > 0.0f) {
+                qm = a.softcap * LOG2E;
 #pragma unroll
                 for (int nt = 0; nt < NT; nt++)
 #pragma unroll
-                    for (int i = 0; i < 2; i++)
-                        s[mt][nt][i] = a.softcap * LOG2E * tanhf(s[mt][nt][i]);
+                    for (int i = 0; i < 2; i++) s[mt][nt][i] = tanhf(s[mt][nt][i] * qc[mt]);
             }
             if (!all) {
 #pragma unroll
@@ -909,7 +929,7 @@ __global__ void __launch_bounds__(AT_THREADS, OCC) paged_attend_kernel(const __g
             for (int nt = 1; nt < NT; nt++) mx = fmaxf(mx, fmaxf(s[mt][nt][0], s[mt][nt][1]));
             mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
             mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
-            const float mn = fmaxf(m[mt], mx), base = mn == -INFINITY ? 0.0f : mn, sub = base - LIFT;
+            const float mn = fmaxf(m[mt], mx * qm), base = mn == -INFINITY ? 0.0f : mn, add = lift - base;
             const float cr = ex2(m[mt] - base);
             corr[mt] = make_float2(cr, cr);
             m[mt] = mn;
@@ -918,11 +938,11 @@ __global__ void __launch_bounds__(AT_THREADS, OCC) paged_attend_kernel(const __g
             for (int nt = 0; nt < NT; nt++)
 #pragma unroll
                 for (int i = 0; i < 2; i++) {
-                    const float p = ex2(s[mt][nt][i] - sub);
+                    const float p = ex2(fmaf(s[mt][nt][i], qm, add));
                     s[mt][nt][i] = p;
                     sum += p;
                 }
-            l[mt] = l[mt] * cr + sum;
+            l[mt] = l[mt] * cr + sum * back;
         }
     };
     /* the weighted sum of V's rows */
@@ -998,23 +1018,15 @@ __global__ void __launch_bounds__(AT_THREADS, OCC) paged_attend_kernel(const __g
                     for (int i = 0; i < 4; i++) carry(acc[mt][4 * j + i], corr[mt], d[mt][i]);
             }
         } else {
-            /* the rows' scales join the weights; a power of two keeps the product in f16's range */
             constexpr int KS = TP / 16;
             const float *vd = scl + stage * SCALES + TP;
-            float top = fabsf(vd[lane]);
-#pragma unroll
-            for (int k = 1; k < LK; k++) top = fmaxf(top, fabsf(vd[k * 32 + lane]));
-            top = warp_max(top);
-            int ex = (int)((__float_as_uint(top) >> 23) & 255) - 127;
-            ex = min(max(ex, -100), 100);
-            const float dn = __uint_as_float((unsigned)(127 - 1 - ex) << 23), upf = __uint_as_float((unsigned)(127 + 1 + ex) << 23);
             unsigned w[MT][KS][4];
 #pragma unroll
             for (int nt = 0; nt < NT; nt++) {
                 const float2 e = *(const float2 *)(vd + nt * 8 + 2 * c);
 #pragma unroll
                 for (int mt = 0; mt < MT; mt++)
-                    split_f16(s[mt][nt][0] * (e.x * dn), s[mt][nt][1] * (e.y * dn), w[mt][nt >> 1][2 * (nt & 1)],
+                    split_f16(s[mt][nt][0] * e.x, s[mt][nt][1] * e.y, w[mt][nt >> 1][2 * (nt & 1)],
                               w[mt][nt >> 1][2 * (nt & 1) + 1]);
             }
             const uint32_t vb = sv + (lane & 15) * PITCH + (((lane >> 4) ^ swz(SWV, lane & 7)) << 4);
@@ -1065,7 +1077,7 @@ __global__ void __launch_bounds__(AT_THREADS, OCC) paged_attend_kernel(const __g
                     for (int k = 0; k < 4; k++)
                         acc[mt][4 * jj + k] = fma2(acc[mt][4 * jj + k], corr[mt],
                                                    mul2(add2(make_float2(d[mt][k][0], d[mt][k][1]),
-                                                             make_float2(d[mt][k][2], d[mt][k][3])), upf));
+                                                             make_float2(d[mt][k][2], d[mt][k][3])), back));
             }
         }
     };
@@ -1201,7 +1213,7 @@ __global__ void __launch_bounds__(AT_THREADS, OCC) paged_attend_kernel(const __g
             unsigned here[LK];
             here[0] = (unsigned)f.z;
             if constexpr (LK > 1) here[1] = (unsigned)f.w;
-            soften(here);
+            soften(stage, here);
             weigh(stage);
         }
         __syncwarp();
