@@ -48,7 +48,9 @@ struct AppendArgs {
 };
 
 constexpr int AP_THREADS = 256;
-constexpr int AP_HEADS = 4;                /* heads that a group of lanes takes at once */
+/* heads that a group of lanes takes at once */
+template <int NV>
+constexpr int ap_heads() { return NV == 1 ? 4 : 2; }
 
 /* The sum over the LPH lanes that hold a head's row. */
 template <int LPH, class T>
@@ -58,26 +60,26 @@ __device__ __forceinline__ T head_sum(T v) {
     return v;
 }
 
-/* 1 / sqrt(mean(x^2) + eps) of each of a lane's AP_HEADS heads, in type T. The
- * root and the division are taken once for all of them: lane k of a group does
- * head k's and hands it round. */
-template <class T, int LPH, int NV>
-__device__ __forceinline__ void head_norms(const float (&x)[AP_HEADS][NV][4], T (&inv)[AP_HEADS], float eps, int hd) {
+/* 1 / sqrt(mean(x^2) + eps) of each of a lane's NH heads, in type T. The root
+ * and the division are taken once for all of them: lane k of a group does head
+ * k's and hands it round. */
+template <class T, int LPH, int NV, int NH>
+__device__ __forceinline__ void head_norms(const float (&x)[NH][NV][4], T (&inv)[NH], float eps, int hd) {
     T mine = (T)0;
 #pragma unroll
-    for (int k = 0; k < AP_HEADS; k++) {
+    for (int k = 0; k < NH; k++) {
         T s = (T)0;
 #pragma unroll
         for (int j = 0; j < NV; j++)
 #pragma unroll
             for (int i = 0; i < 4; i++) s += (T)x[k][j][i] * (T)x[k][j][i];
         s = head_sum<LPH>(s);
-        if (threadIdx.x % AP_HEADS == k) mine = s;
+        if (threadIdx.x % NH == k) mine = s;
     }
     if constexpr (sizeof(T) == 8) mine = 1.0 / sqrt(mine / (double)hd + (double)eps);
     else mine = __fdiv_rn(1.0f, __fsqrt_rn(__fadd_rn(__fdiv_rn(mine, (float)hd), eps)));
 #pragma unroll
-    for (int k = 0; k < AP_HEADS; k++) inv[k] = __shfl_sync(0xffffffffu, mine, k, LPH);
+    for (int k = 0; k < NH; k++) inv[k] = __shfl_sync(0xffffffffu, mine, k, LPH);
 }
 
 /* y = x inv w, then the rotation of adjacent pairs, of 4 * NV values of a head, in type T. */
@@ -100,8 +102,8 @@ __device__ __forceinline__ void norm_rope(float (&x)[NV][4], bool norm, T inv, c
     }
 }
 
-/* A warp takes AP_HEADS heads of one kind (queries, keys or values) of a row
- * for each of its groups of LPH lanes, 4 * NV values of a head a lane. Bound by
+/* A warp takes four heads (two wide ones) of one kind (queries, keys or values)
+ * of a row for each of its groups of LPH lanes, 4 * NV values of a head a lane. Bound by
  * memory: every value is read once and written once, so all of a warp's heads
  * are requested before anything waits, and the row's place in the cache (three
  * dependent loads), its angles and the norm's weights are fetched once for them.
@@ -111,7 +113,7 @@ __device__ __forceinline__ void norm_rope(float (&x)[NV][4], bool norm, T inv, c
  * the order of the norm's sum; queries and wider caches use 32 bits. */
 template <int KV, int LPH, int NV>
 __global__ void __launch_bounds__(AP_THREADS) append_kernel(const AppendArgs a) {
-    constexpr int HW = AP_HEADS * (32 / LPH);          /* heads per warp */
+    constexpr int NH = ap_heads<NV>(), HW = NH * (32 / LPH);   /* heads per lane group and per warp */
     const int lane = threadIdx.x % LPH, sub = threadIdx.x % 32 / LPH, hd = a.kv.hd;
     const int tq = (a.n_heads + HW - 1) / HW, tk = (a.kv.n_kv + HW - 1) / HW, tasks = tq + 2 * tk;
     const long long item = ((long long)blockIdx.x * AP_THREADS + threadIdx.x) / 32;
@@ -122,9 +124,9 @@ __global__ void __launch_bounds__(AP_THREADS) append_kernel(const AppendArgs a) 
     const float *src = isq ? a.q + row * a.ldq : (isv ? a.v + row * a.ldv : a.k + row * a.ldk);
     const int seq = a.seqs ? a.seqs[row] : row, p = a.pos[row];
     if (seq < 0) return;                               /* padding */
-    float x[AP_HEADS][NV][4];
+    float x[NH][NV][4];
 #pragma unroll
-    for (int k = 0; k < AP_HEADS; k++)
+    for (int k = 0; k < NH; k++)
 #pragma unroll
         for (int j = 0; j < NV; j++) {
             const int d = 4 * (lane + j * LPH), h = h0 + k * (32 / LPH);
@@ -160,10 +162,10 @@ __global__ void __launch_bounds__(AP_THREADS) append_kernel(const AppendArgs a) 
         }
         auto turn = [&](auto one) {
             using T = decltype(one);
-            T inv[AP_HEADS];
-            if (wt) head_norms<T, LPH, NV>(x, inv, a.eps, hd);
+            T inv[NH];
+            if (wt) head_norms<T, LPH, NV, NH>(x, inv, a.eps, hd);
 #pragma unroll
-            for (int k = 0; k < AP_HEADS; k++) norm_rope<T, NV>(x[k], wt != nullptr, wt ? inv[k] : one, w, cs, sn);
+            for (int k = 0; k < NH; k++) norm_rope<T, NV>(x[k], wt != nullptr, wt ? inv[k] : one, w, cs, sn);
         };
         if (KV == KC_Q8_0 && !isq) turn(1.0);
         else turn(1.0f);
@@ -171,7 +173,7 @@ __global__ void __launch_bounds__(AP_THREADS) append_kernel(const AppendArgs a) 
     if (isq) {
         float *dst = a.q_out + row * a.ldo;
 #pragma unroll
-        for (int k = 0; k < AP_HEADS; k++)
+        for (int k = 0; k < NH; k++)
 #pragma unroll
             for (int j = 0; j < NV; j++) {
                 const int d = 4 * (lane + j * LPH), h = h0 + k * (32 / LPH);
@@ -182,22 +184,32 @@ __global__ void __launch_bounds__(AP_THREADS) append_kernel(const AppendArgs a) 
     }
     uint8_t *pool = isv ? a.kv.v : a.kv.k;
     const size_t r0 = (size_t)page * a.kv.n_kv * a.kv.page + slot;
+    /* the single-scale row rule of the model's 8-bit cache (ops/ops.c:81-96), its two divisions as the norms' */
+    float id[NH];
+    if constexpr (KV == KC_Q8_0) {
+        float mine = 0.0f;
 #pragma unroll
-    for (int k = 0; k < AP_HEADS; k++) {
-        const int h = h0 + k * (32 / LPH);
-        const size_t r = r0 + (size_t)h * a.kv.page;
-        /* the single-scale row rule of the model's 8-bit cache (ops/ops.c:81-96) */
-        float amax = 0.0f, id = 0.0f;
-        bool tiny = false;
-        if constexpr (KV == KC_Q8_0) {
+        for (int k = 0; k < NH; k++) {
+            float amax = 0.0f;
 #pragma unroll
             for (int j = 0; j < NV; j++)               /* (values beyond the head are zero) */
                 amax = fmaxf(amax, fmaxf(fmaxf(fabsf(x[k][j][0]), fabsf(x[k][j][1])), fmaxf(fabsf(x[k][j][2]), fabsf(x[k][j][3]))));
 #pragma unroll
             for (int o = LPH / 2; o > 0; o >>= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, o));
-            tiny = amax < 1e-30f;
-            id = tiny ? 0.0f : __fdiv_rn(127.0f, amax);
+            if (threadIdx.x % NH == k) mine = amax;
         }
+        const bool tiny = mine < 1e-30f;
+        const float mid = tiny ? 0.0f : __fdiv_rn(127.0f, mine);
+        const int h = h0 + lane * (32 / LPH);          /* lane k holds head k's */
+        if (lane < NH && h < nh)
+            (isv ? a.kv.vd : a.kv.kd)[r0 + (size_t)h * a.kv.page] = tiny ? 0.0f : __fdiv_rn(mine, 127.0f);
+#pragma unroll
+        for (int k = 0; k < NH; k++) id[k] = __shfl_sync(0xffffffffu, mid, k, LPH);
+    }
+#pragma unroll
+    for (int k = 0; k < NH; k++) {
+        const int h = h0 + k * (32 / LPH);
+        const size_t r = r0 + (size_t)h * a.kv.page;
 #pragma unroll
         for (int j = 0; j < NV; j++) {
             const int d = 4 * (lane + j * LPH);
@@ -209,20 +221,14 @@ __global__ void __launch_bounds__(AP_THREADS) append_kernel(const AppendArgs a) 
                 __half2 lo = __floats2half2_rn(y[0], y[1]), hi = __floats2half2_rn(y[2], y[3]);
                 ((uint2 *)pool)[(r * hd + d) / 4] = make_uint2(*(unsigned *)&lo, *(unsigned *)&hi);
             } else {
-                unsigned w = 0;
+                /* rounded half away from zero: at most 127.5 and a rounding, never 128 */
+                int q[4];
 #pragma unroll
-                for (int i = 0; i < 4; i++) {
-                    int qi = 0;
-                    if (!tiny) {
-                        const float u = truncf(__fadd_rn(__fmul_rn(y[i], id), copysignf(0.5f, y[i])));
-                        qi = (int)fminf(fmaxf(u, -127.0f), 127.0f);
-                    }
-                    w |= ((unsigned)qi & 0xffu) << (8 * i);
-                }
-                ((unsigned *)pool)[(r * hd + d) / 4] = w;
+                for (int i = 0; i < 4; i++) q[i] = __float2int_rz(__fadd_rn(__fmul_rn(y[i], id[k]), copysignf(0.5f, y[i])));
+                ((unsigned *)pool)[(r * hd + d) / 4] =
+                    __byte_perm(__byte_perm(q[0], q[1], 0x0040), __byte_perm(q[2], q[3], 0x0040), 0x5410);
             }
         }
-        if (KV == KC_Q8_0 && lane == 0 && h < nh) (isv ? a.kv.vd : a.kv.kd)[r] = tiny ? 0.0f : __fdiv_rn(amax, 127.0f);
     }
 }
 

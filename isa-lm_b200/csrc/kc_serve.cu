@@ -144,7 +144,7 @@ static int take_cache(const kc_paged_kv *kv, const ServeDev &d, PagedKV &o) {
 template <int KV>
 static void launch_append(const AppendArgs &a, cudaStream_t st) {
     const int hd = a.kv.hd, lph = hd <= 32 ? 8 : (hd <= 64 ? 16 : 32);
-    const int hw = AP_HEADS * (32 / lph);
+    const int hw = (hd <= 128 ? ap_heads<1>() : ap_heads<2>()) * (32 / lph);
     const long long warps = (long long)a.rows * ((a.n_heads + hw - 1) / hw + 2 * ((a.kv.n_kv + hw - 1) / hw));
     const unsigned grid = (unsigned)((warps + AP_THREADS / 32 - 1) / (AP_THREADS / 32));
     if (lph == 8) append_kernel<KV, 8, 1><<<grid, AP_THREADS, 0, st>>>(a);
@@ -397,22 +397,18 @@ extern "C" int kc_logits_process_dev(const kc_logits_args *x, void *stream) {
     a.bias_off = x->bias_off; a.bias_ids = x->bias_ids; a.bias_vals = x->bias_vals; a.n_bias = x->n_bias;
     a.mask = x->mask; a.ld_mask = x->ld_mask;
     a.err = d.err;
+    const bool hist = pen && x->history_cap > 0;
     const dim3 grid((unsigned)x->rows, (unsigned)((x->vocab + 3 + LG_CHUNK - 1) / LG_CHUNK));
     const cudaStream_t st = (cudaStream_t)stream;
-    const bool hist = pen && x->history_cap > 0;
-    if (hist && bias) {
-        /* beyond the static limit: the attribute belongs to the device */
-        static bool done[SV_MAX_DEVICES];
-        constexpr int smem = logits_smem<true, true>();
-        if (!done[d.dev]) SK(cudaFuncSetAttribute((const void *)logits_kernel<true, true>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem), "logits");
-        done[d.dev] = true;
-        logits_kernel<true, true><<<grid, LG_THREADS, smem, st>>>(a);
-    } else if (hist) {
-        logits_kernel<true, false><<<grid, LG_THREADS, logits_smem<true, false>(), st>>>(a);
-    } else if (bias) {
-        logits_kernel<false, true><<<grid, LG_THREADS, logits_smem<false, true>(), st>>>(a);
-    } else {
-        logits_kernel<false, false><<<grid, LG_THREADS, 0, st>>>(a);
-    }
+    if (hist && bias && (x->history_cap > 65535 || x->n_bias > 65534)) {
+        /* beyond the 16 bits that a count and a bias share: one after the other */
+        logits_kernel<true, false><<<grid, LG_THREADS, 0, st>>>(a);
+        a.in = a.out;
+        a.ld_in = a.ld_out;
+        logits_kernel<false, true><<<grid, LG_THREADS, 0, st>>>(a);
+    } else if (hist && bias) logits_kernel<true, true><<<grid, LG_THREADS, 0, st>>>(a);
+    else if (hist) logits_kernel<true, false><<<grid, LG_THREADS, 0, st>>>(a);
+    else if (bias) logits_kernel<false, true><<<grid, LG_THREADS, 0, st>>>(a);
+    else logits_kernel<false, false><<<grid, LG_THREADS, 0, st>>>(a);
     return sv_cuda(cudaGetLastError(), "logits");
 }

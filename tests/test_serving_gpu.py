@@ -348,7 +348,7 @@ def rand_logits_case(rng, n, v, hist, bias, mask, inf=False):
 
 @pytest.mark.parametrize("n,v,hist,bias,mask", [
     (1, 32000, 64, 0, 0), (3, 4097, 300, 50, 1), (2, 1, 3, 2, 1), (5, 31, None, 5, 1), (4, 151937, 2000, 0, 2),
-    (2, 8192, None, 0, 1), (3, 8191, 0, 300, 0), (70000, 5, 2, 0, 0)])
+    (2, 8192, None, 0, 1), (3, 8191, 0, 300, 0), (70000, 5, 2, 0, 0), (2, 300, 70001, 10, 1), (2, 12289, 9, 70000, 1)])
 def test_logits(n, v, hist, bias, mask):
     """Bit for bit: every operation is a single IEEE one, on NaN and infinite logits too."""
     rng = np.random.default_rng(n + v)
