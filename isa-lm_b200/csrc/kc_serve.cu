@@ -164,7 +164,7 @@ constexpr int AT_MAX_CTAS = 2048;
 /* One instance: its kernel, shared memory, and on each device the CTAs that fit. */
 struct AttendVariant {
     void (*attend)(const AttendArgs);
-    int smem, part, tile;
+    int smem, part, tile, heads;
     int ctas[SV_MAX_DEVICES];
 };
 
@@ -174,21 +174,24 @@ static AttendVariant make_variant() {
     v.attend = paged_attend_kernel<KV, HD, TM, MT, S, OCC>;
     v.smem = attend_smem<KV, HD, TM, MT, S>();
     v.part = part_floats<HD, MT>();
+    v.heads = 8 * MT;
     v.tile = att_tp<KV, TM>();
     return v;
 }
 
 /* The instance for a cache and group: a template of positions per tile, heads
- * per chunk, ring slots and CTAs an SM. Two slots a warp are enough; what pays
- * is a third CTA (12 warps an SM instead of 8) where the arithmetic, not the
- * copies, fills a tile's time: narrow heads, f32 (both halves of every value are
- * split) and so on. Where a tile is little more than its copies (f16, and 8-bit
- * of head 128), more copies under way only slow the memory down: 64 sequences of
- * 2048..8192 positions, f16, head 128: 206 us with 8 warps, 219 us with 12; 32 of
- * 2048, f32, head 64: 57.7 and 53.4 us; 64 of 4096, 8-bit, head 64: 76 and 65 us. */
+ * per chunk, ring slots and CTAs an SM. Two slots a warp are enough (a third only
+ * puts more copies under way than the memory likes: 64 sequences of 2048..8192
+ * positions, f16, head 128: 206 us with 16 KB a warp under way, 219 us with 24);
+ * a third CTA an SM (12 warps instead of 8) pays where arithmetic or the short
+ * sequences' own time fills the SM, above all at the clocks that a long run is
+ * held to: the same 64 sequences 212 us instead of 224, 256 of 1..1000 100 instead
+ * of 105, 64 of 4096, 8-bit, head 64, 66 instead of 71. Only the 8-bit cache of
+ * head 128 has no registers for it to spare: 32 of 2048 37 us with two CTAs, 38.5
+ * with three. */
 template <int KV>
 static AttendVariant *variants_of(int hd, int group, int &mt) {
-    static AttendVariant v64 = make_variant<KV, 64, 2, 1, 2, 3>(), v128 = make_variant<KV, 128, 1, 1, 2, KV == KC_F32 ? 3 : 2>(),
+    static AttendVariant v64 = make_variant<KV, 64, 2, 1, 2, 3>(), v128 = make_variant<KV, 128, 1, 1, 2, KV == KC_Q8_0 ? 2 : 3>(),
                          v256 = make_variant<KV, 256, 1, 1, 2, 1>();
     if constexpr (KV != KC_F32) {
         /* more than 8 heads share a KV head: 16 at a time, so that the cache is read once */
@@ -347,6 +350,9 @@ extern "C" int kc_paged_attend_dev(const kc_paged_kv *kv, const kc_attend_args *
     a.inv_softcap = x->softcap > 0.0f ? 1.0f / x->softcap : 0.0f;
     a.near = (v->tile - 1) / kv->page_size + 2 <= 32;
     a.unit_cost = AT_UNIT_COST;
+    /* measured: a piece of 16 heads of 128 (8 KB) is joined in 0.28 of a quantum's time, one of 4 heads of 64 in
+     * 0.035; one sequence of 8192 positions, 16 heads to a KV head, takes 61 us in the smallest shares, 31 us so */
+    a.join_cost = 1.4e-4f * (float)(std::min(a.group, v->heads) * kv->head_dim);
     a.grid_inv = ~0ull / (unsigned)ctas + 1;
     a.count = (unsigned *)x->ws;
     a.part = (float *)((char *)x->ws + sizeof(unsigned) * AT_MAX_CTAS);
