@@ -166,6 +166,19 @@ int kc_sample(kc_sampler *p, int *token);
 /* n tokens from `token` at `pos`: per step one decode step and one device
  * sample (no logits copy); out_tokens (host, n ints). */
 int kc_generate_sampled(kc_state *s, kc_sampler *p, int token, int pos, int n, int *out_tokens);
+/* Beside ml_sampler_opts (no reference counterpart): what the logits pass
+ * through before the following samples of `p`, in the order of
+ * kc_logits_process_dev below, until set again. The history is the ring of the
+ * last repeat_last_n tokens. Each copies its host arrays and waits for the
+ * state's stream.
+ * presence, frequency: taken off a ring token's logit once, and once for each
+ * time it is there (0, 0: off). */
+int kc_sampler_set_penalties(kc_sampler *p, float presence, float frequency);
+/* n biases added to tokens' logits (the last for a token counts); n 0: none. */
+int kc_sampler_set_bias(kc_sampler *p, const int *tokens, const float *values, int n);
+/* The tokens that may be chosen, bit v % 32 of word v / 32 of (vocab + 31) / 32
+ * words, at least one of them (a grammar's next tokens); NULL: all. */
+int kc_sampler_set_mask(kc_sampler *p, const uint32_t *words);
 /* The sampler's xorshift64* state (tests and resumption). */
 int kc_sampler_rng(kc_sampler *p, uint64_t *rng);
 void kc_sampler_free(kc_sampler *p);

@@ -1644,11 +1644,21 @@ struct kc_sampler {
     SampleArgs a{};
     SamplerDev host{};        /* mirror of the device state, refreshed after each call */
     std::vector<int> ring;    /* mirror of the device ring */
+    /* penalties, biases and a mask beside the reference's options (kc_sampler_set_*): the logits then pass
+     * through kc_logits_process_dev on their way */
+    bool more = false, masked = false;
+    float *values = nullptr;      /* repeat, presence, frequency, then the processed logits [vocab] */
+    uint32_t *mask = nullptr;
+    int *bias_ids = nullptr;      /* offsets 0 and n, then the ids */
+    float *bias_vals = nullptr;
+    int n_bias = 0;
 };
 
 extern "C" void kc_sampler_free(kc_sampler *p) {
     if (!p) return;
     if (p->arena) cudaFree(p->arena);
+    for (void *q : { (void *)p->values, (void *)p->mask, (void *)p->bias_ids, (void *)p->bias_vals })
+        if (q) cudaFree(q);
     delete p;
 }
 
@@ -1732,6 +1742,141 @@ extern "C" int kc_sampler_rng(kc_sampler *p, uint64_t *rng) {
     return KC_OK;
 }
 
+/* Host values into the sampler's device memory: behind its last sample and before its next, on the state's stream
+ * (a plain copy may end after it returns, on a stream that this one does not wait for). */
+static cudaError_t sampler_copy(kc_sampler *p, void *dst, const void *src, size_t bytes) {
+    const cudaError_t e = cudaMemcpyAsync(dst, src, bytes, cudaMemcpyHostToDevice, p->s->st);
+    return e == cudaSuccess ? cudaStreamSynchronize(p->s->st) : e;
+}
+
+/* Room for the processed logits, and the penalties as kc_logits_process_dev takes them. */
+static int sampler_more(kc_sampler *p) {
+    if (p->values) return KC_OK;
+    float *v = nullptr;
+    CK(cudaMalloc(&v, sizeof(float) * (64 + (size_t)p->s->c.vocab)));
+    const float init[3] = { p->o.repeat_penalty, 0.0f, 0.0f };
+    const cudaError_t e = sampler_copy(p, v, init, sizeof init);
+    if (e != cudaSuccess) {
+        cudaFree(v);
+        return cuda_status(e, "sampler");
+    }
+    p->values = v;
+    return KC_OK;
+}
+
+extern "C" int kc_sampler_set_penalties(kc_sampler *p, float presence, float frequency) {
+    clear_error();
+    if (!std::isfinite(presence) || !std::isfinite(frequency)) {
+        set_error("penalties must be finite");
+        return KC_E_SHAPE;
+    }
+    const int rc = sampler_more(p);
+    if (rc != KC_OK) return rc;
+    const float v[2] = { presence, frequency };
+    CK(sampler_copy(p, p->values + 1, v, sizeof v));
+    p->more = true;
+    return KC_OK;
+}
+
+extern "C" int kc_sampler_set_bias(kc_sampler *p, const int *tokens, const float *values, int n) {
+    clear_error();
+    if (n < 0 || (n > 0 && (!tokens || !values))) {
+        set_error("biases need tokens and values");
+        return KC_E_SHAPE;
+    }
+    for (int i = 0; i < n; i++)
+        if (tokens[i] < 0 || tokens[i] >= p->s->c.vocab || std::isnan(values[i])) {
+            set_error("a bias for a token outside the vocabulary, or not a number");
+            return KC_E_SHAPE;
+        }
+    int rc = sampler_more(p);
+    if (rc != KC_OK) return rc;
+    int *ids = nullptr;
+    float *vals = nullptr;
+    if (n > 0) {
+        std::vector<int> h((size_t)n + 2);
+        h[0] = 0;
+        h[1] = n;
+        std::copy(tokens, tokens + n, h.begin() + 2);
+        cudaError_t e = cudaMalloc(&ids, sizeof(int) * h.size());
+        if (e == cudaSuccess) e = cudaMalloc(&vals, sizeof(float) * (size_t)n);
+        if (e == cudaSuccess) e = sampler_copy(p, ids, h.data(), sizeof(int) * h.size());
+        if (e == cudaSuccess) e = sampler_copy(p, vals, values, sizeof(float) * (size_t)n);
+        if (e != cudaSuccess) {
+            cudaFree(ids);
+            cudaFree(vals);
+            return cuda_status(e, "biases");
+        }
+    }
+    CK(cudaStreamSynchronize(p->s->st));   /* the last sample may still read the old ones */
+    cudaFree(p->bias_ids);
+    cudaFree(p->bias_vals);
+    p->bias_ids = ids;
+    p->bias_vals = vals;
+    p->n_bias = n;
+    p->more = true;
+    return KC_OK;
+}
+
+extern "C" int kc_sampler_set_mask(kc_sampler *p, const uint32_t *words) {
+    clear_error();
+    const int V = p->s->c.vocab, nw = (V + 31) / 32;
+    if (words) {
+        uint32_t any = V & 31 ? words[nw - 1] & ((1u << (V & 31)) - 1u) : words[nw - 1];
+        for (int i = 0; i + 1 < nw; i++) any |= words[i];
+        if (!any) {
+            set_error("a mask that allows no token");
+            return KC_E_SHAPE;
+        }
+    }
+    const int rc = sampler_more(p);
+    if (rc != KC_OK) return rc;
+    if (words) {
+        if (!p->mask) CK(cudaMalloc(&p->mask, sizeof(uint32_t) * (size_t)nw));
+        CK(sampler_copy(p, p->mask, words, sizeof(uint32_t) * (size_t)nw));
+    }
+    p->masked = words != nullptr;
+    p->more = true;
+    return KC_OK;
+}
+
+/* The sampling kernel's arguments for a row of logits, which pass through the penalties, biases and mask that were
+ * set; the kernel's own penalty is theirs then. */
+static int sampler_args(kc_sampler *p, const float *logits, SampleArgs &a) {
+    a = p->a;
+    a.logits = logits;
+    if (!p->more) return KC_OK;
+    kc_logits_args x{};
+    x.in = logits;
+    x.out = p->values + 64;
+    x.rows = 1;
+    x.vocab = a.vocab;
+    x.ld_in = x.ld_out = a.vocab;
+    if (a.repeat_last_n > 0) {
+        x.history = a.recent;
+        x.history_len = &a.st->n_recent;
+        x.history_cap = a.repeat_last_n;
+        x.ld_history = a.repeat_last_n;
+        x.repeat = p->values;
+        x.presence = p->values + 1;
+        x.frequency = p->values + 2;
+    }
+    if (p->n_bias) {
+        x.bias_off = p->bias_ids;
+        x.bias_ids = p->bias_ids + 2;
+        x.bias_vals = p->bias_vals;
+        x.n_bias = p->n_bias;
+    }
+    if (p->masked) {
+        x.mask = p->mask;
+        x.ld_mask = (a.vocab + 31) / 32;
+        a.allowed = p->mask;
+    }
+    a.logits = x.out;
+    a.repeat_penalty = 1.0f;
+    return kc_logits_process_dev(&x, p->s->st);
+}
+
 extern "C" int kc_sample(kc_sampler *p, int *token) {
     clear_error();
     kc_state *s = p->s;
@@ -1739,8 +1884,9 @@ extern "C" int kc_sample(kc_sampler *p, int *token) {
         set_error("no logits of a last token on the device: run kc_forward first");
         return KC_E_SHAPE;
     }
-    SampleArgs a = p->a;
-    a.logits = s->logits + (size_t)s->last_row * s->c.vocab;
+    SampleArgs a;
+    const int rc = sampler_args(p, s->logits + (size_t)s->last_row * s->c.vocab, a);
+    if (rc != KC_OK) return rc;
     a.ls = nullptr;
     a.out_tokens = nullptr;
     sample_kernel<<<1, SM_THREADS, 0, s->st>>>(a);
@@ -1759,8 +1905,9 @@ extern "C" int kc_generate_sampled(kc_state *s, kc_sampler *p, int token, int po
     for (int i = 0; i < n; i++) {
         st = run_steps(s, 1, 1);
         if (st != KC_OK) return st;
-        SampleArgs a = p->a;
-        a.logits = s->logits + (size_t)(i % LOGITS_RING) * c.vocab;
+        SampleArgs a;
+        st = sampler_args(p, s->logits + (size_t)(i % LOGITS_RING) * c.vocab, a);
+        if (st != KC_OK) return st;
         a.ls = s->ls;
         a.out_tokens = s->out_tokens;
         sample_kernel<<<1, SM_THREADS, 0, s->st>>>(a);

@@ -50,6 +50,7 @@ struct SampleArgs {
     int *token_out;           /* the sampled token */
     LoopState *ls;            /* optional: the device loop, advanced to the token */
     int *out_tokens;          /* optional, with ls: the step's slot */
+    const uint32_t *allowed;  /* optional: the tokens that may be chosen, a bit each */
 };
 
 __device__ __forceinline__ float sm_block_max(float v, float *red) {
@@ -431,6 +432,24 @@ __global__ void __launch_bounds__(SM_THREADS, 1) sample_kernel(const SampleArgs 
         }
     }
     __syncthreads();
+    if (a.allowed && !((a.allowed[s_tok >> 5] >> (s_tok & 31)) & 1u)) {
+        /* a masked logit is -inf and its token's probability 0, but a draw that rounding leaves past the last
+         * running sum falls on whatever token is last (:63-70), and so may rows whose allowed logits are all
+         * -inf: the best of the allowed ones then */
+        unsigned long long best = 0ull;
+        for (int i = tid; i < n; i += SM_THREADS)
+            if ((a.allowed[i >> 5] >> (i & 31)) & 1u) {
+                const unsigned long long k = argmax_key(p[i], i);
+                best = k > best ? k : best;
+            }
+        __syncthreads();
+        if (tid == 0) s_best = 0ull;
+        __syncthreads();
+        atomicMax(&s_best, best);
+        __syncthreads();
+        if (tid == 0) s_tok = (int)(0xffffffffu - (unsigned)(s_best & 0xffffffffull));
+        __syncthreads();
+    }
     if (tid == 0) {
         const int tok = s_tok;
         *a.token_out = tok;

@@ -90,6 +90,8 @@ def lib():
             "kc_set_device": (I, [I]), "kc_tp_handle": (I, [P, P, S]), "kc_tp_connect": (I, [P, P]),
             "kc_sampler_init": (I, [C.POINTER(P), P, P]), "kc_sampler_accept": (I, [P, I]),
             "kc_sample": (I, [P, C.POINTER(I)]), "kc_generate_sampled": (I, [P, P, I, I, I, P]),
+            "kc_sampler_set_penalties": (I, [P, F, F]), "kc_sampler_set_bias": (I, [P, P, P, I]),
+            "kc_sampler_set_mask": (I, [P, P]),
             "kc_sampler_rng": (I, [P, C.POINTER(C.c_uint64)]), "kc_sampler_free": (None, [P]),
             "kc_forward": (C.POINTER(F), [P, I, I]), "kc_generate_greedy": (I, [P, I, I, I, P]),
             "kc_state_free": (None, [P]),
@@ -143,6 +145,30 @@ class Sampler:
         t = C.c_int()
         _check(lib().kc_sample(self._h, C.byref(t)), "sample")
         return t.value
+
+    def set_penalties(self, presence=0.0, frequency=0.0):
+        """Taken off the logits of the ring's tokens from now on (kc_sampler_set_penalties)."""
+        _check(lib().kc_sampler_set_penalties(self._h, presence, frequency), "set penalties")
+        return self
+
+    def set_bias(self, biases=None):
+        """{token: value} (or pairs, the last for a token counts) added to logits from now on; None: none."""
+        pairs = list(biases.items() if hasattr(biases, "items") else biases or [])
+        t, v = np.array([p[0] for p in pairs], np.int32), np.array([p[1] for p in pairs], np.float32)
+        _check(lib().kc_sampler_set_bias(self._h, t.ctypes.data_as(C.c_void_p), v.ctypes.data_as(C.c_void_p), len(pairs)),
+               "set bias")
+        return self
+
+    def set_mask(self, allowed=None):
+        """The tokens that may be chosen from now on: a boolean array [vocab]; None: all."""
+        words = None
+        if allowed is not None:
+            a, v = np.asarray(allowed, bool), self.state.cfg["vocab"]
+            if a.shape != (v,):
+                raise _shape_error(f"allowed is {list(a.shape)}, not [{v}]")
+            words = np.packbits(np.pad(a, (0, -v % 32)), bitorder="little").view(np.uint32)
+        _check(lib().kc_sampler_set_mask(self._h, None if words is None else words.ctypes.data_as(C.c_void_p)), "set mask")
+        return self
 
     @property
     def rng(self):
