@@ -307,7 +307,8 @@ int kc_debug_ffn_split(int mode);
  * table[s * ld_table + p / page_size]. Row (page, kv head, slot) of k and v
  * holds head_dim values of kv_type (KC_F32, KC_F16, KC_Q8_0: int8 with the
  * scales kd and vd, one for each row). Entries of the table beyond a
- * sequence's length are not read, slots beyond it may hold anything. */
+ * sequence's length are not followed, slots beyond it may hold anything, NaN
+ * too; keys and values within it are finite. */
 typedef struct {
     void *k, *v;                 /* [n_pages][n_kv_heads][page_size][head_dim], 16-byte aligned */
     float *kd, *vd;              /* KC_Q8_0: [n_pages][n_kv_heads][page_size]; else NULL */
@@ -371,7 +372,8 @@ int kc_paged_attend_dev(const kc_paged_kv *kv, const kc_attend_args *args, void 
 int kc_paged_attend_ws(const kc_paged_kv *kv, int n_heads, size_t *bytes);
 int kc_paged_attend_ws_init(void *ws, size_t bytes);
 
-/* Logits before a token is chosen, rows [vocab] of in to out (out may be in):
+/* Logits before a token is chosen, rows [vocab] of in to out (out may be in,
+ * with the same stride; otherwise the two do not overlap):
  * with c the times that token v is in the row's history,
  *   c > 0: z = z > 0 ? z / repeat : z * repeat (the sampler's penalty,
  *          model/sampler.c:30-42), then z -= frequency * c, z -= presence;

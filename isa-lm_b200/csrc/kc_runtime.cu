@@ -1794,13 +1794,11 @@ extern "C" int kc_sampler_set_bias(kc_sampler *p, const int *tokens, const float
     int *ids = nullptr;
     float *vals = nullptr;
     if (n > 0) {
-        std::vector<int> h((size_t)n + 2);
-        h[0] = 0;
-        h[1] = n;
-        std::copy(tokens, tokens + n, h.begin() + 2);
-        cudaError_t e = cudaMalloc(&ids, sizeof(int) * h.size());
+        const int off[2] = { 0, n };
+        cudaError_t e = cudaMalloc(&ids, sizeof(int) * ((size_t)n + 2));
         if (e == cudaSuccess) e = cudaMalloc(&vals, sizeof(float) * (size_t)n);
-        if (e == cudaSuccess) e = sampler_copy(p, ids, h.data(), sizeof(int) * h.size());
+        if (e == cudaSuccess) e = sampler_copy(p, ids, off, sizeof off);
+        if (e == cudaSuccess) e = sampler_copy(p, ids + 2, tokens, sizeof(int) * (size_t)n);
         if (e == cudaSuccess) e = sampler_copy(p, vals, values, sizeof(float) * (size_t)n);
         if (e != cudaSuccess) {
             cudaFree(ids);

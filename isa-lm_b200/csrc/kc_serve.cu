@@ -368,6 +368,7 @@ extern "C" int kc_logits_process_dev(const kc_logits_args *x, void *stream) {
     if (!x) return refuse("args is NULL");
     if (x->rows < 0 || x->vocab < 1 || x->vocab > (1 << 27)) return refuse("rows must not be negative, vocab 1 to 2^27");
     if (x->rows > 1 && (x->ld_in < x->vocab || x->ld_out < x->vocab)) return refuse("a row stride is shorter than its row");
+    if (x->in == x->out && x->rows > 1 && x->ld_in != x->ld_out) return refuse("in place, but the row strides differ");
     const bool pen = x->repeat || x->presence || x->frequency;
     if (x->history_cap < 0 || (x->history && x->rows > 1 && x->ld_history < x->history_cap))
         return refuse("history_cap must not be negative nor beyond ld_history");

@@ -81,7 +81,7 @@ def logits_args(**kw):
     (dict(rows=-1), "rows"), (dict(vocab=0), "vocab"), (dict(vocab=(1 << 27) + 1), "vocab"), (dict(ld_in=99), "shorter"),
     (dict(history=P, history_cap=9, ld_history=8), "history_cap"), (dict(history_cap=2), "history"),
     (dict(bias_off=P, n_bias=3), "biases"), (dict(bias_ids=P, n_bias=3), "biases"), (dict(bias_off=P, n_bias=-1), "biases"),
-    (dict(mask=P, ld_mask=3), "mask")])
+    (dict(mask=P, ld_mask=3), "mask"), (dict(ld_out=104), "in place")])
 def test_logits_are_refused(kw, word):
     assert word in refused(kb.lib().kc_logits_process_dev, logits_args(**kw))
 

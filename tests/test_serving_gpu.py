@@ -181,6 +181,43 @@ def test_attend_small_and_large_values():
     check(out.numpy(), want, reach, np.abs(v.astype(float)).max(), hd, n)
 
 
+@pytest.mark.parametrize("kv", ["f32", "f16", "q8"])
+@pytest.mark.parametrize("softcap", [0.0, 4.0])
+def test_attend_signs_of_the_scale(kv, softcap):
+    """A negative scale, one of zero (the mean of V), and a query head of zeros."""
+    rng = np.random.default_rng(9)
+    lens, page, hk, hd, heads = [70, 33], 16, 2, 64, 6
+    pools = make_pool(rng, kv, 12, hk, page, hd)
+    table = make_table(rng, lens, page, 12)
+    q = rng.standard_normal((2, heads, hd)).astype(np.float32)
+    q[0, 2] = 0.0
+    c = handle(pools, table, kv, heads)
+    k, v, kd, vd = pools
+    vmax = np.abs(v.astype(np.float64)).max() if kd is None else (127 * vd).max()
+    for scale in (-0.2, 0.0, 0.1):
+        out = c.attend(kb.DevArray.of(q), kb.DevArray.of(np.array(lens, np.int32)), kb.DevArray(q.shape, np.float32),
+                       scale=scale, softcap=softcap)
+        want, reach = ref.attend(q, k, v, table, lens, scale, 0, softcap, kd, vd)
+        check(out.numpy(), want, reach, vmax, hd, 70)
+
+
+def test_attend_one_bad_head_stays_alone():
+    """A NaN in one sequence's KV head reaches that head's queries only."""
+    rng = np.random.default_rng(10)
+    lens, page, hk, hd, heads = [50, 40], 16, 2, 64, 4
+    pools = make_pool(rng, "f16", 12, hk, page, hd)
+    table = make_table(rng, lens, page, 12)
+    q = rng.standard_normal((2, heads, hd)).astype(np.float32)
+    k, v = pools[:2]
+    want, reach = ref.attend(q, k, v, table, lens, hd ** -0.5)
+    k[table[0, 1], 1, 3] = np.nan
+    out = handle(pools, table, "f16", heads).attend(kb.DevArray.of(q), kb.DevArray.of(np.array(lens, np.int32)),
+                                                    kb.DevArray(q.shape, np.float32)).numpy()
+    assert np.isnan(out[0, 2:]).all()
+    out[0, 2:] = want[0, 2:]
+    check(out, want, reach, 6, hd, 50)
+
+
 def test_attend_strides_and_rows_behind():
     """Query and output rows inside wider ones; fewer sequences than the cache has."""
     torch = pytest.importorskip("torch")
@@ -359,6 +396,7 @@ def test_logits(n, v, hist, bias, mask):
     want = ref.logits(z, **kw)
     assert np.array_equal(out.numpy(), want, equal_nan=True)
     kb.process_logits(dz, dz, **dev)                           # in place
+    kb._check(kb.lib().kc_dev_sync(), "sync")
     assert np.array_equal(dz.numpy(), want, equal_nan=True)
 
 
