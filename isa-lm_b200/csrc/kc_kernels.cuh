@@ -47,6 +47,14 @@ struct LoopState {
 
 /* ------------------------------------------------------------ helpers */
 
+/* A kernel launched to overlap the end of the stream's work before it
+ * (launch_after) first waits until everything before is done and its writes are
+ * seen: nothing is read or written before that. launch_next lets the stream's
+ * next such kernel be launched, once every CTA has called it or ended; its CTAs
+ * wait in turn. */
+__device__ __forceinline__ void stream_order() { cudaGridDependencySynchronize(); }
+__device__ __forceinline__ void launch_next() { cudaTriggerProgrammaticLaunchCompletion(); }
+
 __device__ __forceinline__ float warp_sum(float v) {
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);

@@ -56,6 +56,8 @@ __global__ void __launch_bounds__(LG_THREADS, 5) logits_kernel(const LogitsArgs 
     __shared__ __align__(16) uint32_t s_word[ANY ? LG_CHUNK : 4];
     __shared__ unsigned short s_list[ANY ? LG_CHUNK : 1];
     __shared__ int s_n;
+    launch_next();
+    stream_order();
     const int tid = threadIdx.x, V = a.vocab;
     const long long row = blockIdx.x;
     const float *in = a.in + row * a.ld_in;

@@ -113,6 +113,8 @@ __device__ __forceinline__ void norm_rope(float (&x)[NV][4], bool norm, T inv, c
  * the order of the norm's sum; queries and wider caches use 32 bits. */
 template <int KV, int LPH, int NV>
 __global__ void __launch_bounds__(AP_THREADS) append_kernel(const AppendArgs a) {
+    launch_next();
+    stream_order();
     constexpr int NH = ap_heads<NV>(), HW = NH * (32 / LPH);   /* heads per lane group and per warp */
     const int lane = threadIdx.x % LPH, sub = threadIdx.x % 32 / LPH, hd = a.kv.hd;
     const int tq = (a.n_heads + HW - 1) / HW, tk = (a.kv.n_kv + HW - 1) / HW, tasks = tq + 2 * tk;
@@ -519,6 +521,7 @@ __global__ void __launch_bounds__(AT_THREADS, OCC) paged_attend_kernel(const __g
     float *cml = comb + AT_WARPS * AT_COMB * HD;       /* and their maxima and weights' sums */
     const int U = a.kv.n_kv * a.chunks;                /* units per sequence */
     const int W = a.unit_cost;
+    stream_order();
 
     /* ---- this CTA's share: [i chunk, (i + 1) chunk) of the units' times, laid end to end; every warp
      * finds it by itself, a run of sequences a lane ---- */
@@ -1239,6 +1242,8 @@ __global__ void __launch_bounds__(AT_THREADS, OCC) paged_attend_kernel(const __g
             if (!complete) leave(cu_b, cu_u);
         }
     }
+    /* not sooner: the next call's CTAs would crowd the SMs that still have room, and its few working ones share them */
+    launch_next();
     __syncthreads();
     for (int k = 0; k < 2; k++)
         if (s_join[k][0]) {

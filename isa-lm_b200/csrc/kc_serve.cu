@@ -139,18 +139,34 @@ static int take_cache(const kc_paged_kv *kv, const ServeDev &d, PagedKV &o) {
     return KC_OK;
 }
 
+/* A launch that may begin while the stream's kernel before it ends (its CTAs wait in stream_order): in a run of
+ * these operators the launch itself costs nothing then. */
+template <class A>
+static cudaError_t launch_after(void (*kernel)(const A), unsigned gx, unsigned gy, int threads, size_t smem, cudaStream_t st, const A &a) {
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3(gx, gy);
+    cfg.blockDim = dim3((unsigned)threads);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = st;
+    cudaLaunchAttribute at{};
+    at.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    at.val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = &at;
+    cfg.numAttrs = 1;
+    return cudaLaunchKernelEx(&cfg, kernel, a);
+}
+
 /* ------------------------------------------------------------ append */
 
 template <int KV>
-static void launch_append(const AppendArgs &a, cudaStream_t st) {
+static cudaError_t launch_append(const AppendArgs &a, cudaStream_t st) {
     const int hd = a.kv.hd, lph = hd <= 32 ? 8 : (hd <= 64 ? 16 : 32);
     const int hw = (hd <= 128 ? ap_heads<1>() : ap_heads<2>()) * (32 / lph);
     const long long warps = (long long)a.rows * ((a.n_heads + hw - 1) / hw + 2 * ((a.kv.n_kv + hw - 1) / hw));
     const unsigned grid = (unsigned)((warps + AP_THREADS / 32 - 1) / (AP_THREADS / 32));
-    if (lph == 8) append_kernel<KV, 8, 1><<<grid, AP_THREADS, 0, st>>>(a);
-    else if (lph == 16) append_kernel<KV, 16, 1><<<grid, AP_THREADS, 0, st>>>(a);
-    else if (hd <= 128) append_kernel<KV, 32, 1><<<grid, AP_THREADS, 0, st>>>(a);
-    else append_kernel<KV, 32, 2><<<grid, AP_THREADS, 0, st>>>(a);
+    return launch_after(lph == 8 ? append_kernel<KV, 8, 1>
+                                 : (lph == 16 ? append_kernel<KV, 16, 1> : (hd <= 128 ? append_kernel<KV, 32, 1> : append_kernel<KV, 32, 2>)),
+                        grid, 1, AP_THREADS, 0, st, a);
 }
 
 /* ------------------------------------------------------------ attention */
@@ -272,10 +288,9 @@ extern "C" int kc_paged_append_dev(const kc_paged_kv *kv, const kc_append_args *
     a.seqs = x->seqs; a.pos = x->pos; a.rows = x->rows; a.n_heads = x->n_heads; a.n_pos = x->n_pos;
     a.err = d.err;
     const cudaStream_t st = (cudaStream_t)stream;
-    if (kv->kv_type == KC_F32) launch_append<KC_F32>(a, st);
-    else if (kv->kv_type == KC_F16) launch_append<KC_F16>(a, st);
-    else launch_append<KC_Q8_0>(a, st);
-    return sv_cuda(cudaGetLastError(), "append");
+    return sv_cuda(kv->kv_type == KC_F32 ? launch_append<KC_F32>(a, st)
+                                         : (kv->kv_type == KC_F16 ? launch_append<KC_F16>(a, st) : launch_append<KC_Q8_0>(a, st)),
+                   "append");
 }
 
 static int check_heads(const kc_paged_kv *kv, int n_heads) {
@@ -357,8 +372,7 @@ extern "C" int kc_paged_attend_dev(const kc_paged_kv *kv, const kc_attend_args *
     a.count = (unsigned *)x->ws;
     a.part = (float *)((char *)x->ws + sizeof(unsigned) * AT_MAX_CTAS);
     a.err = d.err;
-    v->attend<<<ctas, AT_THREADS, v->smem, (cudaStream_t)stream>>>(a);
-    return sv_cuda(cudaGetLastError(), "attend");
+    return sv_cuda(launch_after(v->attend, (unsigned)ctas, 1, AT_THREADS, (size_t)v->smem, (cudaStream_t)stream, a), "attend");
 }
 
 /* ------------------------------------------------------------ logits */
@@ -405,17 +419,17 @@ extern "C" int kc_logits_process_dev(const kc_logits_args *x, void *stream) {
     a.mask = x->mask; a.ld_mask = x->ld_mask;
     a.err = d.err;
     const bool hist = pen && x->history_cap > 0;
-    const dim3 grid((unsigned)x->rows, (unsigned)((x->vocab + 3 + LG_CHUNK - 1) / LG_CHUNK));
+    const unsigned rows = (unsigned)x->rows, chunks = (unsigned)((x->vocab + 3 + LG_CHUNK - 1) / LG_CHUNK);
     const cudaStream_t st = (cudaStream_t)stream;
     if (hist && bias && (x->history_cap > 65535 || x->n_bias > 65534)) {
         /* beyond the 16 bits that a count and a bias share: one after the other */
-        logits_kernel<true, false><<<grid, LG_THREADS, 0, st>>>(a);
+        SK(launch_after(logits_kernel<true, false>, rows, chunks, LG_THREADS, 0, st, a), "logits");
         a.in = a.out;
         a.ld_in = a.ld_out;
-        logits_kernel<false, true><<<grid, LG_THREADS, 0, st>>>(a);
-    } else if (hist && bias) logits_kernel<true, true><<<grid, LG_THREADS, 0, st>>>(a);
-    else if (hist) logits_kernel<true, false><<<grid, LG_THREADS, 0, st>>>(a);
-    else if (bias) logits_kernel<false, true><<<grid, LG_THREADS, 0, st>>>(a);
-    else logits_kernel<false, false><<<grid, LG_THREADS, 0, st>>>(a);
-    return sv_cuda(cudaGetLastError(), "logits");
+        return sv_cuda(launch_after(logits_kernel<false, true>, rows, chunks, LG_THREADS, 0, st, a), "logits");
+    }
+    return sv_cuda(launch_after(hist ? (bias ? logits_kernel<true, true> : logits_kernel<true, false>)
+                                     : (bias ? logits_kernel<false, true> : logits_kernel<false, false>),
+                                rows, chunks, LG_THREADS, 0, st, a),
+                   "logits");
 }
