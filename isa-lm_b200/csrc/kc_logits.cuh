@@ -13,8 +13,8 @@
  * shared memory which history tokens and biases fall into its stretch while the
  * logits arrive, writes them through the mask, and then goes over the few that
  * are touched, listed once each, whose values it makes meanwhile. 64 rows of
- * 128256: 12.4 us with a mask alone, 18.9 us with 2048 tokens of history and 100
- * biases each (floor 10.4). Measured beside it and not taken: every logit looking
+ * 128256: 11.9 us with a mask alone, 18.4 us with 2048 tokens of history and 100
+ * biases each, from memory (floor 10.4). Measured beside it and not taken: every logit looking
  * at its own counter, 1.9 times the instructions; stretches of 16384 logits that
  * share one look at the history, the same time, since one wave of CTAs then
  * counts while the memory waits and streams while the counters do. */

@@ -102,7 +102,12 @@ __device__ __forceinline__ void norm_rope(float (&x)[NV][4], bool norm, T inv, c
     }
 }
 
-/* A warp takes four heads (two wide ones) of one kind (queries, keys or values)
+/* Measured: 4096 rows of 32 + 8 + 8 heads of 128 into an f16 cache 30.6 us a call in
+ * a run of them (187 MB, floor 28.9 at a copy's rate), 34.6 us where the rows come
+ * from memory; as many normed into an 8-bit cache 42.9 us (floor 27.6), the
+ * difference mostly the conversions to 64 bits and back.
+ *
+ * A warp takes four heads (two wide ones) of one kind (queries, keys or values)
  * of a row for each of its groups of LPH lanes, 4 * NV values of a head a lane. Bound by
  * memory: every value is read once and written once, so all of a warp's heads
  * are requested before anything waits, and the row's place in the cache (three
@@ -254,7 +259,19 @@ __global__ void __launch_bounds__(AP_THREADS) append_kernel(const AppendArgs a) 
  * the high halves leave (two f16 of 11 bits each, or two tf32), so a product
  * keeps 22 bits of a 32-bit query or softmax weight, at no more instructions
  * than one f16 row block takes. The sums of a tile leave the tensor core once
- * per tile and are carried in f32. */
+ * per tile and are carried in f32. (Up to 16 query rows against rows that are
+ * used once: a product of this shape has 4 operations a byte and wants warps
+ * that load for themselves; mma.sync at its operands' rate is far from bounding
+ * it, tcgen05's 128-row tiles would be 7/8 padding.)
+ *
+ * What bounds it: the cache's bytes, read once. 64 sequences of 2048..8192
+ * positions (32 heads on 8, head 128, f16, 1.34 GB) 211 us in a long run, 6.4 TB/s,
+ * what a copy reaches; 2 of 131072 176 us, 5.8 TB/s. Where the bytes are fewer the
+ * arithmetic shows: splitting an f32 value takes four integer and float
+ * instructions, an 8-bit one a fifth of a word's five (64 of 4096, head 64, 8-bit:
+ * 61 us at a floor of 44; 32 of 2048, head 64, f32: 52 at 41). Small calls are
+ * bound by their chain of latencies, about 5.6 us for one tile: launch, length,
+ * table, rows, products, the warps' meeting; a joined unit 3 us more. */
 constexpr int AT_WARPS = 4;
 constexpr int AT_THREADS = AT_WARPS * 32;
 /* Quanta of a unit that is not worth sharing out where every unit has a CTA of its own: of 5 quanta, 78 units 11.2 us
