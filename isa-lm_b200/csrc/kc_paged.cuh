@@ -647,7 +647,7 @@ __global__ void __launch_bounds__(AT_THREADS, OCC) paged_attend_kernel(const __g
     };
     enum { LAST_OF_UNIT = 1 << 28, LAST_OF_SHARE = 1 << 29 };
     unsigned live[LK], row[LK];                        /* of the loader's tile: rows that are there, and where */
-    bool full;                                         /* all of them, and as long as the slot's */
+    bool full;                                         /* all of them */
     /* Rows start at different bank groups, by an exclusive or of the 16-byte chunk's number with swz(row): for
      * row-per-lane reads of eight rows (ldmatrix, and f32 V) the row's low bits, or the next ones where two rows
      * share 128 bytes; for f32 K, read by four lanes a row and eight rows in turn, the low bits reversed. */
@@ -658,17 +658,19 @@ __global__ void __launch_bounds__(AT_THREADS, OCC) paged_attend_kernel(const __g
     auto copy_rows = [&](uint32_t sk) {
         constexpr int RE = CPR < 32 ? 32 / CPR : 1, WE = CPR > 32 ? CPR / 32 : 1;   /* rows per 512 bytes, or the other way round */
         const uint32_t tk = sk + tl * PITCH + ((cl ^ swz(SWK, tl)) << 4), tv = sk + VOFF + tl * PITCH + ((cl ^ swz(SWV, tl)) << 4);
+        const unsigned rowb = (unsigned)a.kv.hd * ES;
         if (full) {
             const uint8_t *ks = a.kv.k + cl * 16, *vs = a.kv.v + cl * 16;
 #pragma unroll
             for (int e = 0; e < TP * CPR / 32; e++) {
                 const int te = e / WE * RE, ce = 32 * (e % WE), to = te * PITCH + ce * 16;
-                const size_t off = (size_t)__shfl_sync(0xffffffffu, row[te / RW], (te + tl) & (RW - 1)) * PITCH;
-                cp_async16s((tk ^ (uint32_t)(swz(SWK, te) << 4)) + to, ks + off + ce * 16);
-                cp_async16s((tv ^ (uint32_t)(swz(SWV, te) << 4)) + to, vs + off + ce * 16);
+                const size_t off = (size_t)__shfl_sync(0xffffffffu, row[te / RW], (te + tl) & (RW - 1)) * rowb;
+                if ((cl + ce) * 16 < (int)rowb) {      /* (the chunks behind a shorter head stay zero) */
+                    cp_async16s((tk ^ (uint32_t)(swz(SWK, te) << 4)) + to, ks + off + ce * 16);
+                    cp_async16s((tv ^ (uint32_t)(swz(SWV, te) << 4)) + to, vs + off + ce * 16);
+                }
             }
         } else {
-            const unsigned rowb = (unsigned)a.kv.hd * ES;
 #pragma unroll 1
             for (int e = 0; e < TP * CPR / 32; e++) {
                 const int te = e / WE * RE, ce = 32 * (e % WE), t = (te + tl) & (RW - 1), k = te / RW, to = te * PITCH + ce * 16;
@@ -680,6 +682,10 @@ __global__ void __launch_bounds__(AT_THREADS, OCC) paged_attend_kernel(const __g
             }
         }
     };
+    if (a.kv.hd < HD) {
+        for (int i = lane; i < S * SLOT / 16; i += 32) ((uint4 *)(slots + (size_t)warp * S * SLOT))[i] = make_uint4(0u, 0u, 0u, 0u);
+        __syncwarp();
+    }
     auto copy_scales = [&](float *dst, const float *src) {
 #pragma unroll
         for (int k = 0; k < LK; k++) cp_async4z(smem_u32(dst + k * 32 + lane), src + row[k], (live[k] >> lane) & 1u);
@@ -688,7 +694,7 @@ __global__ void __launch_bounds__(AT_THREADS, OCC) paged_attend_kernel(const __g
     auto issue = [&](int stage) {
         const int g = lu / a.chunks;
         issued++;
-        full = a.kv.hd == HD;
+        full = true;
 #pragma unroll
         for (int k = 0; k < LK; k++) {
             const bool ok = pin[k] && pg[k] >= 0 && pg[k] < a.kv.n_pages;
