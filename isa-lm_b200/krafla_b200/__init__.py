@@ -468,6 +468,9 @@ class DevArray(DevBuf):
     def numel(self):
         return int(np.prod(self.shape, dtype=np.int64))
 
+    def dim(self):
+        return len(self.shape)
+
     def stride(self):
         return tuple(int(np.prod(self.shape[i + 1:], dtype=np.int64)) for i in range(len(self.shape)))
 
@@ -499,11 +502,13 @@ _F, _I, _W = _Types("float32"), _Types("int32"), _Types("int32", "uint32")
 _H, _B = _Types("float16"), _Types("int8")
 
 
+# The checks of the common case are a few cheap questions (a call's cost is the host's); what fails them is
+# looked at in full, to be taken after all or refused with its reason.
+
 def _rows(x, types, n, width, name):
-    """Rows of `width` values, [n, width] or [n, ...] with contiguous rows: the row stride.
-    (The first test settles the common case in a microsecond's third; the rest explains refusals.)"""
+    """Rows of `width` values, [n, width] or [n, ...] with contiguous rows: the row stride."""
     try:
-        if x.dtype in types.known and x.is_contiguous() and x.shape[0] == n and x.numel() == n * width:
+        if x.dtype in types.known and x.is_contiguous() and x.numel() == n * width and x.shape[0] == n:
             return width
     except (AttributeError, IndexError):
         pass
@@ -521,14 +526,7 @@ def _rows(x, types, n, width, name):
 
 
 def _flat(x, types, shape, name):
-    """A contiguous array of this shape: its address (None passes, as 0)."""
-    if x is None:
-        return 0
-    try:
-        if x.dtype in types.known and x.shape == shape and x.is_contiguous():
-            return x.data_ptr()
-    except AttributeError:
-        pass
+    """A contiguous array of this shape: its address."""
     types.check(x.dtype, name)
     s = x.shape
     if tuple(s) != shape:
@@ -539,6 +537,21 @@ def _flat(x, types, shape, name):
             raise _shape_error(f"{name} is not contiguous")
         at *= s[i]
     return x.data_ptr()
+
+
+def _vec(x, types, n, name):
+    """A contiguous array [n]: its address."""
+    try:
+        if x.dtype in types.known and x.numel() == n and x.is_contiguous() and x.dim() == 1:
+            return x.data_ptr()
+    except AttributeError:
+        pass
+    return _flat(x, types, (n,), name)
+
+
+def _opt(x, types, n, name):
+    """_vec, or 0 for None."""
+    return 0 if x is None else _vec(x, types, n, name)
 
 
 class _PagedKV(C.Structure):
@@ -605,8 +618,8 @@ class PagedKV:
         self.kv_type, self.n_seqs, self.head_dim = kv_type, ts[0], shape[3]
         self.n_kv_heads, self.page_size = shape[1], shape[2]
         self._keep = (k, v, kd, vd, table)
-        self._c = _PagedKV(_flat(k, types, shape, "k"), _flat(v, types, shape, "v"), _flat(kd, _F, shape[:3], "kd"),
-                           _flat(vd, _F, shape[:3], "vd"), _flat(table, _I, ts, "table"), ts[0], ts[1], shape[0],
+        self._c = _PagedKV(_flat(k, types, shape, "k"), _flat(v, types, shape, "v"), _flat(kd, _F, shape[:3], "kd") if kd is not None else None,
+                           _flat(vd, _F, shape[:3], "vd") if vd is not None else None, _flat(table, _I, ts, "table"), ts[0], ts[1], shape[0],
                            shape[2], shape[1], shape[3], kv_type)
         self._ref = C.byref(self._c)
         self._q = self.n_heads * self.head_dim
@@ -633,10 +646,16 @@ class PagedKV:
             pq = qkv.data_ptr()
             pk, pv = pq + 4 * self._q, pq + 4 * (self._q + kw)
         n_pos = cos.shape[0]
-        a = _APPEND.pack(pq, pk, pv, q_out.data_ptr(), ldq, ldk, ldv, _rows(q_out, _F, n, self._q, "q_out"),
-                         _flat(cos, _F, (n_pos, hd // 2), "cos"), _flat(sin, _F, (n_pos, hd // 2), "sin"),
-                         _flat(q_norm, _F, (hd,), "q_norm"), _flat(k_norm, _F, (hd,), "k_norm"),
-                         _flat(seqs, _I, (n,), "seqs"), _flat(pos, _I, (n,), "pos"), n, self.n_heads, n_pos, eps)
+        try:
+            fits = cos.shape == sin.shape == (n_pos, hd // 2) and cos.is_contiguous() and sin.is_contiguous()
+            fits = fits and cos.dtype in _F.known and sin.dtype in _F.known
+        except AttributeError:
+            fits = False
+        pc, ps = (cos.data_ptr(), sin.data_ptr()) if fits else (_flat(t, _F, (n_pos, hd // 2), m) for t, m in ((cos, "cos"), (sin, "sin")))
+        a = _APPEND.pack(pq, pk, pv, q_out.data_ptr(), ldq, ldk, ldv, _rows(q_out, _F, n, self._q, "q_out"), pc, ps,
+                         0 if q_norm is None else _vec(q_norm, _F, hd, "q_norm"),
+                         0 if k_norm is None else _vec(k_norm, _F, hd, "k_norm"),
+                         0 if seqs is None else _vec(seqs, _I, n, "seqs"), _vec(pos, _I, n, "pos"), n, self.n_heads, n_pos, eps)
         st = _lib.kc_paged_append_dev(self._ref, a, stream)
         if st:
             raise KraflaError(st, "append")
@@ -648,7 +667,7 @@ class PagedKV:
         n = q.shape[0]
         w = ws or self._ws
         a = _ATTEND.pack(q.data_ptr(), out.data_ptr(), _rows(q, _F, n, self._q, "q"), _rows(out, _F, n, self._q, "out"),
-                         _flat(lens, _I, (n,), "lens"), n, self.n_heads, window,
+                         _vec(lens, _I, n, "lens"), n, self.n_heads, window,
                          self.head_dim ** -0.5 if scale is None else scale, softcap, w.ptr, w.nbytes)
         st = _lib.kc_paged_attend_dev(self._ref, a, stream)
         if st:
@@ -682,10 +701,10 @@ def process_logits(out, logits, history=None, history_len=None, repeat=None, pre
     if bias_ids is not None:
         n_bias = bias_ids.shape[0]
     a = _LOGITS.pack(logits.data_ptr(), out.data_ptr(), _rows(logits, _F, n, v, "logits"), _rows(out, _F, n, v, "out"),
-                     hist, _flat(history_len, _I, (n,), "history_len"), ld_h, _flat(repeat, _F, (n,), "repeat"),
-                     _flat(presence, _F, (n,), "presence"), _flat(frequency, _F, (n,), "frequency"),
-                     _flat(bias_off, _I, (n + 1,), "bias_off"), _flat(bias_ids, _I, (n_bias,), "bias_ids"),
-                     _flat(bias_vals, _F, (n_bias,), "bias_vals"), bits, ld_m, n, v, cap, n_bias)
+                     hist, _opt(history_len, _I, n, "history_len"), ld_h, _opt(repeat, _F, n, "repeat"),
+                     _opt(presence, _F, n, "presence"), _opt(frequency, _F, n, "frequency"),
+                     _opt(bias_off, _I, n + 1, "bias_off"), _opt(bias_ids, _I, n_bias, "bias_ids"),
+                     _opt(bias_vals, _F, n_bias, "bias_vals"), bits, ld_m, n, v, cap, n_bias)
     st = lib().kc_logits_process_dev(a, stream)
     if st:
         raise KraflaError(st, "process logits")
