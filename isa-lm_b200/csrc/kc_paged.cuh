@@ -21,15 +21,26 @@ namespace kc {
 /* error bits of the serving operators' word */
 enum { SE_HIST = 1, SE_BIAS = 2, SE_LEN = 4, SE_PAGE = 8, SE_ROW = 16 };
 
+/* n / d for 0 <= n < 2^31 as the high half of n * mul, shifted: with 2^(s-1) < d <= 2^s, mul = 2^(31+s) / d rounded up
+ * is off by less than 2^s / d / 2^31 of itself, which no such n turns into a quotient */
+struct Divisor {
+    unsigned mul = 0;
+    int shift = 0;
+    explicit Divisor(int d = 1) {
+        int s = 0;
+        while ((1ll << s) < d) s++;
+        if (s) mul = (unsigned)(((1ull << (31 + s)) + (unsigned)d - 1) / (unsigned)d);
+        shift = s - 1;
+    }
+    __device__ __forceinline__ int operator()(int n) const { return mul ? (int)(__umulhi((unsigned)n, mul) >> shift) : n; }
+};
+
 struct PagedKV {
     uint8_t *k, *v;
     float *kd, *vd;
     const int *table;
     int n_seqs, ld_table, n_pages, page, n_kv, hd;
-    unsigned page_mul;
-    int page_shift;
-    /* p / page for 0 <= p < 2^31 */
-    __device__ __forceinline__ int page_of(int p) const { return page_mul ? (int)(__umulhi((unsigned)p, page_mul) >> page_shift) : p; }
+    Divisor page_of;             /* p / page */
 };
 
 /* ------------------------------------------------------------ append */
@@ -44,6 +55,8 @@ struct AppendArgs {
     float eps;
     const int *seqs, *pos;
     int rows, n_heads, n_pos;
+    int tasks;                   /* warps of a row */
+    Divisor row_of;              /* warp / tasks */
     unsigned *err;
 };
 
@@ -117,15 +130,14 @@ __device__ __forceinline__ void norm_rope(float (&x)[NV][4], bool norm, T inv, c
  * so that which side of a step's border a value falls on does not depend on
  * the order of the norm's sum; queries and wider caches use 32 bits. */
 template <int KV, int LPH, int NV>
-__global__ void __launch_bounds__(AP_THREADS) append_kernel(const AppendArgs a) {
+__global__ void __launch_bounds__(AP_THREADS, KV == KC_Q8_0 ? (NV == 1 ? 4 : 3) : (NV == 1 ? 5 : 4)) append_kernel(const AppendArgs a) {
     launch_next();
     stream_order();
     constexpr int NH = ap_heads<NV>(), HW = NH * (32 / LPH);   /* heads per lane group and per warp */
     const int lane = threadIdx.x % LPH, sub = threadIdx.x % 32 / LPH, hd = a.kv.hd;
-    const int tq = (a.n_heads + HW - 1) / HW, tk = (a.kv.n_kv + HW - 1) / HW, tasks = tq + 2 * tk;
-    const long long item = ((long long)blockIdx.x * AP_THREADS + threadIdx.x) / 32;
-    if (item >= (long long)a.rows * tasks) return;     /* (whole warps) */
-    const int row = (int)(item / tasks), task = (int)(item % tasks);
+    const int tq = (a.n_heads + HW - 1) / HW, tk = (a.kv.n_kv + HW - 1) / HW;
+    const int item = (int)(blockIdx.x * (AP_THREADS / 32) + threadIdx.x / 32), row = a.row_of(item), task = item - row * a.tasks;
+    if (row >= a.rows) return;                         /* (whole warps) */
     const bool isq = task < tq, isv = task >= tq + tk;
     const int h0 = HW * (isq ? task : (isv ? task - tq - tk : task - tq)) + sub, nh = isq ? a.n_heads : a.kv.n_kv;
     const float *src = isq ? a.q + row * a.ldq : (isv ? a.v + row * a.ldv : a.k + row * a.ldk);

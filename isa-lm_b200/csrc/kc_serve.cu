@@ -129,13 +129,8 @@ static int take_cache(const kc_paged_kv *kv, const ServeDev &d, PagedKV &o) {
         PTR(kv->kd, 4);
         PTR(kv->vd, 4);
     }
-    /* p / page_size as the high half of p * page_mul, shifted: with 2^(s-1) < page_size <= 2^s, page_mul =
-     * ceil(2^(31+s) / page_size) is off by less than 2^s / page_size / 2^31 of itself */
-    int s = 0;
-    while ((1ll << s) < kv->page_size) s++;
-    const unsigned mul = s ? (unsigned)(((1ull << (31 + s)) + kv->page_size - 1) / kv->page_size) : 0u;
     o = PagedKV{ (uint8_t *)kv->k, (uint8_t *)kv->v, kv->kd, kv->vd, kv->table, kv->n_seqs, kv->ld_table, kv->n_pages,
-                 kv->page_size, kv->n_kv_heads, kv->head_dim, mul, s - 1 };
+                 kv->page_size, kv->n_kv_heads, kv->head_dim, Divisor(kv->page_size) };
     return KC_OK;
 }
 
@@ -159,10 +154,12 @@ static cudaError_t launch_after(void (*kernel)(const A), unsigned gx, unsigned g
 /* ------------------------------------------------------------ append */
 
 template <int KV>
-static cudaError_t launch_append(const AppendArgs &a, cudaStream_t st) {
+static cudaError_t launch_append(AppendArgs &a, cudaStream_t st) {
     const int hd = a.kv.hd, lph = hd <= 32 ? 8 : (hd <= 64 ? 16 : 32);
     const int hw = (hd <= 128 ? ap_heads<1>() : ap_heads<2>()) * (32 / lph);
-    const long long warps = (long long)a.rows * ((a.n_heads + hw - 1) / hw + 2 * ((a.kv.n_kv + hw - 1) / hw));
+    a.tasks = (a.n_heads + hw - 1) / hw + 2 * ((a.kv.n_kv + hw - 1) / hw);
+    a.row_of = Divisor(a.tasks);
+    const long long warps = (long long)a.rows * a.tasks;
     const unsigned grid = (unsigned)((warps + AP_THREADS / 32 - 1) / (AP_THREADS / 32));
     return launch_after(lph == 8 ? append_kernel<KV, 8, 1>
                                  : (lph == 16 ? append_kernel<KV, 16, 1> : (hd <= 128 ? append_kernel<KV, 32, 1> : append_kernel<KV, 32, 2>)),
@@ -261,7 +258,7 @@ extern "C" int kc_paged_append_dev(const kc_paged_kv *kv, const kc_append_args *
         return refuse("a row stride is shorter than its row");
     if (!x->q_norm != !x->k_norm) return refuse("q_norm and k_norm come together");
     if (!(x->eps >= 0.0f) || std::isinf(x->eps)) return refuse("eps must be finite and not negative");
-    if ((double)x->rows * (x->n_heads + 2 * kv->n_kv_heads) > 2147483647.0) return refuse("too many rows in one call");
+    if ((double)x->rows * (x->n_heads + 2 * kv->n_kv_heads) > 2147483647.0 - 65536.0) return refuse("too many rows in one call");
     if (!x->seqs && x->rows > kv->n_seqs) return refuse("more rows than sequences, and no seqs");
     ServeDev d;
     rc = serve_device(d);
