@@ -26,7 +26,8 @@ enum { SE_HIST = 1, SE_BIAS = 2, SE_LEN = 4, SE_PAGE = 8, SE_ROW = 16 };
 struct Divisor {
     unsigned mul = 0;
     int shift = 0;
-    explicit Divisor(int d = 1) {
+    Divisor() = default;                               /* by 1 */
+    explicit Divisor(int d) {
         int s = 0;
         while ((1ll << s) < d) s++;
         if (s) mul = (unsigned)(((1ull << (31 + s)) + (unsigned)d - 1) / (unsigned)d);
@@ -450,80 +451,65 @@ __device__ __forceinline__ float4 over(float4 o, float l) {
     return make_float4(o.x * inv, o.y * inv, o.z * inv, o.w * inv);
 }
 
-/* The pieces of CTAs c0..c1 of one unit into the output: every four outputs by
- * as many threads as there are to spare, each of which takes a run of the
- * pieces, 16 requested at once; the runs meet in shared memory (`red`, 8 floats
- * a thread) in their order. */
+/* The pieces of CTAs c0..c1 of one unit into the output, AT_THREADS / runs
+ * times four outputs at a time: their parts of as many pieces as fit into the
+ * ring's memory are copied there at once, so that they take one latency and few
+ * instructions (which are fetched for the first time here); then every four
+ * outputs are summed by `runs` neighbouring lanes, which meet in shuffles. */
 template <int HD, int MT>
-__device__ __noinline__ void join_pieces(const AttendArgs &a, int b, int u, int c0, int c1, float *red) {
-    constexpr int HC = 8 * MT, PF = part_floats<HD, MT>(), UN = 16;
+__device__ __noinline__ void join_pieces(const AttendArgs &a, int b, int u, int c0, int c1, unsigned char *mem, int bytes) {
+    constexpr int HC = 8 * MT, PF = part_floats<HD, MT>(), ML = HC / 2;   /* 16-byte units of the maxima and sums */
+    const int tid = threadIdx.x;
     const int g = u / a.chunks, h0 = (u - g * a.chunks) * HC, nh = min(HC, a.group - h0), outs = nh * (HD / 4);
     int runs = 1;
     while (2 * runs * outs <= AT_THREADS) runs *= 2;
-    const int per = (c1 - c0 + runs) / runs;
-    for (int i0 = 0; i0 < outs; i0 += AT_THREADS / runs) {
-        const int idx = i0 + (int)threadIdx.x / runs, run = threadIdx.x % runs;
-        const int h = idx / (HD / 4), e = 4 * (idx - h * (HD / 4));
+    const int lots = AT_THREADS / runs, pitch = 16 * (lots + ML), fit = bytes / pitch, run = tid % runs;
+    for (int i0 = 0; i0 < outs; i0 += lots) {
+        const int idx = i0 + tid / runs, h = min(idx, outs - 1) / (HD / 4), e = 4 * (idx - h * (HD / 4));
         float M = -INFINITY, L = 0.0f;
         float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-        if (idx < outs) {
-            const int k1 = min(c0 + (run + 1) * per, c1 + 1);
-            for (int k0 = c0 + run * per; k0 < k1; k0 += UN) {
-                float m[UN], l[UN];
-                float4 t[UN];
-#pragma unroll
-                for (int i = 0; i < UN; i++) {
-                    m[i] = -INFINITY;
-                    l[i] = 0.0f;
-                    t[i] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-                    if (k0 + i < k1) {
-                        const float *p = a.part + ((size_t)2 * (k0 + i) + (k0 + i == c0 ? 1 : 0)) * PF;
-                        m[i] = __ldcg(p + HC * HD + h);
-                        l[i] = __ldcg(p + HC * HD + HC + h);
-                        t[i] = __ldcg((const float4 *)(p + h * HD + e));
-                    }
-                }
-                float mn = M;
-#pragma unroll
-                for (int i = 0; i < UN; i++) mn = fmaxf(mn, m[i]);
-                const float base = mn == -INFINITY ? 0.0f : mn, f0 = ex2(M - base);
-                M = mn;
-                L *= f0;
-                o = make_float4(o.x * f0, o.y * f0, o.z * f0, o.w * f0);
-#pragma unroll
-                for (int i = 0; i < UN; i++) {
-                    const float f = ex2(m[i] - base);
-                    L += f * l[i];
-                    o.x += f * t[i].x;
-                    o.y += f * t[i].y;
-                    o.z += f * t[i].z;
-                    o.w += f * t[i].w;
-                }
+        for (int k0 = c0; k0 <= c1; k0 += fit) {
+            const int n = min(fit, c1 - k0 + 1);
+            const float *p = a.part + ((size_t)2 * k0 + (k0 == c0 ? 1 : 0)) * PF;
+            uint32_t to = smem_u32(mem) + 16 * tid;
+            for (int j = 0; j < n; j++) {
+                if (tid < lots && i0 + tid < outs) cp_async16s(to, p + 4 * (i0 + tid));
+                if (tid < ML) cp_async16s(to + 16 * lots, p + HC * HD + 4 * tid);
+                p += (j == 0 && k0 == c0 ? 1 : 2) * PF;
+                to += pitch;
             }
+            cp_async_commit();
+            cp_async_wait_all();
+            __syncthreads();
+            const unsigned char *at = mem + run * pitch, *end = mem + n * pitch;
+            const float *ml = (const float *)(at + 16 * lots) + h;
+            float mn = M;
+            for (int j = run; j < n; j += runs) mn = fmaxf(mn, *(const float *)((const unsigned char *)ml + (j - run) * pitch));
+            const float base = mn == -INFINITY ? 0.0f : mn, f0 = ex2(M - base);
+            M = mn;
+            L *= f0;
+            o = make_float4(o.x * f0, o.y * f0, o.z * f0, o.w * f0);
+#pragma unroll 4
+            for (; at < end; at += runs * pitch) {
+                ml = (const float *)(at + 16 * lots) + h;
+                const float f = ex2(ml[0] - base);
+                const float4 t = *(const float4 *)(at + 16 * (idx - i0));
+                L += f * ml[HC];
+                o.x += f * t.x;
+                o.y += f * t.y;
+                o.z += f * t.z;
+                o.w += f * t.w;
+            }
+            __syncthreads();
         }
-        if (runs > 1) {
-            __syncthreads();
-            float *w = red + 8 * threadIdx.x;
-            *(float4 *)w = o;
-            w[4] = M;
-            w[5] = L;
-            __syncthreads();
-            if (run == 0) {
-                float mn = M;
-                for (int i = 1; i < runs; i++) mn = fmaxf(mn, w[8 * i + 4]);
-                const float base = mn == -INFINITY ? 0.0f : mn, f0 = ex2(M - base);
-                L *= f0;
-                o = make_float4(o.x * f0, o.y * f0, o.z * f0, o.w * f0);
-                for (int i = 1; i < runs; i++) {
-                    const float f = ex2(w[8 * i + 4] - base);
-                    const float4 t = *(const float4 *)(w + 8 * i);
-                    L += f * w[8 * i + 5];
-                    o.x += f * t.x;
-                    o.y += f * t.y;
-                    o.z += f * t.z;
-                    o.w += f * t.w;
-                }
-            }
+        for (int d = 1; d < runs; d *= 2) {
+            const float m2 = __shfl_xor_sync(0xffffffffu, M, d), mn = fmaxf(M, m2), base = mn == -INFINITY ? 0.0f : mn;
+            const float f1 = ex2(M - base), f2 = ex2(m2 - base);
+            /* the lower run first, on both sides */
+            auto both = [&](float v) { const float w = __shfl_xor_sync(0xffffffffu, v, d); return run & d ? f2 * w + f1 * v : f1 * v + f2 * w; };
+            L = both(L);
+            o = make_float4(both(o.x), both(o.y), both(o.z), both(o.w));
+            M = mn;
         }
         if (idx < outs && run == 0 && e < a.kv.hd)
             *(float4 *)(a.out + b * a.ldo + (size_t)(g * a.group + h0 + h) * a.kv.hd + e) = over(o, L);
@@ -1282,8 +1268,8 @@ __global__ void __launch_bounds__(AT_THREADS, OCC) paged_attend_kernel(const __g
     __syncthreads();
     for (int k = 0; k < 2; k++)
         if (s_join[k][0]) {
-            join_pieces<HD, MT>(a, s_join[k][2], s_join[k][3], s_join[k][1], s_join[k][0] - 1, comb);
-            __syncthreads();                           /* (comb is the second's) */
+            join_pieces<HD, MT>(a, s_join[k][2], s_join[k][3], s_join[k][1], s_join[k][0] - 1, slots, AT_WARPS * S * SLOT);
+            __syncthreads();
         }
 }
 
