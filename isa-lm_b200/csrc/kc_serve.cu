@@ -362,8 +362,9 @@ extern "C" int kc_paged_attend_dev(const kc_paged_kv *kv, const kc_attend_args *
     a.inv_softcap = x->softcap > 0.0f ? 1.0f / x->softcap : 0.0f;
     a.near = (v->tile - 1) / kv->page_size + 2 <= 32;
     a.unit_cost = AT_UNIT_COST;
-    /* measured: a piece of 16 heads of 128 (8 KB) is joined in 0.28 of a quantum's time, one of 4 heads of 64 in
-     * 0.035; one sequence of 8192 positions, 16 heads to a KV head, takes 61 us in the smallest shares, 31 us so */
+    /* measured: a piece of 16 heads of 128 (8 KB) is joined in about 0.28 of a quantum's time, one of 4 heads of 64 in
+     * 0.035; one sequence of 8192 positions, 16 heads to a KV head, takes 53 us in the smallest shares, 25 us so
+     * (27 with half or twice the cost) */
     a.join_cost = 1.4e-4f * (float)(std::min(a.group, v->heads) * kv->head_dim);
     a.grid_inv = ~0ull / (unsigned)ctas + 1;
     a.count = (unsigned *)x->ws;
