@@ -619,34 +619,41 @@ __global__ void __launch_bounds__(AT_THREADS, OCC) paged_attend_kernel(const __g
     const int nq0 = nq;
     const long long ubase0 = ubase;
     const int prow = lane & (RW - 1);
-    int pg[LK], pslot[LK];
-    bool pin[LK];
+    int ql = nq - lq, p0 = first + (lq * AT_WARPS + warp) * TP, lg = lu / a.chunks;   /* quanta left, the tile's first position, KV head */
     /* 32 entries of the sequence's table row from tb0 on, an entry a lane; a tile's are among them unless
      * pages are so short that it may span more (a.near 0), where each row's entry is loaded */
     int tab = -1, tb0 = 0, tbn = 0;
-    auto look = [&]() {                                /* pages of the lane's rows of the loader's tile */
-        const int p0 = first + (lq * AT_WARPS + warp) * TP;
-        if (a.near && p0 < len) {
-            const int i0 = a.kv.page_of(p0), i1 = min(p0 + TP, len) - 1;
-            if (i0 < tb0 || i1 >= tbn) {
+    unsigned live[LK], row[LK];                        /* of the loader's tile: rows that are there, and where */
+    bool full;                                         /* all of them */
+    auto look = [&]() {
+        const int n = len - p0;                        /* positions of the tile, 0 or fewer: none */
+        full = false;
+#pragma unroll
+        for (int k = 0; k < LK; k++) live[k] = row[k] = 0u;
+        if (n <= 0) return;
+        if (a.near) {
+            const int i0 = a.kv.page_of(p0);
+            if (i0 < tb0 || p0 + min(n, TP) > tbn) {
                 tb0 = i0;
                 tbn = (int)min((long long)(tb0 + 32) * a.kv.page, (long long)INT_MAX);
                 tab = tb0 + lane < a.kv.ld_table ? __ldg(a.kv.table + (size_t)lb * a.kv.ld_table + tb0 + lane) : -1;
             }
         }
+        full = true;
 #pragma unroll
         for (int k = 0; k < LK; k++) {
-            const int p = p0 + k * RW + prow;
-            pin[k] = p < len;
-            const int pi = pin[k] ? a.kv.page_of(p) : tb0;
-            pslot[k] = p - pi * a.kv.page;
-            if (a.near) pg[k] = __shfl_sync(0xffffffffu, tab, (pi - tb0) & 31);
-            else pg[k] = pin[k] ? __ldg(a.kv.table + (size_t)lb * a.kv.ld_table + pi) : -1;
+            const int o = k * RW + prow, pi = a.kv.page_of(p0 + o);
+            const bool in = o < n;
+            int pg = __shfl_sync(0xffffffffu, tab, (pi - tb0) & 31);
+            if (!a.near) pg = in ? __ldg(a.kv.table + (size_t)lb * a.kv.ld_table + pi) : -1;
+            const bool ok = in && (unsigned)pg < (unsigned)a.kv.n_pages;
+            if (in && !ok) atomicOr(a.err, (unsigned)SE_PAGE);
+            live[k] = __ballot_sync(0xffffffffu, ok) & (unsigned)((1ull << RW) - 1);
+            full &= live[k] == (unsigned)((1ull << RW) - 1);
+            if (ok) row[k] = ((unsigned)pg * a.kv.n_kv + lg) * a.kv.page + (p0 + o - pi * a.kv.page);
         }
     };
     enum { LAST_OF_UNIT = 1 << 28, LAST_OF_SHARE = 1 << 29 };
-    unsigned live[LK], row[LK];                        /* of the loader's tile: rows that are there, and where */
-    bool full;                                         /* all of them */
     /* Rows start at different bank groups, by an exclusive or of the 16-byte chunk's number with swz(row): for
      * row-per-lane reads of eight rows (ldmatrix, and f32 V) the row's low bits, or the next ones where two rows
      * share 128 bytes; for f32 K, read by four lanes a row and eight rows in turn, the low bits reversed. */
@@ -691,35 +698,26 @@ __global__ void __launch_bounds__(AT_THREADS, OCC) paged_attend_kernel(const __g
     };
     int issued = 0;
     auto issue = [&](int stage) {
-        const int g = lu / a.chunks;
         issued++;
-        full = true;
-#pragma unroll
-        for (int k = 0; k < LK; k++) {
-            const bool ok = pin[k] && pg[k] >= 0 && pg[k] < a.kv.n_pages;
-            if (pin[k] && !ok) atomicOr(a.err, (unsigned)SE_PAGE);
-            live[k] = __ballot_sync(0xffffffffu, ok) & (unsigned)((1ull << RW) - 1);
-            full &= live[k] == (unsigned)((1ull << RW) - 1);
-            row[k] = ok ? (unsigned)(((size_t)pg[k] * a.kv.n_kv + g) * a.kv.page + pslot[k]) : 0u;
-        }
-        copy_rows(ring_s + stage * SLOT);
-        if constexpr (KV == KC_Q8_0) {
-            copy_scales(scl + stage * SCALES, a.kv.kd);
-            copy_scales(scl + stage * SCALES + TP, a.kv.vd);
+        if (live[0] | live[LK - 1]) {
+            copy_rows(ring_s + stage * SLOT);
+            if constexpr (KV == KC_Q8_0) {
+                copy_scales(scl + stage * SCALES, a.kv.kd);
+                copy_scales(scl + stage * SCALES + TP, a.kv.vd);
+            }
         }
         if (lane == 0) {
-            const bool eu = lq == nq - 1;
-            const int f = (eu ? LAST_OF_UNIT : 0) | (left <= (eu ? 1 + W : 1) ? LAST_OF_SHARE : 0);
+            const int f = (ql == 1 ? LAST_OF_UNIT : 0) | (left <= (ql == 1 ? 1 + W : 1) ? LAST_OF_SHARE : 0);
             info[stage] = make_int4(lb, lu | f, (int)live[0], LK > 1 ? (int)live[LK - 1] : 0);
         }
     };
     auto advance = [&]() {
-        const bool eu = lq == nq - 1;
-        left -= eu ? 1 + W : 1;
+        left -= ql == 1 ? 1 + W : 1;
         if (left <= 0) return;
-        if (eu) {
+        if (--ql > 0) {
+            p0 += QP;
+        } else {
             ubase += nq + W;
-            lq = 0;
             if (++lu == U) {
                 lu = 0;
                 do {
@@ -732,8 +730,9 @@ __global__ void __launch_bounds__(AT_THREADS, OCC) paged_attend_kernel(const __g
                 } while (nq == 0);
                 tbn = 0;                               /* another table row */
             }
-        } else {
-            lq++;
+            ql = nq;
+            p0 = first + warp * TP;
+            lg = lu / a.chunks;
         }
         look();
     };
