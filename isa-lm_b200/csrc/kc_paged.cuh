@@ -379,13 +379,6 @@ __device__ __forceinline__ void mma_s8(int (&c)[4], unsigned a0, unsigned a2, un
 }
 
 __device__ __forceinline__ unsigned h2u(__half2 h) { return *(unsigned *)&h; }
-/* two floats as f16 pairs: the high parts, and what they leave */
-__device__ __forceinline__ void split_f16(float a, float b, unsigned &hi, unsigned &lo) {
-    const __half2 h = __floats2half2_rn(a, b);
-    const float2 f = __half22float2(h);
-    hi = h2u(h);
-    lo = h2u(__floats2half2_rn(a - f.x, b - f.y));
-}
 /* a float as two tf32: the nearest above or below, and what it leaves (|.| <= 2^-10 of it, of which
  * 11 bits are kept); integer operations, since the conversion instruction runs at a fraction of their rate */
 __device__ __forceinline__ void split_tf32(float a, unsigned &hi, unsigned &lo) {
@@ -412,16 +405,21 @@ __device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
         : "=f"(r.x), "=f"(r.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
     return r;
 }
-__device__ __forceinline__ float2 mul2(float2 a, float b) {
+__device__ __forceinline__ float2 mul2(float2 a, float2 b) {
     float2 r;
-    asm("{\n .reg .b64 x, y, z;\n mov.b64 x, {%2, %3};\n mov.b64 y, {%4, %4};\n mul.rn.f32x2 z, x, y;\n mov.b64 {%0, %1}, z;\n}"
-        : "=f"(r.x), "=f"(r.y) : "f"(a.x), "f"(a.y), "f"(b));
+    asm("{\n .reg .b64 x, y, z;\n mov.b64 x, {%2, %3};\n mov.b64 y, {%4, %5};\n mul.rn.f32x2 z, x, y;\n mov.b64 {%0, %1}, z;\n}"
+        : "=f"(r.x), "=f"(r.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
     return r;
 }
-/* o = o * corr + (rows 0-7 and 8-15 of a product) */
-__device__ __forceinline__ void carry(float2 &o, float2 corr, const float (&d)[4]) {
-    o = fma2(o, corr, add2(make_float2(d[0], d[1]), make_float2(d[2], d[3])));
+/* two floats as f16 pairs: the high parts, and what they leave */
+__device__ __forceinline__ void split_f16(float2 a, unsigned &hi, unsigned &lo) {
+    const __half2 h = __floats2half2_rn(a.x, a.y);
+    const float2 r = fma2(__half22float2(h), make_float2(-1.0f, -1.0f), a);
+    hi = h2u(h);
+    lo = h2u(__floats2half2_rn(r.x, r.y));
 }
+/* rows 0-7 and 8-15 of a product together */
+__device__ __forceinline__ float2 halves(const float (&d)[4]) { return add2(make_float2(d[0], d[1]), make_float2(d[2], d[3])); }
 
 /* Positions [first, len) of sequence b, quanta of QP positions, clamped to what the table can hold. */
 __device__ __forceinline__ int seq_span(const AttendArgs &a, int b, int &first, bool &bad) {
@@ -807,7 +805,7 @@ __global__ void __launch_bounds__(AT_THREADS, OCC) paged_attend_kernel(const __g
                     qc[mt] = __uint_as_float((unsigned)(127 - 12 + ex) << 23) * post;
 #pragma unroll
                     for (int i = 0; i < HD / 8; i++)
-                        split_f16(x[2 * i] * up, x[2 * i + 1] * up, qf[mt][2 * i], qf[mt][2 * i + 1]);
+                        split_f16(make_float2(x[2 * i] * up, x[2 * i + 1] * up), qf[mt][2 * i], qf[mt][2 * i + 1]);
                 } else {
                     /* the query head quantized as a cache row is (ops/ops.c:229-233) */
                     const bool tiny = mx < 1e-30f;
@@ -830,7 +828,7 @@ __global__ void __launch_bounds__(AT_THREADS, OCC) paged_attend_kernel(const __g
     };
 
     /* the scores of the tile of TP positions in ring slot `stage`: of head row r, positions 8 nt + 2 c and + 1 */
-    float s[MT][NT][2];
+    float2 s[MT][NT];
     auto scores = [&](int stage) {
         const uint32_t sk = ring_s + stage * SLOT;
         if constexpr (KV == KC_F16) {
@@ -855,8 +853,7 @@ __global__ void __launch_bounds__(AT_THREADS, OCC) paged_attend_kernel(const __g
             for (int mt = 0; mt < MT; mt++)
 #pragma unroll
                 for (int nt = 0; nt < NT; nt++) {
-                    s[mt][nt][0] = d[mt][nt][0] + d[mt][nt][2];
-                    s[mt][nt][1] = d[mt][nt][1] + d[mt][nt][3];
+                    s[mt][nt] = halves(d[mt][nt]);
                 }
         } else if constexpr (KV == KC_F32) {
             float dh[MT][NT][4], dl[MT][NT][4];
@@ -890,8 +887,7 @@ __global__ void __launch_bounds__(AT_THREADS, OCC) paged_attend_kernel(const __g
             for (int mt = 0; mt < MT; mt++)
 #pragma unroll
                 for (int nt = 0; nt < NT; nt++) {
-                    s[mt][nt][0] = (dh[mt][nt][0] + dh[mt][nt][2]) + (dl[mt][nt][0] + dl[mt][nt][2]);
-                    s[mt][nt][1] = (dh[mt][nt][1] + dh[mt][nt][3]) + (dl[mt][nt][1] + dl[mt][nt][3]);
+                    s[mt][nt] = add2(halves(dh[mt][nt]), halves(dl[mt][nt]));
                 }
         } else {
             int d[MT][NT][4];                          /* from 1.5 * 2^23: the sums come out as its floats */
@@ -915,8 +911,9 @@ __global__ void __launch_bounds__(AT_THREADS, OCC) paged_attend_kernel(const __g
                 const float2 e = *(const float2 *)(kd + nt * 8 + 2 * c);
 #pragma unroll
                 for (int mt = 0; mt < MT; mt++) {
-                    s[mt][nt][0] = (__int_as_float(d[mt][nt][0]) - 12582912.0f) * e.x;
-                    s[mt][nt][1] = (__int_as_float(d[mt][nt][1]) - 12582912.0f) * e.y;
+                    s[mt][nt] = mul2(add2(make_float2(__int_as_float(d[mt][nt][0]), __int_as_float(d[mt][nt][1])),
+                                          make_float2(-12582912.0f, -12582912.0f)),
+                                     e);
                 }
             }
         }
@@ -948,35 +945,33 @@ __global__ void __launch_bounds__(AT_THREADS, OCC) paged_attend_kernel(const __g
             if (a.softcap > 0.0f) {
                 qm = a.softcap * LOG2E;
 #pragma unroll
-                for (int nt = 0; nt < NT; nt++)
-#pragma unroll
-                    for (int i = 0; i < 2; i++) s[mt][nt][i] = tanhf(s[mt][nt][i] * qc[mt]);
+                for (int nt = 0; nt < NT; nt++) s[mt][nt] = make_float2(tanhf(s[mt][nt].x * qc[mt]), tanhf(s[mt][nt].y * qc[mt]));
             }
             if (!all) {
 #pragma unroll
-                for (int nt = 0; nt < NT; nt++)
-#pragma unroll
-                    for (int i = 0; i < 2; i++)
-                        if (!((live[nt * 8 / RW] >> ((nt * 8) % RW + 2 * c + i)) & 1u)) s[mt][nt][i] = -INFINITY;
+                for (int nt = 0; nt < NT; nt++) {
+                    const unsigned here = live[nt * 8 / RW] >> ((nt * 8) % RW + 2 * c);
+                    if (!(here & 1u)) s[mt][nt].x = -INFINITY;
+                    if (!(here & 2u)) s[mt][nt].y = -INFINITY;
+                }
             }
-            float mx = fmaxf(s[mt][0][0], s[mt][0][1]);
+            float mx = fmaxf(s[mt][0].x, s[mt][0].y);
 #pragma unroll
-            for (int nt = 1; nt < NT; nt++) mx = fmaxf(mx, fmaxf(s[mt][nt][0], s[mt][nt][1]));
+            for (int nt = 1; nt < NT; nt++) mx = fmaxf(mx, fmaxf(s[mt][nt].x, s[mt][nt].y));
             mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
             mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
             const float mn = fmaxf(m[mt], mx * qm), base = mn == -INFINITY ? 0.0f : mn, add = lift - base;
             const float cr = ex2(m[mt] - base);
             corr[mt] = make_float2(cr, cr);
             m[mt] = mn;
-            float sum = 0.0f;
+            float2 both = make_float2(0.0f, 0.0f);
 #pragma unroll
-            for (int nt = 0; nt < NT; nt++)
-#pragma unroll
-                for (int i = 0; i < 2; i++) {
-                    const float p = ex2(fmaf(s[mt][nt][i], qm, add));
-                    s[mt][nt][i] = p;
-                    sum += p;
-                }
+            for (int nt = 0; nt < NT; nt++) {
+                const float2 x = fma2(s[mt][nt], make_float2(qm, qm), make_float2(add, add));
+                s[mt][nt] = make_float2(ex2(x.x), ex2(x.y));
+                both = nt ? add2(both, s[mt][nt]) : s[mt][nt];
+            }
+            const float sum = both.x + both.y;
             l[mt] = l[mt] * cr + sum * back;
         }
     };
@@ -990,7 +985,7 @@ __global__ void __launch_bounds__(AT_THREADS, OCC) paged_attend_kernel(const __g
             for (int mt = 0; mt < MT; mt++)
 #pragma unroll
                 for (int nt = 0; nt < NT; nt++)
-                    split_f16(s[mt][nt][0], s[mt][nt][1], w[mt][nt >> 1][2 * (nt & 1)], w[mt][nt >> 1][2 * (nt & 1) + 1]);
+                    split_f16(s[mt][nt], w[mt][nt >> 1][2 * (nt & 1)], w[mt][nt >> 1][2 * (nt & 1) + 1]);
             const uint32_t vb = sv + (lane & 15) * PITCH + (((lane >> 4) ^ (lane & 7)) << 4);
 #pragma unroll
             for (int jj = 0; jj < HD / 16; jj++) {
@@ -1012,8 +1007,8 @@ __global__ void __launch_bounds__(AT_THREADS, OCC) paged_attend_kernel(const __g
                 }
 #pragma unroll
                 for (int mt = 0; mt < MT; mt++) {
-                    carry(acc[mt][2 * jj], corr[mt], d[mt][0]);
-                    carry(acc[mt][2 * jj + 1], corr[mt], d[mt][1]);
+                    acc[mt][2 * jj] = fma2(acc[mt][2 * jj], corr[mt], halves(d[mt][0]));
+                    acc[mt][2 * jj + 1] = fma2(acc[mt][2 * jj + 1], corr[mt], halves(d[mt][1]));
                 }
             }
         } else if constexpr (KV == KC_F32) {
@@ -1022,8 +1017,8 @@ __global__ void __launch_bounds__(AT_THREADS, OCC) paged_attend_kernel(const __g
             for (int mt = 0; mt < MT; mt++)
 #pragma unroll
                 for (int nt = 0; nt < NT; nt++) {
-                    split_tf32(s[mt][nt][0], w[mt][nt][0], w[mt][nt][1]);
-                    split_tf32(s[mt][nt][1], w[mt][nt][2], w[mt][nt][3]);
+                    split_tf32(s[mt][nt].x, w[mt][nt][0], w[mt][nt][1]);
+                    split_tf32(s[mt][nt].y, w[mt][nt][2], w[mt][nt][3]);
                 }
             const uint32_t v0 = sv + (2 * c) * PITCH + ((r ^ (2 * c)) << 4), v1 = sv + (2 * c + 1) * PITCH + ((r ^ (2 * c + 1)) << 4);
 #pragma unroll
@@ -1050,7 +1045,7 @@ __global__ void __launch_bounds__(AT_THREADS, OCC) paged_attend_kernel(const __g
 #pragma unroll
                 for (int mt = 0; mt < MT; mt++)
 #pragma unroll
-                    for (int i = 0; i < 4; i++) carry(acc[mt][4 * j + i], corr[mt], d[mt][i]);
+                    for (int i = 0; i < 4; i++) acc[mt][4 * j + i] = fma2(acc[mt][4 * j + i], corr[mt], halves(d[mt][i]));
             }
         } else {
             constexpr int KS = TP / 16;
@@ -1061,7 +1056,7 @@ __global__ void __launch_bounds__(AT_THREADS, OCC) paged_attend_kernel(const __g
                 const float2 e = *(const float2 *)(vd + nt * 8 + 2 * c);
 #pragma unroll
                 for (int mt = 0; mt < MT; mt++)
-                    split_f16(s[mt][nt][0] * e.x, s[mt][nt][1] * e.y, w[mt][nt >> 1][2 * (nt & 1)],
+                    split_f16(mul2(s[mt][nt], e), w[mt][nt >> 1][2 * (nt & 1)],
                               w[mt][nt >> 1][2 * (nt & 1) + 1]);
             }
             const uint32_t vb = sv + (lane & 15) * PITCH + (((lane >> 4) ^ swz(SWV, lane & 7)) << 4);
@@ -1110,9 +1105,7 @@ __global__ void __launch_bounds__(AT_THREADS, OCC) paged_attend_kernel(const __g
                 for (int mt = 0; mt < MT; mt++)
 #pragma unroll
                     for (int k = 0; k < 4; k++)
-                        acc[mt][4 * jj + k] = fma2(acc[mt][4 * jj + k], corr[mt],
-                                                   mul2(add2(make_float2(d[mt][k][0], d[mt][k][1]),
-                                                             make_float2(d[mt][k][2], d[mt][k][3])), back));
+                        acc[mt][4 * jj + k] = fma2(acc[mt][4 * jj + k], corr[mt], mul2(halves(d[mt][k]), make_float2(back, back)));
             }
         }
     };
