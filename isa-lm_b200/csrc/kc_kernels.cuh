@@ -54,6 +54,14 @@ struct LoopState {
  * wait in turn. */
 __device__ __forceinline__ void stream_order() { cudaGridDependencySynchronize(); }
 __device__ __forceinline__ void launch_next() { cudaTriggerProgrammaticLaunchCompletion(); }
+/* What the work before may have written is not read-only for such a kernel, whose
+ * life begins before that work's end: plain loads, and for what is read once this
+ * one, which stays behind stream_order. */
+__device__ __forceinline__ float4 load_once(const float *p) {
+    float4 v;
+    asm volatile("ld.global.cs.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "l"(p) : "memory");
+    return v;
+}
 
 __device__ __forceinline__ float warp_sum(float v) {
 #pragma unroll

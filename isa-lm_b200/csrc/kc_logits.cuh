@@ -13,7 +13,7 @@
  * shared memory which history tokens and biases fall into its stretch while the
  * logits arrive, writes them through the mask, and then goes over the few that
  * are touched, listed once each, whose values it makes meanwhile. 64 rows of
- * 128256: 11.9 us with a mask alone, 16.8 us with 2048 tokens of history and 100
+ * 128256: 12.0 us with a mask alone, 17.0 us with 2048 tokens of history and 100
  * biases each, from memory (floor 10.4). Measured beside it and not taken: every logit looking
  * at its own counter, 1.9 times the instructions; stretches of 16384 logits that
  * share one look at the history, the same time, since one wave of CTAs then
@@ -74,19 +74,19 @@ __global__ void __launch_bounds__(LG_THREADS, 5) logits_kernel(const LogitsArgs 
     const int *h = a.hist + row * a.ld_hist;
     float rep = 1.0f, pres = 0.0f, freq = 0.0f;
     if constexpr (BIAS) {
-        b0 = __ldg(a.bias_off + row);
-        b1 = __ldg(a.bias_off + row + 1);
+        b0 = a.bias_off[row];
+        b1 = a.bias_off[row + 1];
     }
     if constexpr (HIST) {
-        n = a.hist_len ? __ldg(a.hist_len + row) : a.hist_cap;
+        n = a.hist_len ? a.hist_len[row] : a.hist_cap;
 #pragma unroll
         for (int k = 0; k < NH; k++) {
             const int i = tid + k * LG_THREADS;
-            t0[k] = i < a.hist_cap ? __ldg(h + i) : -1;
+            t0[k] = i < a.hist_cap ? h[i] : -1;
         }
-        if (a.repeat) rep = __ldg(a.repeat + row);
-        if (a.presence) pres = __ldg(a.presence + row);
-        if (a.frequency) freq = __ldg(a.frequency + row);
+        if (a.repeat) rep = a.repeat[row];
+        if (a.presence) pres = a.presence[row];
+        if (a.frequency) freq = a.frequency[row];
     }
     float4 z[LG_VEC];
     uint32_t mw[LG_VEC];                               /* the vectors' mask bits from bit 0 on */
@@ -94,8 +94,8 @@ __global__ void __launch_bounds__(LG_THREADS, 5) logits_kernel(const LogitsArgs 
 #pragma unroll
         for (int k = 0; k < LG_VEC; k++) {
             const int e = e0 + 4 * (tid + k * LG_THREADS);
-            z[k] = __ldcs((const float4 *)(in + e));
-            mw[k] = mask ? __ldg(mask + (e >> 5)) >> (e & 31) : 0xfu;
+            z[k] = load_once(in + e);
+            mw[k] = mask ? mask[e >> 5] >> (e & 31) : 0xfu;
         }
     } else {
 #pragma unroll
@@ -105,7 +105,7 @@ __global__ void __launch_bounds__(LG_THREADS, 5) logits_kernel(const LogitsArgs 
             mw[k] = 0xfu;
             if (e + 3 < 0 || e >= V) continue;
             if (e >= 0 && e <= V - 4) {
-                z[k] = __ldcs((const float4 *)(in + e));
+                z[k] = load_once(in + e);
             } else {
                 if (e >= 0) z[k].x = in[e];
                 if (e + 1 >= 0 && e + 1 < V) z[k].y = in[e + 1];
@@ -114,9 +114,9 @@ __global__ void __launch_bounds__(LG_THREADS, 5) logits_kernel(const LogitsArgs 
             }
             if (mask) {
                 uint32_t wa = 0xffffffffu, wb;         /* (elements below 0 are no logits: any bit will do) */
-                if (e >= 0) wa = __ldg(mask + (e >> 5));
+                if (e >= 0) wa = mask[e >> 5];
                 wb = wa;
-                if ((e + 3) >> 5 != e >> 5 && (e + 3) >> 5 <= (V - 1) >> 5) wb = __ldg(mask + ((e + 3) >> 5));
+                if ((e + 3) >> 5 != e >> 5 && (e + 3) >> 5 <= (V - 1) >> 5) wb = mask[(e + 3) >> 5];
                 mw[k] = __funnelshift_r(wa, wb, (unsigned)e & 31u);
             }
         }
@@ -127,7 +127,7 @@ __global__ void __launch_bounds__(LG_THREADS, 5) logits_kernel(const LogitsArgs 
                 if (tid == 0 && blockIdx.y == 0) atomicOr(a.err, 2u);
                 b0 = b1 = 0;
             }
-            if (b0 + tid < b1) i0 = __ldg(a.bias_ids + b0 + tid);
+            if (b0 + tid < b1) i0 = a.bias_ids[b0 + tid];
         }
         for (int i = tid; i < LG_CHUNK / 4; i += LG_THREADS) ((uint4 *)s_word)[i] = make_uint4(0u, 0u, 0u, 0u);
         if (tid == 0) s_n = 0;
@@ -145,7 +145,7 @@ __global__ void __launch_bounds__(LG_THREADS, 5) logits_kernel(const LogitsArgs 
 #pragma unroll
             for (int k = 0; k < NH; k++)
                 if (tid + k * LG_THREADS < n) seen(t0[k]);
-            for (int i = tid + NH * LG_THREADS; i < n; i += LG_THREADS) seen(__ldg(h + i));
+            for (int i = tid + NH * LG_THREADS; i < n; i += LG_THREADS) seen(h[i]);
         }
         if constexpr (BIAS) {
             constexpr int SH = HIST ? 16 : 0;
@@ -163,7 +163,7 @@ __global__ void __launch_bounds__(LG_THREADS, 5) logits_kernel(const LogitsArgs 
                 }
             };
             if (i0 >= 0) named(i0, tid);
-            for (int i = tid + LG_THREADS; i < b1 - b0; i += LG_THREADS) named(__ldg(a.bias_ids + b0 + i), i);
+            for (int i = tid + LG_THREADS; i < b1 - b0; i += LG_THREADS) named(a.bias_ids[b0 + i], i);
         }
     }
     /* the few that are touched and allowed: their values are made while the others are written. (Where `out` is
@@ -175,8 +175,8 @@ __global__ void __launch_bounds__(LG_THREADS, 5) logits_kernel(const LogitsArgs 
         const uint32_t v = s_word[o];
         const int c = HIST && BIAS ? (int)(v & 0xffffu) : (HIST ? (int)v : 0);
         const int b = HIST && BIAS ? (int)(v >> 16) - 1 : (BIAS ? (int)v - 1 : -1);
-        const uint32_t w = mask ? __ldg(mask + (t >> 5)) : 0xffffffffu;
-        const float bv = b >= 0 ? __ldg(a.bias_vals + b0 + b) : 0.0f;
+        const uint32_t w = mask ? mask[t >> 5] : 0xffffffffu;
+        const float bv = b >= 0 ? a.bias_vals[b0 + b] : 0.0f;
         tx = ((volatile const float *)in)[t];
         to = (w >> (t & 31)) & 1u ? t : -1;
         if (c > 0) {

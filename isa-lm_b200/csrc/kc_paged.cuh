@@ -151,7 +151,7 @@ __global__ void __launch_bounds__(AP_THREADS, KV == KC_Q8_0 ? (NV == 1 ? 4 : 3) 
         for (int j = 0; j < NV; j++) {
             const int d = 4 * (lane + j * LPH), h = h0 + k * (32 / LPH);
             float4 t = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-            if (h < nh && d < hd) t = __ldcs((const float4 *)(src + (size_t)h * hd + d));
+            if (h < nh && d < hd) t = load_once(src + (size_t)h * hd + d);
             x[k][j][0] = t.x; x[k][j][1] = t.y; x[k][j][2] = t.z; x[k][j][3] = t.w;
         }
     const int pi = p >= 0 ? a.kv.page_of(p) : 0, slot = p - pi * a.kv.page;
@@ -175,9 +175,9 @@ __global__ void __launch_bounds__(AP_THREADS, KV == KC_Q8_0 ? (NV == 1 ? 4 : 3) 
             cs[j] = sn[j] = make_float2(0.0f, 0.0f);
             w[j] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
             if (d < hd) {
-                cs[j] = __ldg((const float2 *)(a.cos + (size_t)p * (hd / 2) + d / 2));
-                sn[j] = __ldg((const float2 *)(a.sin + (size_t)p * (hd / 2) + d / 2));
-                if (wt) w[j] = __ldg((const float4 *)(wt + d));
+                cs[j] = *(const float2 *)(a.cos + (size_t)p * (hd / 2) + d / 2);
+                sn[j] = *(const float2 *)(a.sin + (size_t)p * (hd / 2) + d / 2);
+                if (wt) w[j] = *(const float4 *)(wt + d);
             }
         }
         auto turn = [&](auto one) {
@@ -634,7 +634,7 @@ __global__ void __launch_bounds__(AT_THREADS, OCC) paged_attend_kernel(const __g
             if (i0 < tb0 || p0 + min(n, TP) > tbn) {
                 tb0 = i0;
                 tbn = (int)min((long long)(tb0 + 32) * a.kv.page, (long long)INT_MAX);
-                tab = tb0 + lane < a.kv.ld_table ? __ldg(a.kv.table + (size_t)lb * a.kv.ld_table + tb0 + lane) : -1;
+                tab = tb0 + lane < a.kv.ld_table ? a.kv.table[(size_t)lb * a.kv.ld_table + tb0 + lane] : -1;
             }
         }
         full = true;
@@ -643,7 +643,7 @@ __global__ void __launch_bounds__(AT_THREADS, OCC) paged_attend_kernel(const __g
             const int o = k * RW + prow, pi = a.kv.page_of(p0 + o);
             const bool in = o < n;
             int pg = __shfl_sync(0xffffffffu, tab, (pi - tb0) & 31);
-            if (!a.near) pg = in ? __ldg(a.kv.table + (size_t)lb * a.kv.ld_table + pi) : -1;
+            if (!a.near) pg = in ? a.kv.table[(size_t)lb * a.kv.ld_table + pi] : -1;
             const bool ok = in && (unsigned)pg < (unsigned)a.kv.n_pages;
             if (in && !ok) atomicOr(a.err, (unsigned)SE_PAGE);
             live[k] = __ballot_sync(0xffffffffu, ok) & (unsigned)((1ull << RW) - 1);
@@ -750,14 +750,14 @@ __global__ void __launch_bounds__(AT_THREADS, OCC) paged_attend_kernel(const __g
                     for (int i = 0; i < 2; i++) {
                         const int d = 16 * j + 8 * i + 2 * c;
                         float2 t = make_float2(0.0f, 0.0f);
-                        if (on && d < a.kv.hd) t = __ldg((const float2 *)(qh + d));
+                        if (on && d < a.kv.hd) t = *(const float2 *)(qh + d);
                         xq[mt][4 * j + 2 * i] = t.x;
                         xq[mt][4 * j + 2 * i + 1] = t.y;
                     }
                 } else {                               /* dims 16 j + 4 c + {0, 1, 2, 3} */
                     const int d = 16 * j + 4 * c;
                     float4 t = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-                    if (on && d < a.kv.hd) t = __ldg((const float4 *)(qh + d));
+                    if (on && d < a.kv.hd) t = *(const float4 *)(qh + d);
                     xq[mt][4 * j] = t.x; xq[mt][4 * j + 1] = t.y; xq[mt][4 * j + 2] = t.z; xq[mt][4 * j + 3] = t.w;
                 }
             }
