@@ -174,7 +174,8 @@ int kc_generate_sampled(kc_state *s, kc_sampler *p, int token, int pos, int n, i
  * presence, frequency: taken off a ring token's logit once, and once for each
  * time it is there (0, 0: off). */
 int kc_sampler_set_penalties(kc_sampler *p, float presence, float frequency);
-/* n biases added to tokens' logits (the last for a token counts); n 0: none. */
+/* n biases added to tokens' logits, finite or -inf (the last for a token counts);
+ * n 0: none. */
 int kc_sampler_set_bias(kc_sampler *p, const int *tokens, const float *values, int n);
 /* The tokens that may be chosen, bit v % 32 of word v / 32 of (vocab + 31) / 32
  * words, at least one of them (a grammar's next tokens); NULL: all. */
@@ -332,7 +333,7 @@ int kc_rope_tables(const kc_config *cfg, int n_pos, int local, float *cos_out, f
  * to position pos[i] of sequence seqs[i] (seqs NULL: of sequence i); a negative
  * sequence is padding: nothing is written for it. q, k, v: rows of n_heads,
  * n_kv_heads, n_kv_heads heads, ld* floats apart (multiples of 4; views of one
- * q|k|v matrix will do), 16-byte aligned. q_out may be q. Two rows of one
+ * q|k|v matrix will do), 16-byte aligned. q_out may be q, with the same stride. Two rows of one
  * call that name the same position leave either's values there, value by
  * value. */
 typedef struct {

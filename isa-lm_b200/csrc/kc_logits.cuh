@@ -135,9 +135,9 @@ __global__ void __launch_bounds__(LG_THREADS, 5) logits_kernel(const LogitsArgs 
         auto here = [&](int t) { return (unsigned)t < (unsigned)V && (unsigned)(t - e0) < (unsigned)LG_CHUNK; };
         auto touch = [&](int o) { s_list[atomicAdd(&s_n, 1)] = (unsigned short)o; };
         if constexpr (HIST) {
-            if (n > a.hist_cap) {
+            if ((unsigned)n > (unsigned)a.hist_cap) {
                 if (tid == 0 && blockIdx.y == 0) atomicOr(a.err, 1u);
-                n = a.hist_cap;
+                n = n < 0 ? 0 : a.hist_cap;
             }
             auto seen = [&](int t) {
                 if (here(t) && atomicAdd(&s_word[t - e0], 1u) == 0u) touch(t - e0);

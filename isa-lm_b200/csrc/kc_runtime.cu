@@ -1785,8 +1785,8 @@ extern "C" int kc_sampler_set_bias(kc_sampler *p, const int *tokens, const float
         return KC_E_SHAPE;
     }
     for (int i = 0; i < n; i++)
-        if (tokens[i] < 0 || tokens[i] >= p->s->c.vocab || std::isnan(values[i])) {
-            set_error("a bias for a token outside the vocabulary, or not a number");
+        if (tokens[i] < 0 || tokens[i] >= p->s->c.vocab || !(values[i] < INFINITY)) {
+            set_error("a bias for a token outside the vocabulary, or neither finite nor -inf");
             return KC_E_SHAPE;
         }
     int rc = sampler_more(p);

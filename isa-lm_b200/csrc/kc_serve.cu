@@ -77,7 +77,7 @@ std::string serve_err_text(unsigned w) {
     auto add = [&](unsigned bit, const char *t) {
         if (w & bit) s += std::string(s.empty() ? "" : ", ") + t;
     };
-    add(SE_HIST, "a history length beyond its rows");
+    add(SE_HIST, "a history length below 0 or beyond its rows");
     add(SE_BIAS, "bias offsets out of order or beyond the list");
     add(SE_LEN, "a sequence length below 0 or beyond its table row");
     add(SE_PAGE, "a page number outside the pool");
@@ -260,6 +260,7 @@ extern "C" int kc_paged_append_dev(const kc_paged_kv *kv, const kc_append_args *
     if (!(x->eps >= 0.0f) || std::isinf(x->eps)) return refuse("eps must be finite and not negative");
     if ((double)x->rows * (x->n_heads + 2 * kv->n_kv_heads) > 2147483647.0 - 65536.0) return refuse("too many rows in one call");
     if (!x->seqs && x->rows > kv->n_seqs) return refuse("more rows than sequences, and no seqs");
+    if (x->q == x->q_out && x->rows > 1 && x->ldq != x->ldo) return refuse("in place, but the row strides differ");
     ServeDev d;
     rc = serve_device(d);
     if (rc != KC_OK) return rc;
@@ -345,7 +346,8 @@ extern "C" int kc_paged_attend_dev(const kc_paged_kv *kv, const kc_attend_args *
     rc = attend_variant(kv, x->n_heads, d, v, a.chunks);
     if (rc != KC_OK) return rc;
     const int ctas = v->ctas[d.dev];
-    if ((double)x->n_seqs * ((double)kv->ld_table * kv->page_size / (AT_WARPS * v->tile) + 2 + AT_UNIT_COST) >= 2147483648.0)
+    const double quanta = (double)x->n_seqs * ((double)kv->ld_table * kv->page_size / (AT_WARPS * v->tile) + 2 + AT_UNIT_COST);
+    if (quanta >= 2147483648.0 || quanta * kv->n_kv_heads * a.chunks / ctas >= 1073741824.0)
         return refuse("n_seqs sequences of ld_table * page_size positions are too many for one call");
     if (x->ws_bytes < ws_bytes(v, ctas))
         return refuse("workspace of " + std::to_string(x->ws_bytes) + " bytes, " + std::to_string(ws_bytes(v, ctas)) +

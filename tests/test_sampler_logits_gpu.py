@@ -92,3 +92,11 @@ def test_refusals(model):
         s.set_penalties(float("inf"))
     with pytest.raises(kb.KraflaError, match="allowed"):
         s.set_mask(np.ones(v + 1, bool))
+
+
+@pytest.mark.parametrize("value", [float("inf"), float("nan")])
+def test_bias_beyond_numbers_is_refused(model, value):
+    s = kb.Sampler(kb.State(model), temperature=0.8)
+    with pytest.raises(kb.KraflaError):
+        s.set_bias({3: value})
+    s.set_bias({3: float("-inf")})                     # a token never to be chosen is a bias

@@ -70,6 +70,10 @@ def test_append_is_refused(kw, word):
     assert word in refused(kb.lib().kc_paged_append_dev, cache(), append_args(**kw))
 
 
+def test_append_in_place_needs_one_stride():
+    assert "in place" in refused(kb.lib().kc_paged_append_dev, cache(), append_args())
+
+
 def logits_args(**kw):
     d = dict({n: 0 for n in kb._LOGITS.names}, out=P, ld_in=100, ld_out=100, rows=3, vocab=100)
     d["in"] = P

@@ -581,3 +581,64 @@ def test_streams_graphs_and_far_offsets():
         else:
             assert (outs[1][1] == 0).all()
     del graphs
+
+
+def test_logits_negative_history_length_is_told():
+    out = kb.process_logits(kb.DevArray((2, 50), np.float32), kb.DevArray.of(np.ones((2, 50), np.float32)),
+                            history=kb.DevArray.of(np.zeros((2, 3), np.int32)),
+                            history_len=kb.DevArray.of(np.array([-5, 3], np.int32)),
+                            frequency=kb.DevArray.of(np.ones(2, np.float32)))
+    with pytest.raises(kb.KraflaError, match="history length"):
+        kb._check(kb.lib().kc_dev_sync(), "sync")
+    assert (out.numpy()[0] == 1).all() and out.numpy()[1, 0] == -2
+
+
+def test_two_streams_in_one_graph():
+    """A graph whose two branches append to and read a cache each, join, and are followed by the logits of both:
+    every launch has a kernel or an event of another stream before it. Replays give what calls in a row give."""
+    torch = pytest.importorskip("torch")
+    heads, hk, hd, page, n = 4, 2, 64, 16, 3
+    g = torch.Generator().manual_seed(3)
+    cos, sin = (torch.from_numpy(t).cuda() for t in kb.rope_tables(dict(head_dim=hd, rope_theta=1e4), 64))
+    table = torch.arange(n * 4, dtype=torch.int32).reshape(n, 4).cuda()
+    caches, xs, qs = [], [], []
+    for _ in range(2):
+        k, v = (torch.randn(n * 4, hk, page, hd, generator=g).half().cuda() for _ in range(2))
+        caches.append(kb.PagedKV(k, v, table, kb.F16, n_heads=heads))
+        xs.append(torch.randn(n, (heads + 2 * hk) * hd, generator=g).cuda())
+        qs.append(torch.empty(n, heads, hd, device="cuda"))
+    pos = torch.tensor([40, 3, 63], dtype=torch.int32, device="cuda")
+    lens = pos + 1
+    both, last = torch.empty(2 * n, heads * hd, device="cuda"), torch.empty(2 * n, heads * hd, device="cuda")
+    hist = torch.randint(0, heads * hd, (2 * n, 9), generator=g, dtype=torch.int32).cuda()
+    rep = torch.full((2 * n,), 1.3, device="cuda")
+
+    def half(i, st):
+        caches[i].append(xs[i], pos, cos, sin, qs[i], stream=st)
+        caches[i].attend(qs[i], lens, both[i * n:(i + 1) * n], stream=st)
+
+    def end(st):
+        kb.process_logits(last, both, history=hist, repeat=rep, stream=st)
+
+    main, side = torch.cuda.Stream(), torch.cuda.Stream()
+    torch.cuda.synchronize()
+    for i in range(2):
+        half(i, main.cuda_stream)
+    end(main.cuda_stream)
+    torch.cuda.synchronize()
+    want = last.clone()
+    gr = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(gr, stream=main):
+        side.wait_stream(main)
+        half(1, side.cuda_stream)
+        half(0, main.cuda_stream)
+        main.wait_stream(side)
+        end(main.cuda_stream)
+    for _ in range(3):
+        both.zero_()
+        last.zero_()
+        torch.cuda.synchronize()
+        gr.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(last, want)
+    del gr
