@@ -282,10 +282,10 @@ __global__ void __launch_bounds__(AP_THREADS, KV == KC_Q8_0 ? (NV == 1 ? 4 : 3) 
  * what a copy reaches; 2 of 131072 176 us, 5.8 TB/s. Where the bytes are fewer the
  * arithmetic shows: splitting an f32 value takes four integer and float
  * instructions, an 8-bit one a fifth of a word's five (64 of 4096, head 64, 8-bit:
- * 61 us at a floor of 44; 32 of 2048, head 64, f32: 52 at 41). Small calls are
- * bound by their chain of latencies, about 5.6 us for one tile: launch, length,
- * table, rows, products, the warps' meeting; a joined unit 3 us more (of which
- * its pieces' sums 1.5). */
+ * 61 us at a floor of 44, 65 in a long run; 32 of 2048, head 64, f32: 52 at 41, in
+ * a long run 56). Small calls are bound by their chain of latencies, about 5.8 us
+ * for one tile: launch, length, table, rows, products, the warps' meeting; a
+ * joined unit 3 us more (of which its pieces' sums 1.5). */
 constexpr int AT_WARPS = 4;
 constexpr int AT_THREADS = AT_WARPS * 32;
 /* Quanta of a unit that is not worth sharing out where every unit has a CTA of its own: of 5 quanta, 78 units 11.2 us
