@@ -201,11 +201,17 @@ static AttendVariant make_variant() {
  * held to: the same 64 sequences 212 us instead of 224, 256 of 1..1000 100 instead
  * of 105, 64 of 4096, 8-bit, head 64, 66 instead of 71. Only the 8-bit cache of
  * head 128 has no registers for it to spare: 32 of 2048 37 us with two CTAs, 38.5
- * with three. */
+ * with three. A tile of head 256 is so large that two slots a warp leave room for
+ * one CTA an SM, whose 4 warps wait for their own results; one slot lets two in:
+ * 16 of 2048, f32, 85 us with two slots, 70 with one; f16 34 and 32, 8-bit (32 of
+ * them) 44 and 38; 200 of 1..300, f16, 47 and 35. A sequence or two alone are cut
+ * into as many pieces as there are CTAs, and half as many are better joined: one of
+ * 32768, f16, 37 us with two slots, 43 with one, 8 heads to a KV head, f32, 71 and
+ * 91; from 16 units on (4 of 8192: f32 84 and 69, f16 34 and 34) it is the other way. */
 template <int KV>
-static AttendVariant *variants_of(int hd, int group, int &mt) {
+static AttendVariant *variants_of(int hd, int group, long long units, int &mt) {
     static AttendVariant v64 = make_variant<KV, 64, 2, 1, 2, 3>(), v128 = make_variant<KV, 128, 1, 1, 2, KV == KC_Q8_0 ? 2 : 3>(),
-                         v256 = make_variant<KV, 256, 1, 1, 2, 1>();
+                         v256 = make_variant<KV, 256, 1, 1, 1, 2>(), few256 = make_variant<KV, 256, 1, 1, 2, 1>();
     if constexpr (KV != KC_F32) {
         /* more than 8 heads share a KV head: 16 at a time, so that the cache is read once */
         static AttendVariant w64 = make_variant<KV, 64, 2, 2, 2, 2>(), w128 = make_variant<KV, 128, 1, 2, 2, 2>();
@@ -215,15 +221,16 @@ static AttendVariant *variants_of(int hd, int group, int &mt) {
         }
     }
     mt = 1;
-    return hd <= 64 ? &v64 : (hd <= 128 ? &v128 : &v256);
+    return hd <= 64 ? &v64 : (hd <= 128 ? &v128 : (units <= 8 ? &few256 : &v256));
 }
 
-static int attend_variant(const kc_paged_kv *kv, int n_heads, const ServeDev &d, AttendVariant *&v, int &chunks) {
+static int attend_variant(const kc_paged_kv *kv, int n_heads, int n_seqs, const ServeDev &d, AttendVariant *&v, int &chunks) {
     const int group = n_heads / kv->n_kv_heads;
+    const long long units = (long long)n_seqs * kv->n_kv_heads * ((group + 7) / 8);
     int mt = 1;
-    v = kv->kv_type == KC_F32 ? variants_of<KC_F32>(kv->head_dim, group, mt)
-                              : (kv->kv_type == KC_F16 ? variants_of<KC_F16>(kv->head_dim, group, mt)
-                                                       : variants_of<KC_Q8_0>(kv->head_dim, group, mt));
+    v = kv->kv_type == KC_F32 ? variants_of<KC_F32>(kv->head_dim, group, units, mt)
+                              : (kv->kv_type == KC_F16 ? variants_of<KC_F16>(kv->head_dim, group, units, mt)
+                                                       : variants_of<KC_Q8_0>(kv->head_dim, group, units, mt));
     chunks = (group + 8 * mt - 1) / (8 * mt);
     if (!v->ctas[d.dev]) {
         SK(cudaFuncSetAttribute((const void *)v->attend, cudaFuncAttributeMaxDynamicSharedMemorySize, v->smem), "attend");
@@ -306,9 +313,13 @@ extern "C" int kc_paged_attend_ws(const kc_paged_kv *kv, int n_heads, size_t *by
     AttendVariant *v = nullptr;
     int chunks = 0;
     rc = serve_device(d);
-    if (rc == KC_OK) rc = attend_variant(kv, n_heads, d, v, chunks);
-    if (rc != KC_OK) return rc;
-    *bytes = ws_bytes(v, v->ctas[d.dev]);
+    size_t most = 0;
+    for (int n : { 1, kv->n_seqs }) {                  /* calls of any number of sequences share it */
+        if (rc == KC_OK) rc = attend_variant(kv, n_heads, n, d, v, chunks);
+        if (rc != KC_OK) return rc;
+        most = std::max(most, ws_bytes(v, v->ctas[d.dev]));
+    }
+    *bytes = most;
     return KC_OK;
 }
 
@@ -343,7 +354,7 @@ extern "C" int kc_paged_attend_dev(const kc_paged_kv *kv, const kc_attend_args *
     if (x->n_seqs == 0) return KC_OK;
     AttendArgs a{};
     AttendVariant *v = nullptr;
-    rc = attend_variant(kv, x->n_heads, d, v, a.chunks);
+    rc = attend_variant(kv, x->n_heads, x->n_seqs, d, v, a.chunks);
     if (rc != KC_OK) return rc;
     const int ctas = v->ctas[d.dev];
     const double quanta = (double)x->n_seqs * ((double)kv->ld_table * kv->page_size / (AT_WARPS * v->tile) + 2 + AT_UNIT_COST);

@@ -642,3 +642,24 @@ def test_two_streams_in_one_graph():
         torch.cuda.synchronize()
         assert torch.equal(last, want)
     del gr
+
+
+@pytest.mark.parametrize("kv", ["f32", "f16", "q8"])
+@pytest.mark.parametrize("heads,hk,hd", [(8, 2, 256), (12, 1, 192), (2, 2, 144)])
+def test_attend_wide_heads_few_and_many(kv, heads, hk, hd):
+    """Calls of one sequence and of many, which wide heads take in different shapes, in turn in one workspace."""
+    rng = np.random.default_rng(heads + hd)
+    lens, page = [2500, 0, 1, 700, 64, 8, 33, 1500, 15, 2049], 16
+    n_pages = sum(-(-m // page) for m in lens)
+    pools = make_pool(rng, kv, n_pages, hk, page, hd)
+    table = make_table(rng, lens, page, n_pages)
+    q = rng.standard_normal((len(lens), heads, hd)).astype(np.float32)
+    c = handle(pools, table, kv, heads)
+    k, v, kd, vd = pools
+    vmax = np.abs(v.astype(np.float64)).max() if kd is None else (127 * vd).max()
+    want, reach = ref.attend(q, k, v, table, lens, hd ** -0.5, 0, 20.0, kd, vd)
+    for n in (1, len(lens), 2, 1, 5, len(lens)):
+        out = kb.DevArray.of(np.full((n, heads, hd), np.nan, np.float32))
+        c.attend(kb.DevArray.of(q[:n]), kb.DevArray.of(np.array(lens[:n], np.int32)), out, softcap=20.0)
+        check(out.numpy(), want[:n], reach[:n], vmax, hd, max(lens))
+    kb._check(kb.lib().kc_dev_sync(), "sync")
