@@ -1223,7 +1223,10 @@ __global__ void __launch_bounds__(AT_THREADS, OCC) paged_attend_kernel(const __g
     /* the first S passes only load */
     for (int it = -S, stage = 0; it < issued; it++, stage = stage + 1 == S ? 0 : stage + 1) {
         int4 f = make_int4(cu_b, cu_u, 0, 0);
-        if (it >= 0) f = info[stage];                  /* written when the slot's copies were issued */
+        /* lane 0 wrote what the slot holds when its copies were issued: with several slots a pass, and its barriers,
+         * ago, with one slot at the end of the pass before */
+        if constexpr (S == 1) __syncwarp();
+        if (it >= 0) f = info[stage];
         const int fu = f.y & (LAST_OF_UNIT - 1);
         if (f.x != cu_b || fu != cu_u) {
             /* a new unit: its queries are on their way while the tile arrives */

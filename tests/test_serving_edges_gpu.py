@@ -1,0 +1,44 @@
+"""Serving operators on the GPU at edges that the tests beside this one leave
+out. Tolerances of attention: test_serving_gpu's."""
+import numpy as np
+import pytest
+
+import krafla_b200 as kb
+import serving_ref as ref
+from test_serving_gpu import check, handle, make_pool, make_table, spoil
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(scope="module", autouse=True)
+def _dev(built):
+    kb.device_check()
+
+
+@pytest.mark.parametrize("kv", ["f32", "f16", "q8"])
+@pytest.mark.parametrize("heads,hk,hd", [(12, 3, 256), (9, 1, 192), (4, 4, 144)])
+def test_attend_wide_heads_tile_by_tile(kv, heads, hk, hd):
+    """Wide heads of more than 8 units keep one tile a warp at a time: what a tile holds (its unit, its mask, whether
+    it is the last) is another in every pass. Lengths of every remainder of a quantum, so that masks differ between
+    warps and between passes, units that begin and end in the middle of a share, and warps without a tile; the same
+    call many times gives the same bits."""
+    rng = np.random.default_rng(heads + hd)
+    page = 8
+    lens = [*range(1, 70, 3), *rng.integers(1, 600, 90).tolist(), 0, 0, *rng.integers(200, 900, 30).tolist()]
+    n_pages = sum(-(-m // page) for m in lens)
+    pools = make_pool(rng, kv, n_pages, hk, page, hd)
+    table = make_table(rng, lens, page, n_pages)
+    spoil(pools, table, lens, page)
+    q = rng.standard_normal((len(lens), heads, hd)).astype(np.float32)
+    c = handle(pools, table, kv, heads)
+    dq, dl = kb.DevArray.of(q), kb.DevArray.of(np.array(lens, np.int32))
+    k, v, kd, vd = pools
+    vmax = np.nanmax(np.abs(v.astype(np.float64))) if kd is None else np.nanmax(127 * vd)
+    first = None
+    for _ in range(20):
+        out = c.attend(dq, dl, kb.DevArray.of(np.full(q.shape, np.nan, np.float32))).numpy()
+        first = out if first is None else first
+        assert np.array_equal(out, first)
+    kb._check(kb.lib().kc_dev_sync(), "sync")
+    want, reach = ref.attend(q, k, v, table, lens, hd ** -0.5, 0, 0.0, kd, vd)
+    check(first, want, reach, vmax, hd, max(lens))
