@@ -175,7 +175,9 @@ int kc_generate_sampled(kc_state *s, kc_sampler *p, int token, int pos, int n, i
  * time it is there (0, 0: off). */
 int kc_sampler_set_penalties(kc_sampler *p, float presence, float frequency);
 /* n biases added to tokens' logits, finite or -inf (the last for a token counts);
- * n 0: none. */
+ * n 0: none. A token biased to -inf is not drawn as long as a logit above -inf
+ * is left; where none is, the draw is uniform over the vocabulary, as the
+ * reference's of such logits, and with a mask the lowest allowed token. */
 int kc_sampler_set_bias(kc_sampler *p, const int *tokens, const float *values, int n);
 /* The tokens that may be chosen, bit v % 32 of word v / 32 of (vocab + 31) / 32
  * words, at least one of them (a grammar's next tokens); NULL: all. */

@@ -1646,7 +1646,7 @@ struct kc_sampler {
     std::vector<int> ring;    /* mirror of the device ring */
     /* penalties, biases and a mask beside the reference's options (kc_sampler_set_*): the logits then pass
      * through kc_logits_process_dev on their way */
-    bool more = false, masked = false;
+    bool more = false, masked = false, banned = false;   /* banned: some bias is -inf */
     float *values = nullptr;      /* repeat, presence, frequency, then the processed logits [vocab] */
     uint32_t *mask = nullptr;
     int *bias_ids = nullptr;      /* offsets 0 and n, then the ids */
@@ -1812,6 +1812,7 @@ extern "C" int kc_sampler_set_bias(kc_sampler *p, const int *tokens, const float
     p->bias_ids = ids;
     p->bias_vals = vals;
     p->n_bias = n;
+    p->banned = std::any_of(values, values + n, [](float v) { return v == -INFINITY; });
     p->more = true;
     return KC_OK;
 }
@@ -1872,6 +1873,7 @@ static int sampler_args(kc_sampler *p, const float *logits, SampleArgs &a) {
     }
     a.logits = x.out;
     a.repeat_penalty = 1.0f;
+    a.barred = p->masked || p->banned;
     return kc_logits_process_dev(&x, p->s->st);
 }
 

@@ -51,7 +51,57 @@ struct SampleArgs {
     LoopState *ls;            /* optional: the device loop, advanced to the token */
     int *out_tokens;          /* optional, with ls: the step's slot */
     const uint32_t *allowed;  /* optional: the tokens that may be chosen, a bit each */
+    int barred;               /* some logits are -inf since a mask or a bias bars their tokens */
 };
+
+__host__ __device__ __forceinline__ float sm_add(float a, float b) {
+#ifdef __CUDA_ARCH__
+    return __fadd_rn(a, b);
+#else
+    return a + b;
+#endif
+}
+
+/* sample_mult (:63-70): the first token whose running sum passes the coin. csum
+ * holds the sums of the stretches of `chunk` tokens, each from 0 in the tokens'
+ * order; they are gone over first, then the tokens of the stretch whose sum
+ * passes the coin. A coin past the sum of all (by rounding) takes the
+ * vocabulary's last token, as in the reference, and so does one that the
+ * tokens, added to the running sum one by one, do not reach although their
+ * stretch's sum does: with one token of nearly all the mass and a flat tail
+ * most of the tail's draws (a sum in [1/2, 1) does not move by less than 2^-25).
+ *
+ * Where tokens are barred the last token may be one of them. The tokens are
+ * then added up from the stretch's beginning as its sum was, so that the last
+ * sum is the stretch's own and one of them passes the coin, for the first time
+ * at a probability above 0; past the sum of all it is the last such token. */
+__host__ __device__ inline int sm_mult_pick(const float *p, const float *csum, int stretches, int chunk, int n, float coin, bool barred) {
+    float cdf = 0.0f;
+    int t = 0;
+    for (; t < stretches; t++) {
+        const float next = sm_add(cdf, csum[t]);
+        if (coin < next) break;
+        cdf = next;
+    }
+    if (t < stretches) {
+        const int l0 = t * chunk, l1 = l0 + chunk < n ? l0 + chunk : n;
+        float in = 0.0f;
+        for (int i = l0; i < l1; i++) {
+            if (barred) {
+                in = sm_add(in, p[i]);
+                if (coin < sm_add(cdf, in)) return i;
+            } else {
+                cdf = sm_add(cdf, p[i]);
+                if (coin < cdf) return i;
+            }
+        }
+    } else if (barred) {
+        while (t > 0 && !(csum[t - 1] > 0.0f)) t--;
+        for (int i = (t * chunk < n ? t * chunk : n) - 1; i >= 0; i--)
+            if (p[i] > 0.0f) return i;
+    }
+    return n - 1;
+}
 
 __device__ __forceinline__ float sm_block_max(float v, float *red) {
     v = warp_max(v);
@@ -404,38 +454,21 @@ __global__ void __launch_bounds__(SM_THREADS, 1) sample_kernel(const SampleArgs 
                 }
             }
         } else {
-            /* sample_mult (:63-70): the first token whose running sum passes the
-             * coin; each thread sums a contiguous range, the ranges in order */
+            /* each thread sums a stretch, a contiguous range; the ranges in order */
             const int chunk = (n + SM_THREADS - 1) / SM_THREADS, lo = tid * chunk, hi = min(n, lo + chunk);
             float cs = 0.0f;
             for (int i = lo; i < hi; i++) cs = __fadd_rn(cs, p[i]);
             float *csum = (float *)hist;
             csum[tid] = cs;
             __syncthreads();
-            if (tid == 0) {
-                float cdf = 0.0f;
-                int tok = n - 1, t = 0;
-                for (; t < SM_THREADS; t++) {
-                    const float next = __fadd_rn(cdf, csum[t]);
-                    if (coin < next) break;
-                    cdf = next;
-                }
-                if (t < SM_THREADS) {
-                    const int l0 = t * chunk, l1 = min(n, l0 + chunk);
-                    for (int i = l0; i < l1; i++) {
-                        cdf = __fadd_rn(cdf, p[i]);
-                        if (coin < cdf) { tok = i; break; }
-                    }
-                }
-                s_tok = tok;
-            }
+            if (tid == 0) s_tok = sm_mult_pick(p, csum, SM_THREADS, chunk, n, coin, a.barred);
         }
     }
     __syncthreads();
     if (a.allowed && !((a.allowed[s_tok >> 5] >> (s_tok & 31)) & 1u)) {
-        /* a masked logit is -inf and its token's probability 0, but a draw that rounding leaves past the last
-         * running sum falls on whatever token is last (:63-70), and so may rows whose allowed logits are all
-         * -inf: the best of the allowed ones then */
+        /* a masked logit is -inf and its token's probability 0, but where every logit is -inf (biases of -inf on
+         * all that the mask allows) the softmax is uniform over the vocabulary, and a row with a NaN has no
+         * probabilities at all: the best of the allowed tokens then, the lowest of equal ones */
         unsigned long long best = 0ull;
         for (int i = tid; i < n; i += SM_THREADS)
             if ((a.allowed[i >> 5] >> (i & 31)) & 1u) {
