@@ -918,13 +918,15 @@ __global__ void __launch_bounds__(AT_THREADS, OCC) paged_attend_kernel(const __g
             }
         }
     };
-    /* soft-cap, mask, running softmax in base 2: the scores become weights, lifted by a power of two that keeps
-     * the small ones normal f16 numbers: 2^15, and for 8-bit rows, whose scales join the weights, over the next
-     * power of two above the tile's largest scale (back: what the tile's sums are multiplied by) */
+    /* soft-cap, mask, running softmax in base 2: the scores become weights. For f16 products they are then lifted
+     * by a power of two that keeps the small ones normal f16 numbers: 2^15, and for 8-bit rows, whose scales join
+     * the weights, over the next power of two above the tile's largest scale (back: what the tile's sums are
+     * multiplied by). By a product, which is exact: added to the exponent it would take as many bits off the
+     * exponent's fraction as it is large, 4 of 24 for 2^15 and up to 7 for the smallest scales. */
+    constexpr float LIFT = KV == KC_F32 ? 1.0f : 32768.0f;
     float2 corr[MT];                                   /* what the sums so far are scaled by */
-    float back = 1.0f;
+    float lift = LIFT, back = 1.0f;
     auto soften = [&](int stage, const unsigned (&live)[LK]) {
-        float lift = KV == KC_F32 ? 0.0f : 15.0f;
         if constexpr (KV == KC_Q8_0) {
             const float *vd = scl + stage * SCALES + TP;
             float top = fabsf(vd[lane]);
@@ -933,7 +935,7 @@ __global__ void __launch_bounds__(AT_THREADS, OCC) paged_attend_kernel(const __g
             top = warp_max(top);
             int ex = (int)((__float_as_uint(top) >> 23) & 255) - 126;
             ex = min(max(ex, -100), 100);
-            lift -= (float)ex;
+            lift = __uint_as_float((unsigned)(127 + 15 - ex) << 23);
             back = __uint_as_float((unsigned)(127 + ex) << 23);
         }
         bool all = true;
@@ -960,19 +962,19 @@ __global__ void __launch_bounds__(AT_THREADS, OCC) paged_attend_kernel(const __g
             for (int nt = 1; nt < NT; nt++) mx = fmaxf(mx, fmaxf(s[mt][nt].x, s[mt][nt].y));
             mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
             mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
-            const float mn = fmaxf(m[mt], mx * qm), base = mn == -INFINITY ? 0.0f : mn, add = lift - base;
+            const float mn = fmaxf(m[mt], mx * qm), base = mn == -INFINITY ? 0.0f : mn;
             const float cr = ex2(m[mt] - base);
             corr[mt] = make_float2(cr, cr);
             m[mt] = mn;
             float2 both = make_float2(0.0f, 0.0f);
 #pragma unroll
             for (int nt = 0; nt < NT; nt++) {
-                const float2 x = fma2(s[mt][nt], make_float2(qm, qm), make_float2(add, add));
+                const float2 x = fma2(s[mt][nt], make_float2(qm, qm), make_float2(-base, -base));
                 s[mt][nt] = make_float2(ex2(x.x), ex2(x.y));
                 both = nt ? add2(both, s[mt][nt]) : s[mt][nt];
             }
             const float sum = both.x + both.y;
-            l[mt] = l[mt] * cr + sum * back;
+            l[mt] = l[mt] * cr + sum * LIFT;
         }
     };
     /* the weighted sum of V's rows */
@@ -985,7 +987,7 @@ __global__ void __launch_bounds__(AT_THREADS, OCC) paged_attend_kernel(const __g
             for (int mt = 0; mt < MT; mt++)
 #pragma unroll
                 for (int nt = 0; nt < NT; nt++)
-                    split_f16(s[mt][nt], w[mt][nt >> 1][2 * (nt & 1)], w[mt][nt >> 1][2 * (nt & 1) + 1]);
+                    split_f16(mul2(s[mt][nt], make_float2(LIFT, LIFT)), w[mt][nt >> 1][2 * (nt & 1)], w[mt][nt >> 1][2 * (nt & 1) + 1]);
             const uint32_t vb = sv + (lane & 15) * PITCH + (((lane >> 4) ^ (lane & 7)) << 4);
 #pragma unroll
             for (int jj = 0; jj < HD / 16; jj++) {
@@ -1053,7 +1055,7 @@ __global__ void __launch_bounds__(AT_THREADS, OCC) paged_attend_kernel(const __g
             unsigned w[MT][KS][4];
 #pragma unroll
             for (int nt = 0; nt < NT; nt++) {
-                const float2 e = *(const float2 *)(vd + nt * 8 + 2 * c);
+                const float2 e = mul2(*(const float2 *)(vd + nt * 8 + 2 * c), make_float2(lift, lift));
 #pragma unroll
                 for (int mt = 0; mt < MT; mt++)
                     split_f16(mul2(s[mt][nt], e), w[mt][nt >> 1][2 * (nt & 1)],

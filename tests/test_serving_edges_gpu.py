@@ -42,3 +42,29 @@ def test_attend_wide_heads_tile_by_tile(kv, heads, hk, hd):
     kb._check(kb.lib().kc_dev_sync(), "sync")
     want, reach = ref.attend(q, k, v, table, lens, hd ** -0.5, 0, 0.0, kd, vd)
     check(first, want, reach, vmax, hd, max(lens))
+
+
+def test_attend_8bit_weights_do_not_lose_bits_to_small_scales():
+    """Rows whose scales are near 1e-30: half of the positions have V = v and score 0, half -v and a score x / log2 e
+    with x = 3.7e-6, so the output is v (w_0 - w_x) / (w_0 + w_x) = -v 1.28e-6. A weight keeps its 22 bits whatever V's
+    scale is. Errors against v, of two weights near 1, half of each: 2^-22 each for exp2 and for the two halves of 11
+    bits, 2^-24 for the product with the scale; 2^-22 for the sums, which stay small since the signs alternate. In all
+    below 2^-20. (Weights rounded at the size of a lift of 2^114 would come out equal, and the output 0.)"""
+    hd, page, n, x = 64, 16, 512, 3.7e-6
+    k = np.zeros((n // page, 1, page, hd), np.int8)
+    k[..., 0] = 1
+    v = np.full(k.shape, 127, np.int8)
+    v[:, :, 1::2] = -127
+    kd = np.zeros(k.shape[:3], np.float32)
+    kd[:, :, 1::2] = 1.0
+    vd = np.full(k.shape[:3], 2.0 ** -100, np.float32)
+    q = np.zeros((1, 1, hd), np.float32)
+    q[0, 0, 0] = 1.0
+    table = np.arange(n // page, dtype=np.int32)[None]
+    c = handle((k, v, kd, vd), table, "q8", 1)
+    scale = x * np.log(2.0)
+    out = c.attend(kb.DevArray.of(q), kb.DevArray.of(np.array([n], np.int32)), kb.DevArray(q.shape, np.float32), scale=scale)
+    want, _ = ref.attend(q, k, v, table, [n], float(np.float32(scale)), 0, 0.0, kd, vd)
+    top = 127 * 2.0 ** -100
+    assert np.allclose(want / top, -1.28e-6, rtol=0.01)
+    assert (np.abs(out.numpy() - want) <= 2.0 ** -20 * top).all()
