@@ -6,6 +6,7 @@
 #include <cuda_runtime.h>
 
 #include <algorithm>
+#include <atomic>
 #include <cmath>
 #include <string>
 
@@ -39,7 +40,9 @@ constexpr int SV_MAX_DEVICES = 64;
 
 /* The serving kernels' error word, one per device, sticky until kc_dev_sync. */
 static __device__ unsigned g_sv_err;
-static unsigned *g_sv_err_ptr[SV_MAX_DEVICES];
+/* What is looked up at a device's first use may be looked up by several threads at once, with the same result: each
+ * stores it whole, the pointer last, and whoever sees the pointer sees what was stored before it. */
+static std::atomic<unsigned *> g_sv_err_ptr[SV_MAX_DEVICES];
 
 struct ServeDev {
     int dev = 0, sms = 0;
@@ -48,10 +51,11 @@ struct ServeDev {
 
 /* The current device: its SMs and error word (looked up once per device). */
 static int serve_device(ServeDev &d) {
-    static int sms[SV_MAX_DEVICES];
+    static std::atomic<int> sms[SV_MAX_DEVICES];
     SK(cudaGetDevice(&d.dev), "current device");
     if (d.dev < 0 || d.dev >= SV_MAX_DEVICES) return refuse("device index " + std::to_string(d.dev) + " beyond this library's table");
-    if (!g_sv_err_ptr[d.dev]) {
+    d.err = g_sv_err_ptr[d.dev].load(std::memory_order_acquire);
+    if (!d.err) {
         int major = 0, minor = 0, n = 0;
         SK(cudaDeviceGetAttribute(&major, cudaDevAttrComputeCapabilityMajor, d.dev), "device");
         SK(cudaDeviceGetAttribute(&minor, cudaDevAttrComputeCapabilityMinor, d.dev), "device");
@@ -62,15 +66,15 @@ static int serve_device(ServeDev &d) {
         SK(cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, d.dev), "device");
         void *p = nullptr;
         SK(cudaGetSymbolAddress(&p, g_sv_err), "error word");
-        sms[d.dev] = n;
-        g_sv_err_ptr[d.dev] = (unsigned *)p;
+        d.err = (unsigned *)p;
+        sms[d.dev].store(n, std::memory_order_relaxed);
+        g_sv_err_ptr[d.dev].store(d.err, std::memory_order_release);
     }
-    d.sms = sms[d.dev];
-    d.err = g_sv_err_ptr[d.dev];
+    d.sms = sms[d.dev].load(std::memory_order_relaxed);
     return KC_OK;
 }
 
-unsigned *serve_err_word(int dev) { return dev >= 0 && dev < SV_MAX_DEVICES ? g_sv_err_ptr[dev] : nullptr; }
+unsigned *serve_err_word(int dev) { return dev >= 0 && dev < SV_MAX_DEVICES ? g_sv_err_ptr[dev].load(std::memory_order_acquire) : nullptr; }
 
 std::string serve_err_text(unsigned w) {
     std::string s;
@@ -178,18 +182,14 @@ constexpr int AT_MAX_CTAS = 2048;
 struct AttendVariant {
     void (*attend)(const AttendArgs);
     int smem, part, tile, heads;
-    int ctas[SV_MAX_DEVICES];
+    std::atomic<int> ctas[SV_MAX_DEVICES];             /* 0: not asked yet */
 };
 
 template <int KV, int HD, int TM, int MT, int S, int OCC>
-static AttendVariant make_variant() {
-    AttendVariant v{};
-    v.attend = paged_attend_kernel<KV, HD, TM, MT, S, OCC>;
-    v.smem = attend_smem<KV, HD, TM, MT, S>();
-    v.part = part_floats<HD, MT>();
-    v.heads = 8 * MT;
-    v.tile = att_tp<KV, TM>();
-    return v;
+static AttendVariant *variant() {
+    static AttendVariant v{ paged_attend_kernel<KV, HD, TM, MT, S, OCC>, attend_smem<KV, HD, TM, MT, S>(), part_floats<HD, MT>(),
+                            att_tp<KV, TM>(), 8 * MT, {} };
+    return &v;
 }
 
 /* The instance for a cache and group: a template of positions per tile, heads
@@ -210,21 +210,20 @@ static AttendVariant make_variant() {
  * 91; from 16 units on (4 of 8192: f32 84 and 69, f16 34 and 34) it is the other way. */
 template <int KV>
 static AttendVariant *variants_of(int hd, int group, long long units, int &mt) {
-    static AttendVariant v64 = make_variant<KV, 64, 2, 1, 2, 3>(), v128 = make_variant<KV, 128, 1, 1, 2, KV == KC_Q8_0 ? 2 : 3>(),
-                         v256 = make_variant<KV, 256, 1, 1, 1, 2>(), few256 = make_variant<KV, 256, 1, 1, 2, 1>();
     if constexpr (KV != KC_F32) {
         /* more than 8 heads share a KV head: 16 at a time, so that the cache is read once */
-        static AttendVariant w64 = make_variant<KV, 64, 2, 2, 2, 2>(), w128 = make_variant<KV, 128, 1, 2, 2, 2>();
         if (group > 8 && hd <= 128) {
             mt = 2;
-            return hd <= 64 ? &w64 : &w128;
+            return hd <= 64 ? variant<KV, 64, 2, 2, 2, 2>() : variant<KV, 128, 1, 2, 2, 2>();
         }
     }
     mt = 1;
-    return hd <= 64 ? &v64 : (hd <= 128 ? &v128 : (units <= 8 ? &few256 : &v256));
+    if (hd <= 64) return variant<KV, 64, 2, 1, 2, 3>();
+    if (hd <= 128) return variant<KV, 128, 1, 1, 2, KV == KC_Q8_0 ? 2 : 3>();
+    return units <= 8 ? variant<KV, 256, 1, 1, 2, 1>() : variant<KV, 256, 1, 1, 1, 2>();
 }
 
-static int attend_variant(const kc_paged_kv *kv, int n_heads, int n_seqs, const ServeDev &d, AttendVariant *&v, int &chunks) {
+static int attend_variant(const kc_paged_kv *kv, int n_heads, int n_seqs, const ServeDev &d, AttendVariant *&v, int &chunks, int &ctas) {
     const int group = n_heads / kv->n_kv_heads;
     const long long units = (long long)n_seqs * kv->n_kv_heads * ((group + 7) / 8);
     int mt = 1;
@@ -232,15 +231,17 @@ static int attend_variant(const kc_paged_kv *kv, int n_heads, int n_seqs, const 
                               : (kv->kv_type == KC_F16 ? variants_of<KC_F16>(kv->head_dim, group, units, mt)
                                                        : variants_of<KC_Q8_0>(kv->head_dim, group, units, mt));
     chunks = (group + 8 * mt - 1) / (8 * mt);
-    if (!v->ctas[d.dev]) {
+    ctas = v->ctas[d.dev].load(std::memory_order_acquire);
+    if (!ctas) {
         SK(cudaFuncSetAttribute((const void *)v->attend, cudaFuncAttributeMaxDynamicSharedMemorySize, v->smem), "attend");
         int n = 0;
         SK(cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, (const void *)v->attend, AT_THREADS, (size_t)v->smem), "attend");
-        if (n < 1) {
+        ctas = std::min(n * d.sms, AT_MAX_CTAS);
+        if (ctas < 1) {
             set_error("attend: no CTA fits an SM");
             return KC_E_IO;
         }
-        v->ctas[d.dev] = std::min(n * d.sms, AT_MAX_CTAS);
+        v->ctas[d.dev].store(ctas, std::memory_order_release);
     }
     return KC_OK;
 }
@@ -311,13 +312,13 @@ extern "C" int kc_paged_attend_ws(const kc_paged_kv *kv, int n_heads, size_t *by
     if (rc != KC_OK) return rc;
     ServeDev d;
     AttendVariant *v = nullptr;
-    int chunks = 0;
+    int chunks = 0, ctas = 0;
     rc = serve_device(d);
     size_t most = 0;
     for (int n : { 1, kv->n_seqs }) {                  /* calls of any number of sequences share it */
-        if (rc == KC_OK) rc = attend_variant(kv, n_heads, n, d, v, chunks);
+        if (rc == KC_OK) rc = attend_variant(kv, n_heads, n, d, v, chunks, ctas);
         if (rc != KC_OK) return rc;
-        most = std::max(most, ws_bytes(v, v->ctas[d.dev]));
+        most = std::max(most, ws_bytes(v, ctas));
     }
     *bytes = most;
     return KC_OK;
@@ -354,9 +355,9 @@ extern "C" int kc_paged_attend_dev(const kc_paged_kv *kv, const kc_attend_args *
     if (x->n_seqs == 0) return KC_OK;
     AttendArgs a{};
     AttendVariant *v = nullptr;
-    rc = attend_variant(kv, x->n_heads, x->n_seqs, d, v, a.chunks);
+    int ctas = 0;
+    rc = attend_variant(kv, x->n_heads, x->n_seqs, d, v, a.chunks, ctas);
     if (rc != KC_OK) return rc;
-    const int ctas = v->ctas[d.dev];
     const double quanta = (double)x->n_seqs * ((double)kv->ld_table * kv->page_size / (AT_WARPS * v->tile) + 2 + AT_UNIT_COST);
     if (quanta >= 2147483648.0 || quanta * kv->n_kv_heads * a.chunks / ctas >= 1073741824.0)
         return refuse("n_seqs sequences of ld_table * page_size positions are too many for one call");

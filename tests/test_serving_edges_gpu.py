@@ -68,3 +68,43 @@ def test_attend_8bit_weights_do_not_lose_bits_to_small_scales():
     top = 127 * 2.0 ** -100
     assert np.allclose(want / top, -1.28e-6, rtol=0.01)
     assert (np.abs(out.numpy() - want) <= 2.0 ** -20 * top).all()
+
+
+FIRST_USE = """
+import sys, threading
+sys.path[:0] = {paths!r}
+import numpy as np
+import krafla_b200 as kb
+kb.lib()
+n, heads, hk, hd, page = 3, 8, 2, 64, 16
+rng = np.random.default_rng(0)
+k, v = (kb.DevArray.of(rng.standard_normal((6, hk, page, hd)).astype(np.float16)) for _ in range(2))
+table = kb.DevArray.of(np.arange(6, dtype=np.int32).reshape(n, 2))
+q, lens = kb.DevArray.of(rng.standard_normal((n, heads, hd)).astype(np.float32)), kb.DevArray.of(np.array([5, 32, 17], np.int32))
+go, outs, errors = threading.Barrier(24), [None] * 24, []
+
+def first(i):
+    out = kb.DevArray(q.shape, np.float32)
+    go.wait()
+    try:
+        outs[i] = kb.PagedKV(k, v, table, kb.F16, n_heads=heads).attend(q, lens, out)
+    except Exception as e:
+        errors.append(e)
+
+ts = [threading.Thread(target=first, args=(i,)) for i in range(24)]
+[t.start() for t in ts]
+[t.join() for t in ts]
+kb._check(kb.lib().kc_dev_sync(), "sync")
+assert not errors, errors
+assert all(np.array_equal(o.numpy(), outs[0].numpy()) for o in outs)
+print("same")
+"""
+
+
+def test_first_use_by_many_threads():
+    """24 threads make a process's first calls at once, each with a handle of its own."""
+    import subprocess
+    import sys
+    for _ in range(3):
+        r = subprocess.run([sys.executable, "-c", FIRST_USE.format(paths=sys.path)], capture_output=True, text=True, timeout=300)
+        assert r.returncode == 0 and r.stdout.strip() == "same", r.stderr[-2000:]
