@@ -310,6 +310,7 @@ extern "C" int kc_paged_attend_ws(const kc_paged_kv *kv, int n_heads, size_t *by
     int rc = check_cache(kv);
     if (rc == KC_OK) rc = check_heads(kv, n_heads);
     if (rc != KC_OK) return rc;
+    if (!bytes) return refuse("bytes is NULL");
     ServeDev d;
     AttendVariant *v = nullptr;
     int chunks = 0, ctas = 0;
