@@ -108,3 +108,56 @@ def test_first_use_by_many_threads():
     for _ in range(3):
         r = subprocess.run([sys.executable, "-c", FIRST_USE.format(paths=sys.path)], capture_output=True, text=True, timeout=300)
         assert r.returncode == 0 and r.stdout.strip() == "same", r.stderr[-2000:]
+
+
+FIRST_IN_A_GRAPH = """
+import sys
+sys.path[:0] = {paths!r}
+import torch
+import krafla_b200 as kb
+n, heads, hk, hd, page, vocab = 3, 8, 2, 64, 16, 5000
+g = torch.Generator().manual_seed(0)
+k, v = (torch.randn(6, hk, page, hd, generator=g).half().cuda() for _ in range(2))
+table = torch.arange(6, dtype=torch.int32).reshape(n, 2).cuda()
+c = kb.PagedKV(k, v, table, kb.F16, n_heads=heads)
+cos, sin = (torch.from_numpy(t).cuda() for t in kb.rope_tables(dict(head_dim=hd, rope_theta=1e4), 32))
+x = torch.randn(n, (heads + 2 * hk) * hd, generator=g).cuda()
+pos = torch.tensor([5, 31, 16], dtype=torch.int32).cuda()
+lens = pos + 1
+q, o = torch.zeros(n, heads, hd).cuda(), torch.zeros(n, heads, hd).cuda()
+z = torch.randn(n, vocab, generator=g).cuda()
+y, w = torch.zeros_like(z), torch.zeros_like(z)
+mask = torch.randint(0, 2 ** 31, (n, (vocab + 31) // 32), generator=g, dtype=torch.int32).cuda()
+hist, rep = torch.randint(0, vocab, (n, 40), generator=g, dtype=torch.int32).cuda(), torch.full((n,), 1.5).cuda()
+kb.process_logits(w, z)                                       # a first call, of the plainest kind
+st = torch.cuda.Stream()
+
+def step():
+    c.append(x, pos, cos, sin, q, stream=st.cuda_stream)
+    c.attend(q, lens, o, stream=st.cuda_stream)
+    kb.process_logits(y, z, history=hist, repeat=rep, mask=mask, stream=st.cuda_stream)
+
+torch.cuda.synchronize()
+gr = torch.cuda.CUDAGraph()
+with torch.cuda.graph(gr, stream=st):
+    step()
+assert not q.any() and not o.any() and not y.any()
+gr.replay()
+torch.cuda.synchronize()
+got = [t.clone() for t in (q, o, y)]
+step()
+torch.cuda.synchronize()
+kb._check(kb.lib().kc_dev_sync(), "sync")
+assert all(torch.equal(a, b) for a, b in zip(got, (q, o, y))) and q.any() and o.any() and y.any()
+del gr
+print("same")
+"""
+
+
+def test_first_calls_inside_a_capture():
+    """A process that has made a PagedKV and one plain call of process_logits captures the rest unseen."""
+    pytest.importorskip("torch")
+    import subprocess
+    import sys
+    r = subprocess.run([sys.executable, "-c", FIRST_IN_A_GRAPH.format(paths=sys.path)], capture_output=True, text=True, timeout=300)
+    assert r.returncode == 0 and r.stdout.strip() == "same", r.stderr[-2000:]
