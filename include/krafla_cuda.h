@@ -172,7 +172,8 @@ int kc_generate_sampled(kc_state *s, kc_sampler *p, int token, int pos, int n, i
  * last repeat_last_n tokens. Each copies its host arrays and waits for the
  * state's stream.
  * presence, frequency: taken off a ring token's logit once, and once for each
- * time it is there (0, 0: off). */
+ * time it is there (0, 0: off; without a ring, repeat_last_n 0, they take
+ * nothing off, as repeat_penalty). */
 int kc_sampler_set_penalties(kc_sampler *p, float presence, float frequency);
 /* n biases added to tokens' logits, finite or -inf (the last for a token counts);
  * n 0: none. A token biased to -inf is not drawn as long as a logit above -inf
@@ -331,7 +332,9 @@ int kc_rope_tables(const kc_config *cfg, int n_pos, int local, float *cos_out, f
  * [head_dim] each; both NULL: none), x / sqrt(mean(x^2) + eps) * w, the rotation
  * of adjacent pairs at the row's position (cos and sin [n_pos][head_dim / 2],
  * the tables of kc_rope_tables), queries to q_out, keys and values into the
- * cache in its type (8-bit rows by the rule of the model's cache). Row i goes
+ * cache in its type (8-bit rows by the rule of the model's cache; their keys are
+ * normed and rotated in 64 bits, where a model's steps use 32, so that a value
+ * next to a rounding border may differ by one). Row i goes
  * to position pos[i] of sequence seqs[i] (seqs NULL: of sequence i); a negative
  * sequence is padding: nothing is written for it. q, k, v: rows of n_heads,
  * n_kv_heads, n_kv_heads heads, ld* floats apart (multiples of 4; views of one
@@ -355,7 +358,7 @@ int kc_paged_append_dev(const kc_paged_kv *kv, const kc_append_args *args, void 
  * against positions max(0, lens[i] - window) .. lens[i] - 1 (window 0: from 0)
  * of sequence i. scores q . k * scale, through softcap * tanh(score / softcap)
  * when softcap > 0; an 8-bit cache takes the query quantized per head, as the
- * model's does. A sequence of length 0 gets zeros. The sums of a row do not
+ * model's does. out and q do not overlap. A sequence of length 0 gets zeros. The sums of a row do not
  * depend on what else is running, but how a row is cut into pieces depends on
  * the other rows' lengths: results of different batches differ by float
  * rounding. ws: at least kc_paged_attend_ws bytes of scratch, 16-byte aligned,

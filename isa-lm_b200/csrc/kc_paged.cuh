@@ -279,13 +279,16 @@ __global__ void __launch_bounds__(AP_THREADS, KV == KC_Q8_0 ? (NV == 1 ? 4 : 3) 
  *
  * What bounds it: the cache's bytes, read once. 64 sequences of 2048..8192
  * positions (32 heads on 8, head 128, f16, 1.34 GB) 211 us in a long run, 6.4 TB/s,
- * what a copy reaches; 2 of 131072 176 us, 5.8 TB/s. Where the bytes are fewer the
- * arithmetic shows: splitting an f32 value takes four integer and float
- * instructions, an 8-bit one a fifth of a word's five (64 of 4096, head 64, 8-bit:
+ * what a copy reaches; 2 of 131072 177 us, 5.8 TB/s. Where the bytes are fewer the
+ * warps' own work shows: splitting an f32 value takes four integer and float
+ * instructions, an 8-bit one a fifth of a word's five, in chains that 12 warps an
+ * SM do not hide (0.36 instructions issued a cycle; 64 of 4096, head 64, 8-bit:
  * 61 us at a floor of 44, 65 in a long run; 32 of 2048, head 64, f32: 52 at 41, in
- * a long run 56). Small calls are bound by their chain of latencies, about 5.8 us
- * for one tile: launch, length, table, rows, products, the warps' meeting; a
- * joined unit 3 us more (of which its pieces' sums 1.5). */
+ * a long run 56). Where more than 8 heads share a KV head, f32 and heads above 128
+ * go over the rows once for every 8 (kc_serve.cu: the instances). Small calls are
+ * bound by their chain of latencies, about 6 us for one f32 tile (f16 4.3):
+ * launch, length, table, rows, products, the warps' meeting; a joined unit 3 us
+ * more (of which its pieces' sums 1.5). */
 constexpr int AT_WARPS = 4;
 constexpr int AT_THREADS = AT_WARPS * 32;
 /* Quanta of a unit that is not worth sharing out where every unit has a CTA of its own: of 5 quanta, 78 units 11.2 us
