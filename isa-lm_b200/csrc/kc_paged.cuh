@@ -286,9 +286,9 @@ __global__ void __launch_bounds__(AP_THREADS, KV == KC_Q8_0 ? (NV == 1 ? 4 : 3) 
  * 61 us at a floor of 44, 65 in a long run; 32 of 2048, head 64, f32: 52 at 41, in
  * a long run 56). Where more than 8 heads share a KV head, f32 and heads above 128
  * go over the rows once for every 8 (kc_serve.cu: the instances). Small calls are
- * bound by their chain of latencies, about 6 us for one f32 tile (f16 4.3):
- * launch, length, table, rows, products, the warps' meeting; a joined unit 3 us
- * more (of which its pieces' sums 1.5). */
+ * bound by their chain of latencies: 128 positions, head 64, f16 4.3 us (a tile a
+ * warp), f32 6.0 (two): launch, length, table, rows, products, the warps' meeting;
+ * a joined unit 3 us more (of which its pieces' sums 1.5). */
 constexpr int AT_WARPS = 4;
 constexpr int AT_THREADS = AT_WARPS * 32;
 /* Quanta of a unit that is not worth sharing out where every unit has a CTA of its own: of 5 quanta, 78 units 11.2 us
